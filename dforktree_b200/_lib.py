@@ -17,7 +17,7 @@ LIB_PATH = os.path.join(_HERE, "libdforktree_b200.so")
 DFT_F32, DFT_BF16, DFT_F16 = 0, 1, 2
 DFT_OK, DFT_ERR_INVALID, DFT_ERR_UNSUPPORTED = 0, 1, 2
 DFT_ERR_TABLE, DFT_ERR_IO = 4, 7
-DEV_BAD_TOKEN, DEV_PROBE_LIMIT, DEV_BAD_INDEX, DEV_TIMEOUT = 1, 2, 4, 8
+DEV_BAD_TOKEN, DEV_PROBE_LIMIT, DEV_BAD_INDEX, DEV_TIMEOUT, DEV_NO_PAGES = 1, 2, 4, 8, 16
 
 _DTYPES = {torch.float32: DFT_F32, torch.bfloat16: DFT_BF16, torch.float16: DFT_F16}
 
@@ -79,6 +79,35 @@ class TreeAttnArgs(C.Structure):
                 ("kv_indptr", vp), ("kv_indices", vp), ("anc", vp), ("anc_sb", i64),
                 ("sm_scale", f32), ("max_kv_len", i32),
                 ("o", vp), ("o_sb", i64), ("o_sn", i64), ("o_sh", i64)]
+
+
+class PagePlanArgs(C.Structure):
+    _fields_ = [("B", i32), ("page_size", i32), ("cached", vp), ("fresh", vp), ("rows", vp),
+                ("block_table", vp), ("bt_sr", i64), ("n_rows", i32), ("max_pages", i32), ("held", vp),
+                ("free_pages", vp), ("n_free", vp), ("n_pages", i32),
+                ("qo_indptr", vp), ("kv_indptr", vp), ("kv_indices", vp), ("kv_capacity", i64),
+                ("slot_map", vp), ("positions", vp), ("token_capacity", i64)]
+
+
+class KvAppendArgs(C.Structure):
+    _fields_ = [("T", i64), ("Hkv", i32), ("D", i32), ("dtype", i32),
+                ("k", vp), ("k_st", i64), ("k_sh", i64), ("v", vp), ("v_st", i64), ("v_sh", i64),
+                ("k_cache", vp), ("v_cache", vp), ("kv_st", i64), ("kv_sh", i64), ("n_slots", i64),
+                ("slot_map", vp)]
+
+
+class KvCommitArgs(C.Structure):
+    _fields_ = [("L", i32), ("B", i32), ("N", i32), ("P", i32), ("Hkv", i32), ("D", i32), ("dtype", i32),
+                ("k_cache", vp), ("v_cache", vp), ("kv_sl", i64), ("kv_st", i64), ("kv_sh", i64), ("n_slots", i64),
+                ("kv_indptr", vp), ("kv_indices", vp), ("n_kv", i64), ("path", vp), ("accept_len", vp)]
+
+
+class ChunkAttnArgs(C.Structure):
+    _fields_ = [("B", i32), ("T", i32), ("Hq", i32), ("Hkv", i32), ("D", i32), ("dtype", i32),
+                ("q", vp), ("q_st", i64), ("q_sh", i64),
+                ("k_cache", vp), ("v_cache", vp), ("kv_st", i64), ("kv_sh", i64), ("n_slots", i64),
+                ("qo_indptr", vp), ("kv_indptr", vp), ("kv_indices", vp), ("n_kv", i64),
+                ("sm_scale", f32), ("o", vp), ("o_st", i64), ("o_sh", i64)]
 
 
 class GdnConvArgs(C.Structure):
@@ -145,6 +174,11 @@ SIGNATURES = {
     "dft_conv_commit": (C.c_int, [C.POINTER(ConvCommitArgs), vp, vp]),
     "dft_tree_attn_workspace_bytes": (i64, [C.POINTER(TreeAttnArgs)]),
     "dft_tree_attn": (C.c_int, [C.POINTER(TreeAttnArgs), vp, vp, vp]),
+    "dft_page_plan": (C.c_int, [C.POINTER(PagePlanArgs), vp, vp]),
+    "dft_kv_append": (C.c_int, [C.POINTER(KvAppendArgs), vp, vp]),
+    "dft_kv_commit": (C.c_int, [C.POINTER(KvCommitArgs), vp, vp]),
+    "dft_chunk_attn_workspace_bytes": (i64, [C.POINTER(ChunkAttnArgs)]),
+    "dft_chunk_attn": (C.c_int, [C.POINTER(ChunkAttnArgs), vp, vp, vp]),
     "dft_gdn_tree_verify": (C.c_int, [C.POINTER(GdnArgs), vp, vp]),
     "dft_gdn_commit": (C.c_int, [C.POINTER(CommitArgs), vp, vp]),
 }

@@ -16,7 +16,9 @@ State layout in HBM (one GPU holds whole requests; requests shard across GPUs):
   aux_g     [L, B, Hv, N]     fp32    ancestor-cumulative gates
   k_cache / v_cache [La, slots, Hkv, Da] bf16   per attention layer, page size 1:
             request b's keys are slots kv_indices[kv_indptr[b]:kv_indptr[b+1]],
-            its prefix first and its N tree tokens last
+            its prefix first and its N tree tokens last.  With page_size > 0
+            the caches, their page tables and these maps are a PagedKV's: filled
+            by extend(), planned per step, compacted by commit()
 """
 from __future__ import annotations
 
@@ -47,6 +49,10 @@ class CycleConfig:
     Hkv: int = 4
     Da: int = 256
     prefix: int = 4096    # prior context per request in the KV cache
+    # 0: a fixed random prefix per request (page size 1); otherwise the caches are
+    # paged, start empty, are filled by extend() and grow by each step's accepted path
+    page_size: int = 0
+    max_len: int = 0      # longest request in tokens, its tree included (0: prefix + 16 P + N)
 
     @property
     def layer_kinds(self):
@@ -114,6 +120,18 @@ class DraftTreeCycle:
         tree's ancestor matrix from its buffer at every run."""
         from .tree_attn import TreeAttentionWrapper
         c, dev = self.cfg, self.device
+        self.o_attn = torch.empty(c.B, c.N, c.Hq, c.Da, dtype=torch.bfloat16, device=dev)
+        if c.page_size:
+            from .paged_kv import PagedKV
+            self.kv = PagedKV(c.B, c.max_len or c.prefix + 16 * c.P + c.N, c.attn_layers, c.Hkv, c.Da,
+                              page_size=c.page_size, device=dev)
+            self.kv.status = self.status
+            self.kv_len = torch.zeros(c.B, dtype=torch.int64, device=dev)      # tokens in the caches
+            self.tree_fresh = torch.full((c.B,), c.N, dtype=torch.int64, device=dev)
+            self.tree_maps = self.kv.maps = self.kv.outputs(c.B, c.B * c.N)
+            self.attn = self.kv.tree(self.tree["anc"], c.Hq)
+            self.launches_per_step += 2 + c.attn_layers * 3 + 1
+            return
         keys = c.prefix + c.N
         slots = c.B * keys
         self.kv_indices = torch.randperm(slots, device=dev, generator=g).to(torch.int32)
@@ -126,7 +144,6 @@ class DraftTreeCycle:
         self.attn = TreeAttentionWrapper(dev).plan(self.kv_indptr, self.kv_indices, c.Hq, c.Hkv, c.Da, n=c.N,
                                                    anc=self.tree["anc"], kv_lens_host=[keys] * c.B)
         self.attn.status = self.status
-        self.o_attn = torch.empty(c.B, c.N, c.Hq, c.Da, dtype=torch.bfloat16, device=dev)
         self.launches_per_step += c.attn_layers * 2
 
     # -- stages --------------------------------------------------------------
@@ -135,10 +152,39 @@ class DraftTreeCycle:
         K.score_build(self.table, logits, root, pre1, c.N, self.ws, self.tree, chain_first=c.chain_first,
                       lam_a=c.lam_a, lam_p=c.lam_p, status=self.status)
 
-    def attend_layer(self, j, q):
+    def extend(self, fresh, q, k, v):
+        """Prompt tokens through the paged caches of the attention layers (page_size > 0):
+        fresh [B] new tokens per request (int64), packed in request order in
+        q [La, T, Hq, Da] and k, v [La, T, Hkv, Da] (T >= sum(fresh)).  Returns
+        o [La, T, Hq, Da]; its rows past the last request's are zero."""
+        c = self.cfg
+        if not c.page_size or not c.attn_layers:
+            raise K.L.DFTError("extend needs attention layers and page_size > 0")
+        o = torch.zeros_like(q, memory_format=torch.contiguous_format)
+        self.kv.plan(self.kv_len, fresh, tokens=q.shape[1])
+        for j in range(c.attn_layers):
+            self.kv.append(j, k[j], v[j])
+            self.kv.attend(j, q[j], o=o[j])
+        self.kv_len += self._planned_tokens(self.kv.maps)
+        return o
+
+    @staticmethod
+    def _planned_tokens(maps):
+        """New tokens per request of a plan: none where it could not be made."""
+        return maps["qo_indptr"][1:] - maps["qo_indptr"][:-1]
+
+    def plan_tree(self):
+        """Pages and maps for this step's N tree tokens per request (paged caches)."""
+        self.kv.plan(self.kv_len, self.tree_fresh, out=self.tree_maps)
+
+    def attend_layer(self, j, q, k=None, v=None):
         """Tree-masked attention verify of attention layer j: q [B, N, Hq, Da]
         against the request's prefix and its tree keys (mask of
-        fc1_branch64.py:39); output in self.o_attn."""
+        fc1_branch64.py:39); output in self.o_attn.  Paged caches take the
+        tree's k, v [B, N, Hkv, Da] first."""
+        if self.cfg.page_size:
+            self.kv.append(j, k.flatten(0, 1), v.flatten(0, 1))
+            return self.attn.run(q, (self.kv.k_cache[j], self.kv.v_cache[j]), out=self.o_attn)
         return self.attn.run(q, (self.k_cache[j], self.v_cache[j]), out=self.o_attn)
 
     def verify_layer(self, l, x, a, b):
@@ -174,25 +220,33 @@ class DraftTreeCycle:
                      self.last.view(-1, 1), c.Hk, c.Hv, aux_k_per_v=False, status=self.status)
         if x is not None:
             K.conv_commit(x, self.conv_state, self.tree["cidx"], self.last, status=self.status)
+        if c.attn_layers and c.page_size:
+            self.kv.maps = self.tree_maps
+            self.kv.commit(self.path, self.accept_len, c.N)
+            self.kv_len += torch.minimum(self.accept_len.clamp(max=c.P), self._planned_tokens(self.tree_maps))
 
-    def verify(self, x, a, b, q=None):
+    def verify(self, x, a, b, q=None, k=None, v=None):
         """Every layer in model order: tree conv + GDN verify per GDN layer
         (each launch overlapping the previous layer's tail), tree attention
-        per attention layer (q [La, B, N, Hq, Da])."""
+        per attention layer (q [La, B, N, Hq, Da]; with paged caches also the
+        tree tokens' k, v [La, B, N, Hkv, Da])."""
         l = j = 0
+        if self.cfg.attn_layers and self.cfg.page_size:
+            self.plan_tree()
         for kind in self.cfg.layer_kinds:
             if kind == "gdn":
                 self.verify_layer(l, x[l], a[l], b[l])
                 l += 1
             else:
-                self.attend_layer(j, q[j])
+                self.attend_layer(j, q[j], None if k is None else k[j], None if v is None else v[j])
                 j += 1
 
-    def step(self, logits, root, pre1, x, a, b, target_fn, q=None):
+    def step(self, logits, root, pre1, x, a, b, target_fn, q=None, k=None, v=None):
         """One cycle.  x [L, B, N, C], a / b [L, B, N, Hv]; q [La, B, N, Hq, Da]
-        when the cycle has attention layers; target_fn(tree) -> the target
-        model's token per node [B, N] (int64)."""
+        when the cycle has attention layers, and k, v [La, B, N, Hkv, Da] when
+        their caches are paged; target_fn(tree) -> the target model's token
+        per node [B, N] (int64)."""
         self.build(logits, root, pre1)
-        self.verify(x, a, b, q)
+        self.verify(x, a, b, q, k, v)
         self.accept(target_fn(self.tree))
         self.commit(x)

@@ -516,3 +516,183 @@ def tree_attention(q, k_cache, v_cache, kv_indptr, kv_indices, anc, max_kv_len=N
                               L.stream_handle()), "dft_tree_attn")
     del keep
     return o
+
+
+# --------------------------------------------------------- paged KV cache --
+def _on_current_device(what, *tensors):
+    """Every tensor on the current CUDA device (the stream's)."""
+    cur = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != cur:
+            raise L.DFTError(f"{what}: every tensor must be on the current CUDA device (cuda:{cur}), got one on "
+                             f"{t.device}")
+
+
+def _want(what, ok, msg):
+    if not ok:
+        raise L.DFTError(f"{what}: {msg}")
+
+
+def _stride(t, d):
+    """Element stride of dim d; of a dim of size 1, whose stride means nothing,
+    that of a contiguous tensor."""
+    if t.shape[d] != 1:
+        return t.stride(d)
+    n = 1
+    for size in t.shape[d + 1:]:
+        n *= size
+    return n
+
+
+def _ids(t, dtype):
+    return t if t.dtype is dtype and t.is_contiguous() else t.to(dtype).contiguous()
+
+
+def _cache_pair(what, k_cache, v_cache):
+    _want(what, v_cache.shape == k_cache.shape and v_cache.stride() == k_cache.stride() and
+          v_cache.dtype is k_cache.dtype, "k_cache and v_cache must have one shape, dtype and set of strides")
+    _want(what, k_cache.shape[-1] <= 1 or k_cache.stride(-1) == 1, "the cache's head dim must be contiguous")
+
+
+def page_plan_outputs(B, tokens, keys, device):
+    """Buffers that page_plan writes: `tokens` new tokens and `keys` keys at most."""
+    return dict(qo_indptr=torch.empty(B + 1, dtype=torch.int32, device=device),
+                kv_indptr=torch.empty(B + 1, dtype=torch.int32, device=device),
+                kv_indices=torch.empty(keys, dtype=torch.int32, device=device),
+                slot_map=torch.empty(tokens, dtype=torch.int64, device=device),
+                positions=torch.empty(tokens, dtype=torch.int64, device=device))
+
+
+def page_plan(cached, fresh, block_table, held, free_pages, n_free, page_size, rows=None, out=None, tokens=None,
+              status=None):
+    """Page tables grown or shrunk to cached + fresh tokens per request, and
+    the maps made of them (dft_page_plan).
+
+    cached, fresh [B] int64; rows [B] int64 (None: row b), each at most once;
+    block_table [R, max_pages], held [R], free_pages [n_pages], n_free [1], all
+    int32, updated in place.  out: the buffers of page_plan_outputs (their
+    sizes are the capacities); or tokens, a host bound on sum(fresh), to have
+    them made, with room for every slot of the cache.  Returns out.  A plan
+    that cannot be made changes no page and yields empty offsets; `status`
+    [1] int32 takes the reason."""
+    w = "page_plan"
+    B = cached.numel()
+    n_pages = free_pages.numel()
+    _want(w, fresh.numel() == B and (rows is None or rows.numel() == B), "cached, fresh and rows hold B entries each")
+    _want(w, block_table.dim() == 2 and (block_table.shape[1] <= 1 or block_table.stride(1) == 1),
+          "block_table is [rows, max_pages], its pages contiguous")
+    _want(w, block_table.dtype is torch.int32 and held.dtype is torch.int32 and free_pages.dtype is torch.int32 and
+          n_free.dtype is torch.int32, "block_table, held, free_pages and n_free are int32")
+    _want(w, held.is_contiguous() and free_pages.is_contiguous() and held.numel() == block_table.shape[0] and
+          n_free.numel() == 1, "held [rows] and free_pages are contiguous, n_free holds one count")
+    _want(w, rows is not None or B <= block_table.shape[0], "more requests than table rows")
+    if out is None:
+        _want(w, tokens is not None, "pass out, or tokens (a bound on the new tokens)")
+        out = page_plan_outputs(B, int(tokens), n_pages * int(page_size), block_table.device)
+    qo, kv, idx, slots, pos = (out[k] for k in ("qo_indptr", "kv_indptr", "kv_indices", "slot_map", "positions"))
+    _want(w, qo.dtype is torch.int32 and kv.dtype is torch.int32 and idx.dtype is torch.int32 and
+          slots.dtype is torch.int64 and pos.dtype is torch.int64, "out: offsets and indices int32, the rest int64")
+    _want(w, qo.numel() == B + 1 and kv.numel() == B + 1 and pos.numel() == slots.numel() and
+          qo.is_contiguous() and kv.is_contiguous() and idx.is_contiguous() and slots.is_contiguous() and
+          pos.is_contiguous(), "out: contiguous, offsets of B + 1 entries, slot_map and positions alike")
+    lib = L.lib()
+    _on_current_device(w, cached, fresh, rows, block_table, held, free_pages, n_free, qo, kv, idx, slots, pos, status)
+    cached, fresh = _ids(cached, torch.int64), _ids(fresh, torch.int64)
+    rows = None if rows is None else _ids(rows, torch.int64)
+    a = L.PagePlanArgs(B, int(page_size), cached.data_ptr(), fresh.data_ptr(), L.ptr(rows), block_table.data_ptr(),
+                       _stride(block_table, 0), block_table.shape[0], block_table.shape[1], held.data_ptr(),
+                       free_pages.data_ptr(), n_free.data_ptr(), n_pages, qo.data_ptr(), kv.data_ptr(),
+                       idx.data_ptr(), idx.numel(), slots.data_ptr(), pos.data_ptr(), slots.numel())
+    L.check(lib.dft_page_plan(C.byref(a), _status_ptr(status), L.stream_handle()), "dft_page_plan")
+    return out
+
+
+def kv_append(k, v, k_cache, v_cache, slot_map, status=None):
+    """cache[slot_map[t]] = k[t], v[t]: k, v [T, Hkv, D] (any token and head
+    strides), k_cache / v_cache [slots, Hkv, D], slot_map [T] (negative: the row
+    is skipped; otherwise distinct).  16-bit types, in place."""
+    w = "kv_append"
+    T, Hkv, D = k.shape
+    _want(w, v.shape == k.shape and k_cache.dim() == 3 and tuple(k_cache.shape[1:]) == (Hkv, D) and
+          slot_map.numel() == T, "k, v [T, Hkv, D], caches [slots, Hkv, D], slot_map [T]")
+    _cache_pair(w, k_cache, v_cache)
+    _want(w, k.dtype is v.dtype and k.dtype is k_cache.dtype and k.dtype in (torch.bfloat16, torch.float16),
+          "k, v and the caches must be alike bfloat16 or float16")
+    _want(w, D <= 1 or (k.stride(2) == 1 and v.stride(2) == 1), "the head dim of k and v must be contiguous")
+    lib = L.lib()
+    _on_current_device(w, k, v, k_cache, v_cache, slot_map, status)
+    slot_map = _ids(slot_map, torch.int64)
+    a = L.KvAppendArgs(T, Hkv, D, L.dtype_code(k), k.data_ptr(), _stride(k, 0), _stride(k, 1), v.data_ptr(),
+                       _stride(v, 0), _stride(v, 1), k_cache.data_ptr(), v_cache.data_ptr(), _stride(k_cache, 0),
+                       _stride(k_cache, 1), k_cache.shape[0], slot_map.data_ptr())
+    L.check(lib.dft_kv_append(C.byref(a), _status_ptr(status), L.stream_handle()), "dft_kv_append")
+
+
+def kv_commit(k_cache, v_cache, kv_indptr, kv_indices, path, accept_len, N, status=None):
+    """Accepted tree rows to the tree's first positions, in place: k_cache /
+    v_cache [slots, Hkv, D] or [layers, slots, Hkv, D]; the last N keys of each
+    request are its tree; path [B, P] and accept_len [B] as accept_greedy
+    returns them."""
+    w = "kv_commit"
+    _cache_pair(w, k_cache, v_cache)
+    if k_cache.dim() == 3:
+        k_cache, v_cache = k_cache.unsqueeze(0), v_cache.unsqueeze(0)
+    _want(w, k_cache.dim() == 4 and path.dim() == 2, "caches [layers, slots, Hkv, D], path [B, P]")
+    Ln, slots, Hkv, D = k_cache.shape
+    B, P = path.shape
+    _want(w, accept_len.numel() == B and kv_indptr.numel() == B + 1, "accept_len [B], kv_indptr [B + 1]")
+    lib = L.lib()
+    _on_current_device(w, k_cache, v_cache, kv_indptr, kv_indices, path, accept_len, status)
+    kv_indptr, kv_indices = _ids(kv_indptr, torch.int32), _ids(kv_indices, torch.int32)
+    path, accept_len = _ids(path, torch.int64), _ids(accept_len, torch.int64)
+    a = L.KvCommitArgs(Ln, B, int(N), P, Hkv, D, L.dtype_code(k_cache), k_cache.data_ptr(), v_cache.data_ptr(),
+                       _stride(k_cache, 0), _stride(k_cache, 1), _stride(k_cache, 2), slots, kv_indptr.data_ptr(),
+                       kv_indices.data_ptr(), kv_indices.numel(), path.data_ptr(), accept_len.data_ptr())
+    L.check(lib.dft_kv_commit(C.byref(a), _status_ptr(status), L.stream_handle()), "dft_kv_commit")
+
+
+def chunk_attention(q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, sm_scale=None, o=None, workspace=None,
+                    status=None):
+    """Causal attention of new tokens over the paged cache (dft_chunk_attn):
+    q [T, Hq, D] packed, request b's rows q[qo_indptr[b]:qo_indptr[b+1]] and
+    keys kv_indices[kv_indptr[b]:kv_indptr[b+1]], its new tokens' keys last;
+    k_cache / v_cache [slots, Hkv, D].  bfloat16 or float16, D in {64, 128,
+    256}.  Returns o [T, Hq, D]; rows of q outside every request are not
+    written (pass o to keep what they hold).  workspace: uint8, at least
+    dft_chunk_attn_workspace_bytes, for this call alone; made here if None."""
+    w = "chunk_attention"
+    T, Hq, D = q.shape
+    _want(w, k_cache.dim() == 3 and k_cache.shape[2] == D, "q [T, Hq, D], caches [slots, Hkv, D]")
+    _cache_pair(w, k_cache, v_cache)
+    _want(w, q.dtype is k_cache.dtype and q.dtype in (torch.bfloat16, torch.float16),
+          "q and the caches must be alike bfloat16 or float16")
+    _want(w, q.stride(2) == 1, "the head dim of q must be contiguous")
+    if o is None:
+        o = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
+    else:
+        _want(w, o.shape == q.shape and o.dtype is q.dtype and o.stride(2) == 1,
+              "o must be [T, Hq, D] of q's type, its head dim contiguous")
+    B = qo_indptr.numel() - 1
+    _want(w, B >= 0 and kv_indptr.numel() == B + 1, "qo_indptr and kv_indptr hold B + 1 offsets each")
+    lib = L.lib()
+    _on_current_device(w, q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, o, workspace, status)
+    qo_indptr, kv_indptr = _ids(qo_indptr, torch.int32), _ids(kv_indptr, torch.int32)
+    kv_indices = _ids(kv_indices, torch.int32)
+    a = L.ChunkAttnArgs(B, T, Hq, k_cache.shape[1], D, L.dtype_code(q), q.data_ptr(), _stride(q, 0), _stride(q, 1),
+                        k_cache.data_ptr(), v_cache.data_ptr(), _stride(k_cache, 0), _stride(k_cache, 1),
+                        k_cache.shape[0], qo_indptr.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(),
+                        kv_indices.numel(), float(D ** -0.5 if sm_scale is None else sm_scale), o.data_ptr(),
+                        _stride(o, 0), _stride(o, 1))
+    need = lib.dft_chunk_attn_workspace_bytes(C.byref(a))
+    if need < 0:
+        raise L.DFTError("chunk_attention: outside what the kernel takes (D in {64, 128, 256}, Hq a multiple of Hkv "
+                         "with at most 128 q-heads each, at most 1024 requests, 16-byte aligned rows, sm_scale > 0)")
+    if need > 0:
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        else:
+            _want(w, workspace.is_contiguous() and workspace.numel() * workspace.element_size() >= need,
+                  f"workspace needs {need} contiguous bytes")
+    L.check(lib.dft_chunk_attn(C.byref(a), workspace.data_ptr() if need else None, _status_ptr(status),
+                               L.stream_handle()), "dft_chunk_attn")
+    return o

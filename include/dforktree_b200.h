@@ -44,7 +44,8 @@ enum {
   DFT_DEV_BAD_TOKEN = 1,    /* token id outside [-V, V)                    */
   DFT_DEV_PROBE_LIMIT = 2,  /* hash probe ran over the whole table         */
   DFT_DEV_BAD_INDEX = 4,    /* node / conv column / slot index out of range */
-  DFT_DEV_TIMEOUT = 8       /* a bounded wait gave up                      */
+  DFT_DEV_TIMEOUT = 8,      /* a bounded wait gave up                      */
+  DFT_DEV_NO_PAGES = 16     /* fewer free pages than a plan needs          */
 };
 typedef enum { DFT_F32 = 0, DFT_BF16 = 1, DFT_F16 = 2 } dft_dtype;
 
@@ -352,6 +353,123 @@ typedef struct {
 } dft_tree_attn_args;
 DFT_API int64_t dft_tree_attn_workspace_bytes(const dft_tree_attn_args* a);
 DFT_API int dft_tree_attn(const dft_tree_attn_args* a, void* workspace, int32_t* dev_status, void* stream);
+
+/* ------------------------------------------------------ paged KV cache -- */
+/* The serving stack's side of the attention layers' cache, which the plugin
+ * leaves to SGLang (req_to_token rows, out_cache_loc, the verify plan's
+ * kv_indptr / kv_indices of fc1_plan.py:16-33): page tables grown and shrunk
+ * from request lengths, new K / V rows written, causal attention of new
+ * tokens over the cache, and the accepted path's rows compacted.
+ *
+ * A cache is [n_slots, Hkv, D]; page p of page_size tokens is the slots
+ * [p * page_size, (p + 1) * page_size).
+ *
+ * dft_page_plan brings every request b of the call to cached[b] + fresh[b]
+ * tokens.  Its table row r = rows[b] then holds need = ceil(tokens /
+ * page_size) pages: first, requests in order push their pages need ..
+ * held[r]-1 (ascending) on the free stack free_pages[0 .. *n_free); then,
+ * requests in order, pages held[r] .. need-1 (ascending) pop its top.  held
+ * and *n_free follow; 0 + 0 tokens give a finished request's pages back.
+ * Entries of the stack's array at and above *n_free keep what they held or
+ * were pushed.  Written besides:
+ *   qo_indptr [B+1]  offsets of the requests' new tokens
+ *   kv_indptr [B+1]  offsets of the requests' keys (cached, then new)
+ *   kv_indices       slot of every key: what dft_tree_attn and
+ *                    dft_chunk_attn read; entries past the last key are left
+ *   slot_map, positions [token_capacity]  slot and position of every new
+ *                    token; -1 and 0 past the last (dft_kv_append skips -1)
+ * A plan that cannot be made changes no table, stack or count: the offsets
+ * become 0 and every slot -1, and dev_status takes DFT_DEV_NO_PAGES (stack
+ * too short) or DFT_DEV_BAD_INDEX (a negative length, cached tokens beyond
+ * the pages held, a row out of range or named twice, a length beyond
+ * max_pages, keys or tokens beyond their capacities, inconsistent counts).
+ * The row pitch bt_sr is in elements.  B <= 1024; page_size a power of two
+ * up to 1024; n_pages * page_size < 2^31.  B = 0 only clears slot_map and
+ * positions and writes the two zero offsets. */
+typedef struct {
+  int32_t B, page_size;
+  const int64_t* cached;          /* [B] tokens in the cache                */
+  const int64_t* fresh;           /* [B] tokens this step appends           */
+  const int64_t* rows;            /* [B] table row of request b; NULL: b    */
+  int32_t* block_table; int64_t bt_sr;          /* [n_rows, max_pages]      */
+  int32_t n_rows, max_pages;
+  int32_t* held;                  /* [n_rows] pages each row holds          */
+  int32_t* free_pages;            /* [n_pages] stack                        */
+  int32_t* n_free;                /* [1]                                    */
+  int32_t n_pages;
+  int32_t* qo_indptr;
+  int32_t* kv_indptr;
+  int32_t* kv_indices; int64_t kv_capacity;
+  int64_t* slot_map; int64_t* positions; int64_t token_capacity;
+} dft_page_plan_args;
+DFT_API int dft_page_plan(const dft_page_plan_args* a, int32_t* dev_status, void* stream);
+
+/* K / V rows of T new tokens into their slots: cache[slot_map[t], h, :] =
+ * k[t, h, :], for K and V.  A negative slot writes nothing (padding rows); one
+ * at or above n_slots writes nothing and sets DFT_DEV_BAD_INDEX.  Slots are
+ * distinct: of a slot named twice each piece takes one of the two rows.
+ * 16-bit elements (bfloat16 or float16, k / v / caches alike); head dim
+ * contiguous, any other strides. */
+typedef struct {
+  int64_t T;
+  int32_t Hkv, D, dtype;
+  const void* k; int64_t k_st, k_sh;            /* [T, Hkv, D]              */
+  const void* v; int64_t v_st, v_sh;
+  void* k_cache; void* v_cache;                 /* [n_slots, Hkv, D]        */
+  int64_t kv_st, kv_sh, n_slots;
+  const int64_t* slot_map;        /* [T]                                    */
+} dft_kv_append_args;
+DFT_API int dft_kv_append(const dft_kv_append_args* a, int32_t* dev_status, void* stream);
+
+/* After acceptance: the K / V rows of the accepted path take the tree's first
+ * positions, in every layer's cache.  The last N keys of request b (in
+ * kv_indices[kv_indptr[b] .. kv_indptr[b+1])) are its tree nodes; for i <
+ * min(accept_len[b], P), up to the first negative entry, the row of node
+ * path[b, i] is copied to the row of tree position i, in place.  path ascends
+ * strictly (a child's id is above its parent's, as dft_accept_greedy returns
+ * it): a path that does not, a node outside [0, N), a slot out of range or
+ * offsets that do not hold N keys leave the request unchanged and set
+ * DFT_DEV_BAD_INDEX. */
+typedef struct {
+  int32_t L, B, N, P, Hkv, D, dtype;
+  void* k_cache; void* v_cache;                 /* [L, n_slots, Hkv, D]     */
+  int64_t kv_sl, kv_st, kv_sh, n_slots;
+  const int32_t* kv_indptr; const int32_t* kv_indices; int64_t n_kv;  /* n_kv: entries of kv_indices */
+  const int64_t* path;            /* [B, P]                                 */
+  const int64_t* accept_len;      /* [B]                                    */
+} dft_kv_commit_args;
+DFT_API int dft_kv_commit(const dft_kv_commit_args* a, int32_t* dev_status, void* stream);
+
+/* Causal attention of new tokens over the paged cache.  Request b's new
+ * tokens are the rows [qo_indptr[b], qo_indptr[b+1]) of q, n of them, and its
+ * keys kv_indices[kv_indptr[b] .. kv_indptr[b+1]), L of them, the new tokens'
+ * own last: for token i of the n and q-head hq
+ *   o = softmax_j(q . k[j, hq/G] * sm_scale) . v[j, hq/G] over j <= L - n + i
+ * with G = Hq / Hkv.  A token that sees no key (L < n) gets 0; rows of q
+ * outside every request are left as they were in o.  Every length is read on
+ * the device, so a captured call follows its plan's buffers.  Values at keys
+ * that a token does not see do not reach its row, whatever they are.
+ * q, caches and o alike bfloat16 or float16; fp32 scores, softmax and sums,
+ * P rounded to the type for the second product.  D in {64, 128, 256}; G <=
+ * 128; rows and strides 16-byte aligned; B <= 1024; sm_scale > 0.
+ * Offsets outside [0, T] / [0, n_kv] or descending leave the request's rows
+ * unwritten and set DFT_DEV_BAD_INDEX; a slot outside [0, n_slots) sets it
+ * too and leaves that request's result unspecified.  o overlaps no input.
+ * workspace: dft_chunk_attn_workspace_bytes bytes, 16-byte aligned (0: none),
+ * used by this call alone while it runs. */
+typedef struct {
+  int32_t B, T, Hq, Hkv, D, dtype;
+  const void* q; int64_t q_st, q_sh;            /* [T, Hq, D]               */
+  const void* k_cache; const void* v_cache;     /* [n_slots, Hkv, D]        */
+  int64_t kv_st, kv_sh, n_slots;
+  const int32_t* qo_indptr;       /* [B + 1]                                */
+  const int32_t* kv_indptr;       /* [B + 1]                                */
+  const int32_t* kv_indices; int64_t n_kv;
+  float sm_scale;
+  void* o; int64_t o_st, o_sh;                  /* [T, Hq, D]               */
+} dft_chunk_attn_args;
+DFT_API int64_t dft_chunk_attn_workspace_bytes(const dft_chunk_attn_args* a);
+DFT_API int dft_chunk_attn(const dft_chunk_attn_args* a, void* workspace, int32_t* dev_status, void* stream);
 
 #ifdef __cplusplus
 }
