@@ -61,25 +61,29 @@ def chunk_attention(q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, scale
     o = np.full((T, Hq, D), np.nan)
     bound = np.zeros((T, Hq, D))
     for b in range(len(qo_indptr) - 1):
-        rows = range(qo_indptr[b], qo_indptr[b + 1])
+        t0, t1 = int(qo_indptr[b]), int(qo_indptr[b + 1])
         idx = np.asarray(kv_indices[kv_indptr[b]:kv_indptr[b + 1]], np.int64)
-        n, L = len(rows), len(idx)
-        for i, t in enumerate(rows):
-            seen = idx[:max(0, L - n + i + 1)]
-            if not len(seen):
-                o[t] = 0.0
-                continue
-            for h in range(Hq):
-                k, v = kc[seen, h // G], vc[seen, h // G]
-                s = (k @ q[t, h]) * scale
-                w = np.exp(s - s.max())
-                w /= w.sum()
-                o[t, h] = w @ v
-                if bound_unit is not None:
-                    A = w @ np.abs(v)
-                    ds = D * 2.0 ** -23 * scale * (np.abs(k) @ np.abs(q[t, h])).max()
-                    bound[t, h] = 1.01 * (bound_unit * np.abs(o[t, h]) + bound_unit * A + 2 * (ds + 2.0 ** -20) * A +
-                                          len(seen) * (2.0 ** -23 * A + 2.0 ** -31 * np.abs(v).max()))
+        n, L = t1 - t0, len(idx)
+        if n == 0:
+            continue
+        seen = np.arange(L)[None, :] <= (L - n + np.arange(n))[:, None]      # [n, L]
+        some = seen.any(1)
+        o[t0:t1][~some] = 0.0
+        if not some.any():
+            continue
+        seen, rows = seen[some], t0 + np.nonzero(some)[0]
+        for h in range(Hq):
+            k, v, qh = kc[idx, h // G], vc[idx, h // G], q[rows, h]
+            s = np.where(seen, (qh @ k.T) * scale, -np.inf)
+            w = np.exp(s - s.max(1, keepdims=True))
+            w /= w.sum(1, keepdims=True)
+            o[rows, h] = w @ v
+            if bound_unit is not None:
+                A = w @ np.abs(v)
+                ds = D * 2.0 ** -23 * scale * np.where(seen, np.abs(qh) @ np.abs(k).T, 0.0).max(1)[:, None]
+                bound[rows, h] = 1.01 * (bound_unit * np.abs(o[rows, h]) + bound_unit * A +
+                                         2 * (ds + 2.0 ** -20) * A +
+                                         seen.sum(1)[:, None] * (2.0 ** -23 * A + 2.0 ** -31 * np.abs(v).max()))
     return (o, bound) if bound_unit is not None else o
 
 

@@ -324,6 +324,12 @@ BF, HF = torch.bfloat16, torch.float16
     ([0, 5, 0, 1, 0], [10, 3, 0, 200, 64], 16, 4, 256, BF, 16),   # requests that bring nothing
     ([300], [700], 4, 1, 256, BF, 16),
     ([190], [2500], 4, 2, 128, HF, 16),
+    # several long units to a CTA, masked tiles far apart
+    ([1] * 40, list(range(2000, 4000, 50)), 16, 4, 256, BF, 16),
+    ([1] * 70, [1500 + 13 * b for b in range(70)], 32, 8, 128, HF, 16),
+    ([1, 250, 1, 1, 1, 40] * 3, [1900] * 18, 16, 2, 128, BF, 16),
+    ([700, 650, 1, 900], [0, 300, 1700, 20], 16, 8, 64, BF, 16),
+    ([1500], [100], 16, 8, 256, BF, 64),
 ])
 def test_attention_within_the_derived_bound(fresh, cached, Hq, Hkv, D, dtype, page):
     c = _attn_case(fresh, cached, Hq, Hkv, D, dtype, page)
@@ -484,6 +490,13 @@ def test_the_same_call_twice_and_on_another_stream():
     s.synchronize()
     torch.cuda.synchronize()
     assert torch.equal(a, b) and torch.equal(a, d)
+
+
+def test_a_workspace_that_is_too_small_is_refused():
+    from dforktree_b200 import _lib as L
+    c = _attn_case([1], [300], 4, 1, 256, BF)
+    with pytest.raises(L.DFTError):
+        _attend(c, workspace=torch.empty(64, dtype=torch.uint8, device=DEV))
 
 
 # -------------------------------------------------------------- together --
