@@ -8,8 +8,11 @@
 // + head) and one tcgen05 MMA of M = 128 serves them all; a single token's G
 // rows go through the same tile, whose spare rows cost no memory traffic.  Per
 // tile of KT keys, one pass with a running maximum and sum:
-//   K, V  gathered by slot with TMA (tile::gather4: four cache rows x 64 dims a
-//         copy), separate rings of stages for K and V, one producer warp
+//   K, V  by slot, 16 keys at a time, into separate rings of stages by three
+//         producer warps: where the 16 slots are consecutive (pages of 16 and
+//         more) one TMA box of 16 cache rows x 64 dims per copy, else 16-byte
+//         cp.async row by row (a gather of four rows per TMA copy took 39 ns a
+//         copy, 5 us per 64 KB tile)
 //   S     = Q K^T    kind::f16, A = Q from TMEM, M=128 N=KT K=D, fp32 in TMEM
 //   P     = 2^(S sm_scale log2e - m), two threads per row; the reference m
 //         moves (and O is rescaled in TMEM) only when the maximum grows by
@@ -26,8 +29,8 @@
 // share's border leaves partials (O, m, l) that a second kernel merges.
 //
 // Tiles past a row's last key hold the masked keys' values: their P is 0, but 0
-// times NaN or infinity is not.  In those tiles alone two checker warps zero
-// the rows past the request's end and every non-finite element before the P V
+// times NaN or infinity is not.  In those tiles alone the softmax threads zero
+// V's rows past the request's end and its non-finite elements before the P V
 // product reads them; the epilogue adds such an element back to the rows that
 // do see its key.
 //
@@ -47,8 +50,8 @@ namespace {
 constexpr int kMaxB = 1024;
 constexpr int kRows = 128;
 constexpr int kSoftmax = 256;     // two threads per query row
-constexpr int kCtlWarp = 8, kProdWarp = 9, kCheckWarp0 = 10, kCheckers = 64;
-constexpr int kThreads = 384;
+constexpr int kCtlWarp = 8, kProdWarp0 = 9, kProdWarps = 3, kProducers = 32 * kProdWarps;
+constexpr int kThreads = 384;     // twelve warps leave 168 registers a thread
 constexpr uint32_t kTmemCols = 512;
 // A unit's fixed cost in keys (query load, first tile's latency, output), and
 // the least share of a CTA: under it a cut costs more than it spreads.
@@ -69,7 +72,6 @@ struct Cfg {
 struct Small {
   uint64_t q_ready;
   uint64_t k_full[6], k_empty[6], v_full[6], v_empty[6];
-  uint64_t check[2], checked[2];  // [masked tile & 1]: its S has been issued; its V is fit to read
   uint64_t s_full[2], p_full[2];
   uint64_t o_done, o_full, o_free, mma_done;
   uint32_t tmem_base;
@@ -225,14 +227,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       mbar_init(smem_u32(&sm.q_ready), kSoftmax);
       for (int i = 0; i < kStages; ++i) {
-        mbar_init(smem_u32(&sm.k_full[i]), 1);
+        mbar_init(smem_u32(&sm.k_full[i]), kProducers + 1);
         mbar_init(smem_u32(&sm.k_empty[i]), 1);
-        mbar_init(smem_u32(&sm.v_full[i]), 1);
+        mbar_init(smem_u32(&sm.v_full[i]), kProducers + 1);
         mbar_init(smem_u32(&sm.v_empty[i]), 1);
       }
       for (int i = 0; i < 2; ++i) {
-        mbar_init(smem_u32(&sm.check[i]), 1);
-        mbar_init(smem_u32(&sm.checked[i]), kCheckers);
         mbar_init(smem_u32(&sm.s_full[i]), 1);
         mbar_init(smem_u32(&sm.p_full[i]), kSoftmax);
       }
@@ -307,7 +307,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t id_s = BF ? idesc_bf16(128, KT, false) : idesc_f16(128, KT, false);
       constexpr uint32_t id_o = BF ? idesc_bf16(128, D, true) : idesc_f16(128, D, true);
       int g = 0, ui = 0;
-      int asked = 0, told = 0;  // masked tiles handed to the checkers, and waited for
       bool ok = true;
       while (ok && next_piece<KT>(sm, P, w, w1, p)) {
         const int T = p.t1 - p.t0;
@@ -324,6 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (ok && t >= 1 && gt >= 2) ok = mbar_wait_or_abort(smem_u32(&sm.o_done), (gt - 2) & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
+            fence_async_smem();  // cp.async (generic proxy) writes -> tensor-core reads
             const uint32_t kb = k_base + st * kTile;
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
@@ -332,17 +332,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             mma_commit(smem_u32(&sm.k_empty[st]));
             mma_commit(smem_u32(&sm.s_full[sb]));
-            const int j1 = (p.t0 + t + 1) * KT;  // end of the tile
-            if (j1 > p.vis0 || j1 > p.L) mbar_arrive(smem_u32(&sm.check[asked++ & 1]));
           }
           if (t >= 1) {
             const int gu = g + t - 1, st = gu % kStages, pb = gu & 1;
             ok = mbar_wait_or_abort(smem_u32(&sm.v_full[st]), (gu / kStages) & 1, abort_flag);
-            const int j1 = (p.t0 + t) * KT;  // end of tile gu
-            if (ok && (j1 > p.vis0 || j1 > p.L)) {
-              ok = mbar_wait_or_abort(smem_u32(&sm.checked[told & 1]), (told >> 1) & 1, abort_flag);
-              ++told;
-            }
             ok = ok && mbar_wait_or_abort(smem_u32(&sm.p_full[pb]), (gu >> 1) & 1, abort_flag);
             // the first P V of a unit overwrites O: the previous unit's epilogue has read it
             if (ok && t == 1 && ui > 0) ok = mbar_wait_or_abort(smem_u32(&sm.o_free), (ui - 1) & 1, abort_flag);
@@ -350,6 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (ok && t == T && gu >= 1) ok = mbar_wait_or_abort(smem_u32(&sm.o_done), (gu - 1) & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
+            fence_async_smem();
             const uint32_t vb = v_base + st * kTile;
 #pragma unroll
             for (int k = 0; k < KT / 16; ++k) {
@@ -371,11 +365,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!mbar_wait(smem_u32(&sm.mma_done), 0)) raise_status(status, DFT_DEV_TIMEOUT);
     }
     __syncwarp();
-  } else if (warp == kProdWarp) {
-    // ------------------------------------------- producer: paged K/V gather
-    // lane's four keys of a tile, then 64-dim chunks kLanes apart
-    constexpr int kGroups = KT / 4, kStep = 32 / kGroups;
-    const int grp = lane % kGroups, c0 = lane / kGroups;
+  } else if (warp >= kProdWarp0) {
+    // ------------------------------------------- producers: paged K/V tiles
+    constexpr int kPer = KT / 32, kGroups = KT / 16;
+    const int pt = tid - kProdWarp0 * 32, pw = warp - kProdWarp0;
     const uint64_t pol_first = l2_evict_first(), pol_keep = l2_evict_normal();
     int g = 0;
     bool ok = true;
@@ -384,40 +377,71 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (T == 0) continue;
       const int32_t* idx = a.kv_indices + sm.kv[p.b];
       const uint64_t pol = p.once ? pol_first : pol_keep;
-      const int x0 = p.h * P.x_head, row0 = p.h * P.row_head;
-      int s[4];
-      // keys past the request's end repeat its last (the checkers zero their V)
+      const int64_t head = (int64_t)p.h * a.kv_sh;
+      int s[kPer];  // slots of keys lane + 32 q of a tile; -1 past the request's end
       auto fetch = [&](int tile) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) s[q] = __ldg(idx + min(tile * KT + 4 * grp + q, p.L - 1));
+        for (int q = 0; q < kPer; ++q) {
+          const int j = tile * KT + 32 * q + lane;
+          s[q] = j < p.L ? __ldg(idx + j) : -1;
+        }
       };
       fetch(p.t0);
       for (int t = 0; t < T; ++t) {
-        const int gt = g + t, st = gt % kStages;
-        int r[4];
+        const int gt = g + t, st = gt % kStages, j0 = (p.t0 + t) * KT;
+        int cur[kPer];
+        uint32_t boxes = 0;  // bit i: the 16 slots of group i are consecutive
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const bool in = s[q] >= 0 && (int64_t)s[q] < a.n_slots;
-          if (!in) raise_status(status, DFT_DEV_BAD_INDEX);
-          r[q] = (in ? s[q] : 0) + row0;
+        for (int q = 0; q < kPer; ++q) {
+          const int j = j0 + 32 * q + lane;
+          cur[q] = s[q];
+          if (j < p.L && (cur[q] < 0 || (int64_t)cur[q] >= a.n_slots)) {
+            raise_status(status, DFT_DEV_BAD_INDEX);
+            cur[q] = 0;
+          }
+          // keys past the end go along with their group's box
+          const int first = __shfl_sync(0xffffffffu, cur[q], lane & 16);
+          const uint32_t with = __ballot_sync(
+              0xffffffffu, first >= 0 && (int64_t)first + 16 <= a.n_slots && (j >= p.L || cur[q] == first + (lane & 15)));
+          boxes |= (with & 0xFFFFu) == 0xFFFFu ? 1u << (2 * q) : 0u;
+          boxes |= (with >> 16) == 0xFFFFu ? 2u << (2 * q) : 0u;
         }
         if (t + 1 < T) fetch(p.t0 + t + 1);
-        auto load = [&](uint64_t& full, uint64_t& empty, const CUtensorMap& map, uint32_t base) {
+        const int live = min(kGroups, (p.L - j0 + 15) / 16);  // groups with a key; the rest stay as they are
+        auto load = [&](uint64_t& full, uint64_t& empty, const CUtensorMap& map, const void* cache, uint32_t base) {
           if (gt >= kStages) {
             ok = __all_sync(0xffffffffu,
                             mbar_wait_or_abort(smem_u32(&empty), (gt / kStages - 1) & 1, abort_flag));
             if (!ok) return;
           }
-          if (lane == 0) mbar_expect_tx(smem_u32(&full), kTile);
-          __syncwarp();
+          const uint32_t bar = smem_u32(&full), dst = base + st * kTile;
+          if (pt == 0) mbar_expect_tx(bar, __popc(boxes) * 16 * D * 2);
 #pragma unroll
-          for (int c = 0; c < F::kChunks; c += kStep)
-            if (c + c0 < F::kChunks)
-              tma_gather4(base + st * kTile + (c + c0) * kChunk + grp * 512, &map, x0 + 64 * (c + c0), r[0], r[1], r[2],
-                          r[3], smem_u32(&full), pol);
+          for (int i = 0; i < kGroups; ++i) {
+            if (i >= live) break;
+            if (boxes >> i & 1) {
+              const int row = __shfl_sync(0xffffffffu, cur[i >> 1], (i & 1) * 16);
+              if (i % kProdWarps == pw && lane < F::kChunks)
+                tma_load_2d(dst + lane * kChunk + i * 2048, &map, p.h * P.x_head + 64 * lane, row + p.h * P.row_head, bar,
+                            pol);
+              continue;
+            }
+            constexpr int kUnits = D / 8;  // 16-byte pieces of a row
+#pragma unroll
+            for (int w0 = 0; w0 < kUnits / 2; w0 += kProdWarps) {  // 32 pieces a warp
+              if (w0 + pw >= kUnits / 2) break;
+              const int u = (w0 + pw) * 32 + lane, row = u / kUnits, col = u % kUnits, r = 16 * i + row;
+              const int slot = __shfl_sync(0xffffffffu, cur[i >> 1], (i & 1) * 16 + row);
+              if (j0 + r < p.L)
+                cp_async16(dst + (col >> 3) * kChunk + r * 128 + (((uint32_t)(col ^ r) & 7) << 4),
+                           static_cast<const unsigned char*>(cache) + (slot * a.kv_st + head) * 2 + col * 16, 16u, pol);
+            }
+          }
+          cp_async_arrive_noinc(bar);
         };
-        load(sm.k_full[st], sm.k_empty[st], k_map, k_base);
-        if (ok) load(sm.v_full[st], sm.v_empty[st], v_map, v_base);
+        // a group without a key has first = -1: no box
+        load(sm.k_full[st], sm.k_empty[st], k_map, a.k_cache, k_base);
+        if (ok) load(sm.v_full[st], sm.v_empty[st], v_map, a.v_cache, v_base);
         if (!ok) {
           g += t;
           break;
@@ -428,68 +452,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok && lane == 0 && !*abort_flag) set_abort(sm, status);
     // The last copies land before the block's shared memory goes, whatever
     // became of their readers; after an abort tile g may have its K on the way.
+    cp_async_wait_all();
     for (int gt = max(0, g - kStages); gt < g; ++gt) {
       mbar_wait(smem_u32(&sm.k_full[gt % kStages]), (gt / kStages) & 1);
       mbar_wait(smem_u32(&sm.v_full[gt % kStages]), (gt / kStages) & 1);
     }
     if (!ok) mbar_wait(smem_u32(&sm.k_full[g % kStages]), (g / kStages) & 1);
-  } else if (warp >= kCheckWarp0) {
-    // ------------- checkers: V rows past the end and non-finite values -> 0
-    const int ct = tid - kCheckWarp0 * 32;
-    constexpr uint32_t kExp = BF ? 0x7F807F80u : 0x7C007C00u, kOne = BF ? 0x00800080u : 0x04000400u;
-    // The checkers skip the other tiles, so v_full's parity means nothing to them
-    // until the control thread has reached the tile: it says so when it issues
-    // the tile's S (at most two such tiles are then unchecked).
-    int g = 0, ui = 0, seen = 0;
-    bool ok = true;
-    while (ok && next_piece<KT>(sm, P, w, w1, p)) {
-      const int T = p.t1 - p.t0;
-      if (T == 0) continue;
-      for (int t = 0; t < T; ++t) {
-        const int j0 = (p.t0 + t) * KT, gt = g + t, st = gt % kStages;
-        if (j0 + KT <= p.vis0 && j0 + KT <= p.L) continue;
-        ok = mbar_wait_or_abort(smem_u32(&sm.check[seen & 1]), (seen >> 1) & 1, abort_flag);
-        ok = ok && mbar_wait_or_abort(smem_u32(&sm.v_full[st]), (gt / kStages) & 1, abort_flag);
-        if (!ok) break;
-        const int live = min(KT, p.L - j0);               // rows of real keys
-        const bool scan = p.vis0 < j0 + live;             // some token does not see them all
-        unsigned char* vb = smem + (kStages + st) * kTile;
-        uint32_t any = 0;
-        for (int u = (scan ? 0 : live * 8) + ct; u < KT * 8; u += kCheckers) {
-#pragma unroll
-          for (int c = 0; c < F::kChunks; ++c) {
-            uint4* q = reinterpret_cast<uint4*>(vb + c * kChunk) + u;
-            if (u >= live * 8) {
-              *q = make_uint4(0u, 0u, 0u, 0u);
-              continue;
-            }
-            uint4 x = *q;
-            // a half's exponent is all ones iff adding one to it carries out
-            const uint32_t hit = (((x.x & kExp) + kOne) | ((x.y & kExp) + kOne) | ((x.z & kExp) + kOne) |
-                                  ((x.w & kExp) + kOne)) & 0x80008000u;
-            if (hit) {
-              any = 1;
-              auto clean = [&](uint32_t& y) {
-                const uint32_t e = ((y & kExp) + kOne) & 0x80008000u;
-                y &= ~((e >> 15) * 0xFFFFu);
-              };
-              clean(x.x);
-              clean(x.y);
-              clean(x.z);
-              clean(x.w);
-              *q = x;
-            }
-          }
-        }
-        if (any) *reinterpret_cast<volatile int*>(&sm.odd[ui & 7]) = ui + 1;
-        fence_async_smem();  // these writes before the tensor core's reads
-        mbar_arrive(smem_u32(&sm.checked[seen & 1]));
-        ++seen;
-      }
-      g += T;
-      ++ui;
-    }
-    if (!ok && !*abort_flag) set_abort(sm, status);
   } else {
     // ---------------------- softmax / epilogue: two threads per row, one half each
     constexpr int kCols = KT / 2;           // S columns of a thread
@@ -541,9 +509,51 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       return false;
     };
+    int g = 0, ui = 0;
+    // this thread's share of a masked tile's V: rows past the end and non-finite values -> 0
+    auto clean_v = [&](const Piece& u, int t, int gt) -> bool {
+      constexpr uint32_t kExp = BF ? 0x7F807F80u : 0x7C007C00u, kOne = BF ? 0x00800080u : 0x04000400u;
+      const int j0 = (u.t0 + t) * KT, st = gt % kStages;
+      const bool got =
+          __all_sync(0xffffffffu, mbar_wait_or_abort(smem_u32(&sm.v_full[st]), (gt / kStages) & 1, abort_flag));
+      if (!got) {
+        if (lane == 0 && !*abort_flag) set_abort(sm, status);
+        return false;
+      }
+      const int live = min(KT, u.L - j0);          // rows of real keys
+      const bool scan = u.vis0 < j0 + live;        // some token does not see them all
+      unsigned char* vb = smem + (kStages + st) * kTile;
+      bool any = false;
+#pragma unroll
+      for (int c = 0; c < F::kChunks; ++c) {
+#pragma unroll
+        for (int i = 0; i < KT * 8; i += kSoftmax) {
+          uint4* q = reinterpret_cast<uint4*>(vb + c * kChunk) + i + tid;
+          if (i + tid >= live * 8) {
+            *q = make_uint4(0u, 0u, 0u, 0u);
+          } else if (scan) {
+            uint4 x = *q;
+            // a half's exponent is all ones iff adding one to it carries out
+            const uint32_t hit = (((x.x & kExp) + kOne) | ((x.y & kExp) + kOne) | ((x.z & kExp) + kOne) |
+                                  ((x.w & kExp) + kOne)) & 0x80008000u;
+            if (hit) {
+              any = true;
+              auto clean = [&](uint32_t& y) { y &= ~(((((y & kExp) + kOne) & 0x80008000u) >> 15) * 0xFFFFu); };
+              clean(x.x);
+              clean(x.y);
+              clean(x.z);
+              clean(x.w);
+              *q = x;
+            }
+          }
+        }
+      }
+      if (any) *reinterpret_cast<volatile int*>(&sm.odd[ui & 7]) = ui + 1;
+      fence_async_smem();  // these writes before the tensor core's reads
+      return true;
+    };
     bool more = next_live(p);
     if (more) load_q(p);
-    int g = 0, ui = 0;
     bool ok = true;
     while (ok && more) {
       const Piece u = p;
@@ -554,12 +564,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       // A row's two warps meet at the same named barriers in the same order;
       // every early exit is decided from outcomes both have exchanged there.
       float m_used = -INFINITY, l = 0.f;
+      bool held = true;  // false: the last tile's V never came; told to the other warp at the next barrier
       for (int t = 0; t < T; ++t) {
         const int gt = g + t, sb = gt & 1;
-        const bool got =
-            __all_sync(0xffffffffu, mbar_wait_or_abort(smem_u32(&sm.s_full[sb]), (gt >> 1) & 1, abort_flag));
+        const bool got = __all_sync(0xffffffffu, held && mbar_wait_or_abort(smem_u32(&sm.s_full[sb]), (gt >> 1) & 1,
+                                                                           abort_flag));
+        // keys that every token of the tile sees need no mask (block-uniform)
+        const bool plain = (u.t0 + t + 1) * KT <= u.vis0 && (u.t0 + t + 1) * KT <= u.L;
         if (!busy) {  // spare rows: whatever P holds stays in them
-          ok = got;
+          ok = got && (plain || clean_v(u, t, gt));
           if (!ok) break;
           mbar_arrive(smem_u32(&sm.p_full[sb]));
           continue;
@@ -577,8 +590,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < kCols; ++i) x[i] = 0.f;
         }
         const int j0 = (u.t0 + t) * KT + kCols * hf;
-        // keys that every token of the tile sees need no mask: x stays raw, P = 2^(x sc - m)
-        const bool plain = (u.t0 + t + 1) * KT <= u.vis0 && (u.t0 + t + 1) * KT <= u.L;  // block-uniform
+        // x stays raw: P = 2^(x sc - m)
         float tmax = -INFINITY;
         if (!plain) {
 #pragma unroll
@@ -647,8 +659,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t(&pc)[16] = *reinterpret_cast<const uint32_t(*)[16]>(&pk[16 * c]);
           tmem_st16(tmem + lane_base + F::COL_S + KT * sb + kPk * hf + 16 * c, pc);
         }
+        held = plain || clean_v(u, t, gt);
         tc_fence_before();
-        mbar_arrive(smem_u32(&sm.p_full[sb]));
+        if (held) mbar_arrive(smem_u32(&sm.p_full[sb]));
       }
       if (!ok) break;
       g += T;
@@ -656,7 +669,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       more = next_live(p);
       if (more) load_q(p);
       // ---- epilogue: wait for this unit's last P V, then O (or its partial) out
-      const bool got = __all_sync(0xffffffffu, mbar_wait_or_abort(smem_u32(&sm.o_full), ui & 1, abort_flag));
+      const bool got =
+          __all_sync(0xffffffffu, held && mbar_wait_or_abort(smem_u32(&sm.o_full), ui & 1, abort_flag));
       tc_fence_after();
       if (busy) {
         sm.lsum[hf][r] = l;
@@ -846,7 +860,7 @@ bool encode(CUtensorMap* m, const dft_chunk_attn_args* a, const void* base, bool
   const cuuint64_t dims[2] = {(cuuint64_t)(inner ? (a->Hkv - 1) * a->kv_sh + a->D : a->D),
                               (cuuint64_t)(inner ? a->n_slots : a->n_slots + (a->Hkv - 1) * (a->kv_sh / a->kv_st))};
   const cuuint64_t strides[1] = {(cuuint64_t)a->kv_st * 2};
-  const cuuint32_t box[2] = {64, 1}, estr[2] = {1, 1};
+  const cuuint32_t box[2] = {64, 16}, estr[2] = {1, 1};
   return gtile::encode_fn() &&
          gtile::encode_fn()(m, a->dtype == DFT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                             2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
