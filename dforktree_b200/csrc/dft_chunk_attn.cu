@@ -4,29 +4,38 @@
 // q-head hq:  o = softmax_j(q . k_j * sm_scale | j <= L - n + i) . v_j.
 //
 // A unit is (request, kv-head, query tile).  The G q-heads of a kv-head share
-// its keys, so a tile's 128 rows are 128 / G tokens x G heads (row = token * G
-// + head) and one tcgen05 MMA of M = 128 serves them all; a single token's G
-// rows go through the same tile, whose spare rows cost no memory traffic.  Per
-// tile of KT keys, one pass with a running maximum and sum:
+// its keys, so a tile's rows are tokens x G heads (row = token * G + head) and
+// one tcgen05 MMA serves them all; a single token's G rows go through the same
+// tile, whose spare rows cost no memory traffic.  D <= 128: a CTA and 128 rows.
+// D = 256: two CTAs (cta_group::2) and 256 rows, each CTA holding half of every
+// K / V tile: 128 rows against 128 keys need O, two S and Q in 640 TMEM columns
+// of 512, and with 64 keys the S MMAs run at half rate (72 cycles for 128 x 64
+// x 16 from TMEM, bound by reading A); Q in shared memory leaves a CTA alone no
+// room for two 128 KB tiles.  Per tile of 128 keys, one pass with a running
+// maximum and sum:
 //   K, V  by slot, 16 keys at a time, into separate rings of stages by three
 //         producer warps: where the 16 slots are consecutive (pages of 16 and
 //         more) one TMA box of 16 cache rows x 64 dims per copy, else 16-byte
 //         cp.async row by row (a gather of four rows per TMA copy took 39 ns a
-//         copy, 5 us per 64 KB tile)
-//   S     = Q K^T    kind::f16, A = Q from TMEM, M=128 N=KT K=D, fp32 in TMEM
-//   P     = 2^(S sm_scale log2e - m), two threads per row; the reference m
-//         moves (and O is rescaled in TMEM) only when the maximum grows by
-//         more than 8, so P <= 2^8; rounded to the 16-bit type over its own S
-//         (the second product's operand has V's type), summed unrounded
-//   O    += P V      A = P from TMEM, V as an MN-major operand, N = D
-// S / P are double-buffered, so the S MMA of tile t+1 runs under the softmax
-// of tile t.
+//         copy, 5 us per 64 KB)
+//   S     = Q K^T    kind::f16, fp32 in TMEM; Q from TMEM, or from shared memory
+//         for a pair
+//   P     = 2^(S sm_scale log2e - m), a thread per row; the reference m moves
+//         (and O is rescaled in TMEM) only when the maximum grows by more than
+//         8, so P <= 2^8; rounded to the 16-bit type over its own S (the second
+//         product's operand has V's type), summed unrounded
+//   O    += P V      P from TMEM, V as an MN-major operand
+// Two softmax warpgroups take the tiles in turn, each with twice a tile's MMA
+// time to hide its latencies in; m goes from one to the other through shared
+// memory as soon as a tile's maximum is known.  S / P are double-buffered and
+// the S MMA runs a tile ahead of the P V MMA.
 //
 // Work is split by keys, not by unit: unit costs (keys + a fixed part) are laid
-// out on one line, and CTA c takes the c-th share of it, whatever units that
-// crosses.  One long prompt, many ragged requests and one long decode all fill
-// the GPU evenly, from lengths that only the device knows.  A unit cut by a
-// share's border leaves partials (O, m, l) that a second kernel merges.
+// out on one line, and worker c (a CTA, a pair) takes the c-th share of it,
+// whatever units that crosses.  One long prompt, many ragged requests and one
+// long decode all fill the GPU evenly, from lengths that only the device knows.
+// A unit cut by a share's border leaves partials (O, m, l) that a second kernel
+// merges.
 //
 // Tiles past a row's last key hold the masked keys' values: their P is 0, but 0
 // times NaN or infinity is not.  In those tiles alone the softmax threads zero
@@ -41,6 +50,7 @@
 #include "dft_tc.cuh"
 
 #include <cstring>
+#include <type_traits>
 
 using namespace dft;
 using namespace dft::tc;
@@ -48,58 +58,67 @@ using namespace dft::tc;
 namespace {
 
 constexpr int kMaxB = 1024;
-constexpr int kRows = 128;
-constexpr int kSoftmax = 256;     // two threads per query row
+constexpr int kRows = 128;        // query rows of a CTA
+constexpr int KT = 128;           // keys per tile
+constexpr int kSoftmax = 256;     // two warpgroups, a thread per query row in each
 constexpr int kCtlWarp = 8, kProdWarp0 = 9, kProdWarps = 3, kProducers = 32 * kProdWarps;
 constexpr int kThreads = 384;     // twelve warps leave 168 registers a thread
 constexpr uint32_t kTmemCols = 512;
 // A unit's fixed cost in keys (query load, first tile's latency, output), and
-// the least share of a CTA: under it a cut costs more than it spreads.
-constexpr int kUnitKeys = 128;
-constexpr int kMinShare = 256;
+// the least share of a worker: under it a cut costs more than it spreads.
+constexpr int kUnitKeys = 256;
+constexpr int kMinShare = 384;
+
+template <int N>
+using Int = std::integral_constant<int, N>;
 
 template <int D>
 struct Cfg {
-  static constexpr int KT = D == 256 ? 64 : 128;              // keys per tile: O, Q and two S fit TMEM's 512 columns
-  static constexpr int kStages = D == 64 ? 6 : 3;
-  static constexpr int kChunks = D / 64;                      // 128-byte columns of a tile
-  static constexpr uint32_t kChunkBytes = KT * 128;
-  static constexpr uint32_t kTileBytes = kChunks * kChunkBytes;
-  static constexpr uint32_t COL_O = 0, COL_Q = D, COL_S = D + D / 2;  // S / P buffer b at COL_S + KT b
+  static constexpr bool kPair = D == 256;
+  static constexpr int CG = kPair ? 2 : 1;                    // CTAs of a worker
+  static constexpr int kStages = kPair ? 2 : D == 128 ? 3 : 6;
+  static constexpr int KR = KT / CG, KC = D / 64;             // K rows and 64-dim chunks in this CTA
+  static constexpr int VC = D / 64 / CG;                      // V chunks in this CTA (all KT rows)
+  static constexpr uint32_t kKBytes = KR * KC * 128, kVBytes = KT * VC * 128;
+  static constexpr uint32_t kQBytes = kPair ? kRows * D * 2 : 0;
+  static constexpr uint32_t OFF_V = kStages * kKBytes, OFF_Q = OFF_V + kStages * kVBytes;
+  static constexpr uint32_t OFF_SMALL = OFF_Q + kQBytes;
+  static constexpr uint32_t COL_O = 0, COL_Q = D, COL_S = kPair ? D : D + D / 2;  // S / P buffer b at COL_S + KT b
   static_assert(COL_S + 2 * KT <= kTmemCols, "TMEM");
 };
 
 struct Small {
   uint64_t q_ready;
   uint64_t k_full[6], k_empty[6], v_full[6], v_empty[6];
-  uint64_t s_full[2], p_full[2];
-  uint64_t o_done, o_full, o_free, mma_done;
+  uint64_t k_peer[2], v_peer[2];  // the other CTA's half of the stage (rank 0 of a pair)
+  uint64_t s_full[2], p_full[2], pv_done[2];
+  uint64_t m_ready[2][4];   // [tile & 1][row warp]: the tile's reference is in m
+  uint64_t l_ready, o_full, o_free, mma_done;
   uint32_t tmem_base;
   int abort;
   int odd[8];               // [piece & 7] = piece + 1 when one of its masked tiles held a non-finite value
-  float xmax[2][2][kRows];  // [tile parity][half][row] tile max exchange between a row's two threads
-  float lsum[2][kRows];     // [half][row] final row sums
-  int okx[2][2][4];         // [tile parity][half][row warp] wait outcomes, shared by a row's two warps
-  int okr[2][2][4];         // the same for the rescale's wait
-  int oke[2][4];            // [half][row warp] the epilogue's wait
+  float m[kRows];           // the reference after the last tile whose maximum is known
+  float2 ml[2][2][kRows];   // [piece & 1][warpgroup] its reference and its part of the row sum
   int64_t warp_sum[kThreads / 32];
   int64_t pre[kMaxB + 1];   // cost of the requests before b
   int qo[kMaxB + 1], kv[kMaxB + 1];
+  int slots[kProdWarps][KT];
+  int k_mixed[6], v_mixed[6];  // [stage]: the CTA's part holds rows copied by cp.async
 };
 
 struct Params {
   dft_chunk_attn_args a;
   int G, TQ;                // q-heads per kv-head, tokens per query tile
   int x_head, row_head;     // kv-head h starts at column h * x_head, row h * row_head of the tensor map
-  float* ws_o;              // [2 grid][128][D] partial O: slot 2c continues a unit, 2c + 1 begins one
-  float* ws_ml;             // [2 grid][128][2] partial (m, l)
-  int4* ws_meta;            // [2 grid] (flags, first token row, tokens, kv-head); flags 1: used, 2: the unit's last
+  float* ws_o;              // [2 workers][rows][D] partial O: slot 2c continues a unit, 2c + 1 begins one
+  float* ws_ml;             // [2 workers][rows][2] partial (m, l)
+  int4* ws_meta;            // [2 workers] (flags, first token row, tokens, kv-head); flags 1: used, 2: the unit's last
 };
 
 template <int D>
 constexpr uint32_t smem_bytes() {
-  static_assert(2 * Cfg<D>::kStages * Cfg<D>::kTileBytes + sizeof(Small) + 1024 <= 232448, "shared memory");
-  return 2 * Cfg<D>::kStages * Cfg<D>::kTileBytes + (uint32_t)sizeof(Small) + 1024;  // + alignment slack
+  static_assert(Cfg<D>::OFF_SMALL + sizeof(Small) + 1024 <= 232448, "shared memory");
+  return Cfg<D>::OFF_SMALL + (uint32_t)sizeof(Small) + 1024;  // + alignment slack
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -122,6 +141,40 @@ __device__ __forceinline__ float unpack(uint16_t v) {
 __device__ __forceinline__ void set_abort(Small& sm, int32_t* status) {
   *reinterpret_cast<volatile int*>(&sm.abort) = 1;
   raise_status(status, DFT_DEV_TIMEOUT);
+}
+
+// Bounded wait that also gives up once another role has; the clock is read
+// only when the first try fails.
+__device__ __forceinline__ bool wait(uint64_t& bar, uint32_t parity, const volatile int* abort) {
+  return mbar_try(smem_u32(&bar), parity) || mbar_wait_or_abort(smem_u32(&bar), parity, abort);
+}
+// The same for barriers that the pair's other CTA arrives on.
+template <bool PAIR>
+__device__ __forceinline__ bool wait_pair(uint64_t& bar, uint32_t parity, const volatile int* abort) {
+  if (!PAIR) return wait(bar, parity, abort);
+  if (mbar_try_cluster(smem_u32(&bar), parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_cluster(smem_u32(&bar), parity)) {
+    if (*abort || clock64() - t0 > 2000000000ll) return false;
+  }
+  return true;
+}
+// Arrive, once per warp and after all of its lanes, on the barrier of the CTA
+// that issues the MMAs.
+template <bool PAIR>
+__device__ __forceinline__ void warp_arrive(uint64_t& bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) {
+    if (PAIR) mbar_arrive_cluster(map_rank(smem_u32(&bar), 0));
+    else mbar_arrive(smem_u32(&bar));
+  }
+}
+
+// 64 columns of this thread's TMEM lane
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
+  tmem_ld32_async(taddr, &v[0]);
+  tmem_ld32_async(taddr + 32, &v[32]);
+  tmem_ld_wait(v);
 }
 
 // -------------------------------------------------------------- schedule --
@@ -154,7 +207,7 @@ __device__ __forceinline__ int64_t cost_before(const Req& r, int i, int TQ) {
   return last + (int64_t)i * kUnitKeys + (i - z) * a + TQ * (((int64_t)i * (i + 1) - z * (z + 1)) / 2);
 }
 
-// A CTA's part of one unit: key tiles [t0, t1) of nt.
+// A worker's part of one unit: key tiles [t0, t1) of nt.
 struct Piece {
   int b, h, tok0, ntok;  // first token row of q, tokens
   int vis0, L;           // keys that the first token sees (may be negative), keys of the request
@@ -164,7 +217,6 @@ struct Piece {
 };
 
 // The next piece of the line from w, w < w1, that has something to do.
-template <int KT>
 __device__ __forceinline__ bool next_piece(const Small& sm, const Params& P, int64_t& w, int64_t w1, Piece& p) {
   while (w < w1) {
     int lo = 0, hi = P.a.B;  // pre[lo] <= w < pre[hi]
@@ -211,21 +263,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     chunk_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                       const __grid_constant__ Params P, int32_t* status) {
   using F = Cfg<D>;
-  constexpr int KT = F::KT, kStages = F::kStages;
-  constexpr uint32_t kTile = F::kTileBytes, kChunk = F::kChunkBytes;
+  constexpr bool PAIR = F::kPair;
+  constexpr int kStages = F::kStages, CG = F::CG;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  Small& sm = *reinterpret_cast<Small*>(smem + 2 * kStages * kTile);
+  Small& sm = *reinterpret_cast<Small*>(smem + F::OFF_SMALL);
   const volatile int* abort_flag = &sm.abort;
   const dft_chunk_attn_args& a = P.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t k_base = smem_u32(smem), v_base = k_base + kStages * kTile;
+  const uint32_t k_base = smem_u32(smem), v_base = k_base + F::OFF_V;
+  const int rank = PAIR ? (int)cluster_rank() : 0;
+  const int worker = blockIdx.x / CG, workers = gridDim.x / CG;
 
   // the merge kernel's blocks may come up now; they wait for this grid to end
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp == kCtlWarp) {
     if (lane == 0) {
-      mbar_init(smem_u32(&sm.q_ready), kSoftmax);
+      mbar_init(smem_u32(&sm.q_ready), kSoftmax / 32 * CG);
       for (int i = 0; i < kStages; ++i) {
         mbar_init(smem_u32(&sm.k_full[i]), kProducers + 1);
         mbar_init(smem_u32(&sm.k_empty[i]), 1);
@@ -233,19 +287,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(smem_u32(&sm.v_empty[i]), 1);
       }
       for (int i = 0; i < 2; ++i) {
+        mbar_init(smem_u32(&sm.k_peer[i]), 1);
+        mbar_init(smem_u32(&sm.v_peer[i]), 1);
         mbar_init(smem_u32(&sm.s_full[i]), 1);
-        mbar_init(smem_u32(&sm.p_full[i]), kSoftmax);
+        mbar_init(smem_u32(&sm.p_full[i]), kSoftmax / 64 * CG);
+        mbar_init(smem_u32(&sm.pv_done[i]), 1);
+        for (int j = 0; j < 4; ++j) mbar_init(smem_u32(&sm.m_ready[i][j]), 1);
       }
-      mbar_init(smem_u32(&sm.o_done), 1);
+      mbar_init(smem_u32(&sm.l_ready), kSoftmax / 32);
       mbar_init(smem_u32(&sm.o_full), 1);
-      mbar_init(smem_u32(&sm.o_free), kSoftmax);
+      mbar_init(smem_u32(&sm.o_free), kSoftmax / 32 * CG);
       mbar_init(smem_u32(&sm.mma_done), 1);
       sm.abort = 0;
       for (int i = 0; i < 8; ++i) sm.odd[i] = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
-    tmem_alloc(smem_u32(&sm.tmem_base), kTmemCols);
+    if (PAIR) tmem_alloc_2(smem_u32(&sm.tmem_base), kTmemCols);
+    else tmem_alloc(smem_u32(&sm.tmem_base), kTmemCols);
   }
   // offsets and the requests' costs: thread t sums requests [t per, ...)
   {
@@ -293,91 +352,124 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync();  // the other CTA's barriers are up before anything arrives on them
   tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
   const int64_t total = sm.pre[a.B];
-  const int64_t share = max((int64_t)kMinShare, (total + gridDim.x - 1) / gridDim.x);
-  const int64_t w0 = min(total, share * blockIdx.x), w1 = min(total, w0 + share);
+  const int64_t share = max((int64_t)kMinShare, (total + workers - 1) / workers);
+  const int64_t w0 = min(total, share * worker), w1 = min(total, w0 + share);
   int64_t w = w0;
   Piece p;
 
   if (warp == kCtlWarp) {
-    // ------------------------------------------------------ control: MMAs
-    if (lane == 0) {
-      constexpr uint32_t id_s = BF ? idesc_bf16(128, KT, false) : idesc_f16(128, KT, false);
-      constexpr uint32_t id_o = BF ? idesc_bf16(128, D, true) : idesc_f16(128, D, true);
+    if (rank == 0) {
+      // ---------------------------------------------------- control: MMAs
+      const uint32_t lead = elect_lane();
+      const auto commit = [&](uint64_t& bar) { mma_commit_lead<CG>(lead, smem_u32(&bar)); };
+      // waits of the whole warp: one outcome for all lanes
+      const auto all = [](bool x) { return __all_sync(0xffffffffu, x) != 0; };
+      constexpr uint32_t id_s = BF ? idesc_bf16(128 * CG, KT, false) : idesc_f16(128 * CG, KT, false);
+      constexpr uint32_t id_o = BF ? idesc_bf16(128 * CG, D, true) : idesc_f16(128 * CG, D, true);
+      const uint32_t q_base = k_base + F::OFF_Q;
       int g = 0, ui = 0;
       bool ok = true;
-      while (ok && next_piece<KT>(sm, P, w, w1, p)) {
+      while (ok && next_piece(sm, P, w, w1, p)) {
         const int T = p.t1 - p.t0;
         if (T == 0) continue;
-        ok = mbar_wait_or_abort(smem_u32(&sm.q_ready), ui & 1, abort_flag);
+        ok = all(wait_pair<PAIR>(sm.q_ready, ui & 1, abort_flag));
         for (int t = 0; ok && t <= T; ++t) {
           if (t < T) {
             const int gt = g + t, st = gt % kStages, sb = gt & 1;
-            ok = mbar_wait_or_abort(smem_u32(&sm.k_full[st]), (gt / kStages) & 1, abort_flag);
-            // S/P buffer sb is free once P V of tile gt-2 has retired.  For a
-            // unit's first tile that wait happened before the previous unit's
-            // last P V was issued: o_done's parity tells phases apart only
-            // while P V gt-1 is not yet issued.
-            if (ok && t >= 1 && gt >= 2) ok = mbar_wait_or_abort(smem_u32(&sm.o_done), (gt - 2) & 1, abort_flag);
+            bool got = wait(sm.k_full[st], (gt / kStages) & 1, abort_flag);
+            if (PAIR) got = got && wait_pair<PAIR>(sm.k_peer[st], (gt / kStages) & 1, abort_flag);
+            if (got && gt >= 2) got = wait(sm.pv_done[sb], (gt / 2 - 1) & 1, abort_flag);  // P of tile gt - 2 is read
+            ok = all(got);
             if (!ok) break;
             tc_fence_after();
-            fence_async_smem();  // cp.async (generic proxy) writes -> tensor-core reads
-            const uint32_t kb = k_base + st * kTile;
+            if (sm.k_mixed[st]) fence_async_smem();  // cp.async (generic proxy) writes -> tensor-core reads
+            const uint32_t kb = __shfl_sync(0xffffffffu, k_base + st * F::kKBytes, 0);
+            const uint32_t ds = __shfl_sync(0xffffffffu, tmem + F::COL_S + KT * sb, 0);
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
-              const uint64_t bd = sw128_desc(kb + (k >> 2) * kChunk + (k & 3) * 32);
-              mma_bf16_ts(tmem + F::COL_S + KT * sb, tmem + F::COL_Q + 8 * k, bd, id_s, k > 0);
+              const uint64_t bd = sw128_desc(kb + (k >> 2) * (F::KR * 128) + (k & 3) * 32);
+              if (PAIR)
+                mma_ss<CG>(lead, ds, sw128_desc(q_base + (k >> 2) * (kRows * 128) + (k & 3) * 32), bd, id_s, k > 0);
+              else
+                mma_ts<CG>(lead, ds, tmem + F::COL_Q + 8 * k, bd, id_s, k > 0);
             }
-            mma_commit(smem_u32(&sm.k_empty[st]));
-            mma_commit(smem_u32(&sm.s_full[sb]));
+            commit(sm.k_empty[st]);
+            commit(sm.s_full[sb]);
           }
           if (t >= 1) {
             const int gu = g + t - 1, st = gu % kStages, pb = gu & 1;
-            ok = mbar_wait_or_abort(smem_u32(&sm.v_full[st]), (gu / kStages) & 1, abort_flag);
-            ok = ok && mbar_wait_or_abort(smem_u32(&sm.p_full[pb]), (gu >> 1) & 1, abort_flag);
+            bool got = wait(sm.v_full[st], (gu / kStages) & 1, abort_flag);
+            if (PAIR) got = got && wait_pair<PAIR>(sm.v_peer[st], (gu / kStages) & 1, abort_flag);
             // the first P V of a unit overwrites O: the previous unit's epilogue has read it
-            if (ok && t == 1 && ui > 0) ok = mbar_wait_or_abort(smem_u32(&sm.o_free), (ui - 1) & 1, abort_flag);
-            // before a unit's last P V, P V gu-1 has retired (frees the next unit's first S/P buffer)
-            if (ok && t == T && gu >= 1) ok = mbar_wait_or_abort(smem_u32(&sm.o_done), (gu - 1) & 1, abort_flag);
+            if (got && t == 1 && ui > 0) got = wait_pair<PAIR>(sm.o_free, (ui - 1) & 1, abort_flag);
+            ok = all(got && wait_pair<PAIR>(sm.p_full[pb], (gu >> 1) & 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
-            fence_async_smem();
-            const uint32_t vb = v_base + st * kTile;
+            if (sm.v_mixed[st]) fence_async_smem();
+            const uint32_t vb = __shfl_sync(0xffffffffu, v_base + st * F::kVBytes, 0);
+            const uint32_t ps = __shfl_sync(0xffffffffu, tmem + F::COL_S + KT * pb, 0);
+            const uint32_t keep = __shfl_sync(0xffffffffu, t > 1 ? 1u : 0u, 0);
 #pragma unroll
             for (int k = 0; k < KT / 16; ++k) {
-              // V [keys x dims] is MN-major: 64-dim chunks kChunk apart, 8-key groups 1 KB apart
-              const uint64_t bd = sw128_desc(vb + k * 16 * 128, kChunk, 1024);
-              mma_bf16_ts(tmem + F::COL_O, tmem + F::COL_S + KT * pb + 8 * k, bd, id_o, (t > 1 || k > 0) ? 1u : 0u);
+              // V [keys x dims] is MN-major: 64-dim chunks KT rows apart, 8-key groups 1 KB apart
+              const uint64_t bd = sw128_desc(vb + k * 16 * 128, KT * 128, 1024);
+              mma_ts<CG>(lead, tmem + F::COL_O, ps + 8 * k, bd, id_o, k > 0 ? 1u : keep);
             }
-            mma_commit(smem_u32(&sm.v_empty[st]));
-            mma_commit(smem_u32(&sm.o_done));
-            if (t == T) mma_commit(smem_u32(&sm.o_full));
+            commit(sm.v_empty[st]);
+            commit(sm.pv_done[pb]);
+            if (t == T) commit(sm.o_full);
           }
         }
         g += T;
         ++ui;
       }
-      if (!ok && !*abort_flag) set_abort(sm, status);
+      if (!ok && lane == 0 && !*abort_flag) set_abort(sm, status);
       // every MMA issued above has retired before TMEM is freed
-      mma_commit(smem_u32(&sm.mma_done));
-      if (!mbar_wait(smem_u32(&sm.mma_done), 0)) raise_status(status, DFT_DEV_TIMEOUT);
+      commit(sm.mma_done);
+    } else if (lane == 0) {
+      // rank 1 of a pair: tell rank 0 of this CTA's halves as they land
+      int g = 0;
+      bool ok = true;
+      while (ok && next_piece(sm, P, w, w1, p)) {
+        const int T = p.t1 - p.t0;
+        for (int gt = g; ok && gt < g + T; ++gt) {
+          const int st = gt % kStages;
+          ok = wait(sm.k_full[st], (gt / kStages) & 1, abort_flag);
+          if (!ok) break;
+          if (sm.k_mixed[st]) fence_async_smem();
+          mbar_arrive_cluster(map_rank(smem_u32(&sm.k_peer[st & 1]), 0));
+          ok = wait(sm.v_full[st], (gt / kStages) & 1, abort_flag);
+          if (!ok) break;
+          if (sm.v_mixed[st]) fence_async_smem();
+          mbar_arrive_cluster(map_rank(smem_u32(&sm.v_peer[st & 1]), 0));
+        }
+        g += T;
+      }
+      if (!ok && !*abort_flag) set_abort(sm, status);
     }
+    if (lane == 0 && !mbar_wait(smem_u32(&sm.mma_done), 0)) raise_status(status, DFT_DEV_TIMEOUT);
     __syncwarp();
   } else if (warp >= kProdWarp0) {
     // ------------------------------------------- producers: paged K/V tiles
-    constexpr int kPer = KT / 32, kGroups = KT / 16;
+    // Code is kept short (loops rolled, K and V through one body): unrolled, the
+    // roles' instructions together starved the warps of each other's.
+    constexpr int kPer = KT / 32;
     const int pt = tid - kProdWarp0 * 32, pw = warp - kProdWarp0;
     const uint64_t pol_first = l2_evict_first(), pol_keep = l2_evict_normal();
+    const uint32_t lead = elect_lane();
+    int* slots = sm.slots[pw];  // the tile's slots, this warp's copy
     int g = 0;
     bool ok = true;
-    while (ok && next_piece<KT>(sm, P, w, w1, p)) {
+    while (ok && next_piece(sm, P, w, w1, p)) {
       const int T = p.t1 - p.t0;
       if (T == 0) continue;
       const int32_t* idx = a.kv_indices + sm.kv[p.b];
       const uint64_t pol = p.once ? pol_first : pol_keep;
-      const int64_t head = (int64_t)p.h * a.kv_sh;
+      const int x0 = p.h * P.x_head, row0 = p.h * P.row_head;
       int s[kPer];  // slots of keys lane + 32 q of a tile; -1 past the request's end
       auto fetch = [&](int tile) {
 #pragma unroll
@@ -387,61 +479,76 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       fetch(p.t0);
+#pragma unroll 1
       for (int t = 0; t < T; ++t) {
         const int gt = g + t, st = gt % kStages, j0 = (p.t0 + t) * KT;
-        int cur[kPer];
         uint32_t boxes = 0;  // bit i: the 16 slots of group i are consecutive
+        bool bad = false;
+        __syncwarp();
 #pragma unroll
         for (int q = 0; q < kPer; ++q) {
           const int j = j0 + 32 * q + lane;
-          cur[q] = s[q];
-          if (j < p.L && (cur[q] < 0 || (int64_t)cur[q] >= a.n_slots)) {
-            raise_status(status, DFT_DEV_BAD_INDEX);
-            cur[q] = 0;
+          int cur = s[q];
+          if (j < p.L && (cur < 0 || (int64_t)cur >= a.n_slots)) {
+            bad = true;
+            cur = 0;
           }
-          // keys past the end go along with their group's box
-          const int first = __shfl_sync(0xffffffffu, cur[q], lane & 16);
+          slots[32 * q + lane] = cur;
+          // keys past the end go along with their group's box; a group without a key has none
+          const int first = __shfl_sync(0xffffffffu, cur, lane & 16);
           const uint32_t with = __ballot_sync(
-              0xffffffffu, first >= 0 && (int64_t)first + 16 <= a.n_slots && (j >= p.L || cur[q] == first + (lane & 15)));
+              0xffffffffu, first >= 0 && (int64_t)first + 16 <= a.n_slots && (j >= p.L || cur == first + (lane & 15)));
           boxes |= (with & 0xFFFFu) == 0xFFFFu ? 1u << (2 * q) : 0u;
           boxes |= (with >> 16) == 0xFFFFu ? 2u << (2 * q) : 0u;
         }
+        if (bad) raise_status(status, DFT_DEV_BAD_INDEX);
+        __syncwarp();
         if (t + 1 < T) fetch(p.t0 + t + 1);
-        const int live = min(kGroups, (p.L - j0 + 15) / 16);  // groups with a key; the rest stay as they are
-        auto load = [&](uint64_t& full, uint64_t& empty, const CUtensorMap& map, const void* cache, uint32_t base) {
+        const int live = min(KT / 16, (p.L - j0 + 15) / 16);  // groups with a key; the rest stay as they are
+#pragma unroll 1
+        for (int v = 0; v < 2; ++v) {
+          // K: this CTA's rows, all chunks; V: all rows, this CTA's chunks; chunks ng * 16 rows apart
+          const int ng = v ? KT / 16 : F::KR / 16, nc = v ? F::VC : F::KC;
+          const int g0 = v ? 0 : rank * (F::KR / 16), c0 = v ? rank * F::VC : 0;
+          uint64_t& full = v ? sm.v_full[st] : sm.k_full[st];
           if (gt >= kStages) {
-            ok = __all_sync(0xffffffffu,
-                            mbar_wait_or_abort(smem_u32(&empty), (gt / kStages - 1) & 1, abort_flag));
-            if (!ok) return;
+            ok = __all_sync(0xffffffffu, wait(v ? sm.v_empty[st] : sm.k_empty[st], (gt / kStages - 1) & 1, abort_flag));
+            if (!ok) break;
           }
-          const uint32_t bar = smem_u32(&full), dst = base + st * kTile;
-          if (pt == 0) mbar_expect_tx(bar, __popc(boxes) * 16 * D * 2);
-#pragma unroll
-          for (int i = 0; i < kGroups; ++i) {
-            if (i >= live) break;
-            if (boxes >> i & 1) {
-              const int row = __shfl_sync(0xffffffffu, cur[i >> 1], (i & 1) * 16);
-              if (i % kProdWarps == pw && lane < F::kChunks)
-                tma_load_2d(dst + lane * kChunk + i * 2048, &map, p.h * P.x_head + 64 * lane, row + p.h * P.row_head, bar,
-                            pol);
+          const uint32_t bar = smem_u32(&full);
+          const uint32_t dst = v ? v_base + st * F::kVBytes : k_base + st * F::kKBytes;
+          const uint32_t mine = boxes >> g0 & ((1u << ng) - 1);
+          if (pt == 0) {
+            // groups with a key that go by cp.async: their readers need a proxy fence
+            (v ? sm.v_mixed : sm.k_mixed)[st] = __popc(mine) < max(0, min(ng, live - g0));
+            mbar_expect_tx(bar, __popc(mine) * 16 * nc * 128);
+          }
+          const CUtensorMap* map = v ? &v_map : &k_map;
+          const unsigned char* base =
+              static_cast<const unsigned char*>(v ? a.v_cache : a.k_cache) + ((int64_t)p.h * a.kv_sh + 64 * c0) * 2;
+#pragma unroll 1
+          for (int i = 0; i < min(ng, live - g0); ++i) {
+            if (mine >> i & 1) {
+              if (i % kProdWarps == pw) {
+                const int row = slots[16 * (g0 + i)] + row0;
+#pragma unroll 1
+                for (int c = 0; c < nc; ++c)
+                  tma_load_2d(lead, dst + c * (ng * 2048) + i * 2048, map, x0 + 64 * (c0 + c), row, bar, pol);
+              }
               continue;
             }
-            constexpr int kUnits = D / 8;  // 16-byte pieces of a row
-#pragma unroll
-            for (int w0 = 0; w0 < kUnits / 2; w0 += kProdWarps) {  // 32 pieces a warp
-              if (w0 + pw >= kUnits / 2) break;
-              const int u = (w0 + pw) * 32 + lane, row = u / kUnits, col = u % kUnits, r = 16 * i + row;
-              const int slot = __shfl_sync(0xffffffffu, cur[i >> 1], (i & 1) * 16 + row);
-              if (j0 + r < p.L)
-                cp_async16(dst + (col >> 3) * kChunk + r * 128 + (((uint32_t)(col ^ r) & 7) << 4),
-                           static_cast<const unsigned char*>(cache) + (slot * a.kv_st + head) * 2 + col * 16, 16u, pol);
+            // 16 rows of 8 nc pieces of 16 bytes, 32 pieces a turn
+            const int shift = nc == 4 ? 5 : nc == 2 ? 4 : 3;
+#pragma unroll 2
+            for (int turn = pw; turn < nc * 4; turn += kProdWarps) {
+              const int u = turn * 32 + lane, row = u >> shift, col = u & ((1 << shift) - 1), r = 16 * i + row;
+              const int slot = slots[16 * g0 + r];
+              cp_async16(dst + (col >> 3) * (ng * 2048) + r * 128 + (((uint32_t)(col ^ r) & 7) << 4),
+                         base + (slot < 0 ? 0 : (int64_t)slot * a.kv_st * 2 + col * 16), slot < 0 ? 0u : 16u, pol);
             }
           }
           cp_async_arrive_noinc(bar);
-        };
-        // a group without a key has first = -1: no box
-        load(sm.k_full[st], sm.k_empty[st], k_map, a.k_cache, k_base);
-        if (ok) load(sm.v_full[st], sm.v_empty[st], v_map, a.v_cache, v_base);
+        }
         if (!ok) {
           g += t;
           break;
@@ -459,50 +566,60 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (!ok) mbar_wait(smem_u32(&sm.k_full[g % kStages]), (g / kStages) & 1);
   } else {
-    // ---------------------- softmax / epilogue: two threads per row, one half each
-    constexpr int kCols = KT / 2;           // S columns of a thread
-    constexpr int kPk = KT / 4;             // its packed P columns
+    // ------------- softmax, a thread per row; output, by halves of the columns
     constexpr float kBias = BF ? 0.f : 6.f; // float16 P: up to 2^14, so that small weights stay clear of its smallest step
-    const int r = (warp & 3) * 32 + lane;   // TMEM lane (query row)
-    const int hf = warp >> 2;               // S columns [kCols hf, ..), O / Q columns by halves
-    const int pair_bar = 1 + (warp & 3);    // named barrier of warps w and w + 4 (same rows)
+    const int r = (warp & 3) * 32 + lane;   // TMEM lane
+    const int R = rank * kRows + r;         // query row of the tile
+    const int wg = warp >> 2;               // this warpgroup's tiles: gt & 1 == wg; its half of O's and Q's columns
     const int wq = warp & 3;
-    const int tok = r / P.G, g_ = r - tok * P.G;
+    const int tok = R / P.G, g_ = R - tok * P.G;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const float sc = a.sm_scale * 1.4426950408889634f;
     // a partial slot that no piece of this CTA fills is marked so
     int slots_used = 0;
-    // Q row half of a piece -> TMEM (packed, D / 4 columns; spare rows are zero)
+    // Q row half of a piece -> TMEM (packed, D / 4 columns), or shared memory (128B-swizzled); spare rows are zero
     auto load_q = [&](const Piece& u) {
       const bool row_ok = tok < u.ntok;
       const uint4* qrow = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(a.q) +
                                                          ((int64_t)(u.tok0 + (row_ok ? tok : 0)) * a.q_st +
                                                           (int64_t)(u.h * P.G + (row_ok ? g_ : 0)) * a.q_sh) * 2 +
-                                                         hf * D);
-#pragma unroll 1
-      for (int c = 0; c < D / 4; c += 16) {
-        uint32_t v[16];
+                                                         wg * D);
+      if (PAIR) {
+        uint4 x[D / 16];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint4 x = row_ok ? __ldg(qrow + c / 4 + q) : make_uint4(0u, 0u, 0u, 0u);
-          v[4 * q] = x.x;
-          v[4 * q + 1] = x.y;
-          v[4 * q + 2] = x.z;
-          v[4 * q + 3] = x.w;
+        for (int q = 0; q < D / 16; ++q) x[q] = row_ok ? __ldg(qrow + q) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int q = 0; q < D / 16; ++q) {
+          const int col = wg * (D / 16) + q;  // 16-byte piece of the row
+          *reinterpret_cast<uint4*>(smem + F::OFF_Q + (col >> 3) * (kRows * 128) + r * 128 + (((col ^ r) & 7) << 4)) = x[q];
         }
-        tmem_st16(tmem + lane_base + F::COL_Q + (D / 4) * hf + c, v);
+        fence_async_smem();
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < D / 4; c += 16) {
+          uint32_t v[16];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint4 x = row_ok ? __ldg(qrow + c / 4 + q) : make_uint4(0u, 0u, 0u, 0u);
+            v[4 * q] = x.x;
+            v[4 * q + 1] = x.y;
+            v[4 * q + 2] = x.z;
+            v[4 * q + 3] = x.w;
+          }
+          tmem_st16(tmem + lane_base + F::COL_Q + (D / 4) * wg + c, v);
+        }
+        tc_fence_before();
       }
-      tc_fence_before();
-      mbar_arrive(smem_u32(&sm.q_ready));
+      warp_arrive<PAIR>(sm.q_ready);
     };
     // pieces without keys give zero rows; true when u then holds a piece with some
     auto next_live = [&](Piece& u) {
-      while (next_piece<KT>(sm, P, w, w1, u)) {
+      while (next_piece(sm, P, w, w1, u)) {
         if (u.t1 > u.t0) return true;
         if (tok < u.ntok) {
           uint4* orow = reinterpret_cast<uint4*>(static_cast<unsigned char*>(a.o) +
                                                  ((int64_t)(u.tok0 + tok) * a.o_st + (int64_t)(u.h * P.G + g_) * a.o_sh) * 2 +
-                                                 hf * D);
+                                                 wg * D);
 #pragma unroll 4
           for (int q = 0; q < D / 16; ++q) orow[q] = make_uint4(0u, 0u, 0u, 0u);
         }
@@ -514,22 +631,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto clean_v = [&](const Piece& u, int t, int gt) -> bool {
       constexpr uint32_t kExp = BF ? 0x7F807F80u : 0x7C007C00u, kOne = BF ? 0x00800080u : 0x04000400u;
       const int j0 = (u.t0 + t) * KT, st = gt % kStages;
-      const bool got =
-          __all_sync(0xffffffffu, mbar_wait_or_abort(smem_u32(&sm.v_full[st]), (gt / kStages) & 1, abort_flag));
-      if (!got) {
-        if (lane == 0 && !*abort_flag) set_abort(sm, status);
-        return false;
-      }
+      if (!__all_sync(0xffffffffu, wait(sm.v_full[st], (gt / kStages) & 1, abort_flag))) return false;
       const int live = min(KT, u.L - j0);          // rows of real keys
       const bool scan = u.vis0 < j0 + live;        // some token does not see them all
-      unsigned char* vb = smem + (kStages + st) * kTile;
+      unsigned char* vb = smem + F::OFF_V + st * F::kVBytes;
       bool any = false;
+#pragma unroll 1
+      for (int c = 0; c < F::VC; ++c) {
 #pragma unroll
-      for (int c = 0; c < F::kChunks; ++c) {
-#pragma unroll
-        for (int i = 0; i < KT * 8; i += kSoftmax) {
-          uint4* q = reinterpret_cast<uint4*>(vb + c * kChunk) + i + tid;
-          if (i + tid >= live * 8) {
+        for (int i = 0; i < KT * 8; i += kSoftmax / 2) {
+          const int at = i + (tid & 127);
+          uint4* q = reinterpret_cast<uint4*>(vb + c * (KT * 128)) + at;
+          if (at >= live * 8) {
             *q = make_uint4(0u, 0u, 0u, 0u);
           } else if (scan) {
             uint4 x = *q;
@@ -548,7 +661,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      if (any) *reinterpret_cast<volatile int*>(&sm.odd[ui & 7]) = ui + 1;
+      if (any) {  // every row's epilogue, the other CTA's too
+        *reinterpret_cast<volatile int*>(&sm.odd[ui & 7]) = ui + 1;
+        if (PAIR) st_cluster(map_rank(smem_u32(&sm.odd[ui & 7]), rank ^ 1), ui + 1);
+      }
       fence_async_smem();  // these writes before the tensor core's reads
       return true;
     };
@@ -560,144 +676,148 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool row_ok = tok < u.ntok;
       const int T = u.t1 - u.t0;
       const int vis = max(0, min(u.L, u.vis0 + (row_ok ? tok : 0)));  // keys this row sees: j < vis
-      const bool busy = wq * 32 < u.ntok * P.G;                       // the warp holds rows
-      // A row's two warps meet at the same named barriers in the same order;
-      // every early exit is decided from outcomes both have exchanged there.
-      float m_used = -INFINITY, l = 0.f;
-      bool held = true;  // false: the last tile's V never came; told to the other warp at the next barrier
-      for (int t = 0; t < T; ++t) {
+      const bool busy = rank * kRows + wq * 32 < u.ntok * P.G;        // the warp holds rows
+      float m_used = -INFINITY, l = 0.f;  // this warpgroup's reference and part of the sum
+      for (int t = (g ^ wg) & 1; ok && t < T; t += 2) {
         const int gt = g + t, sb = gt & 1;
-        const bool got = __all_sync(0xffffffffu, held && mbar_wait_or_abort(smem_u32(&sm.s_full[sb]), (gt >> 1) & 1,
-                                                                           abort_flag));
-        // keys that every token of the tile sees need no mask (block-uniform)
-        const bool plain = (u.t0 + t + 1) * KT <= u.vis0 && (u.t0 + t + 1) * KT <= u.L;
-        if (!busy) {  // spare rows: whatever P holds stays in them
-          ok = got && (plain || clean_v(u, t, gt));
-          if (!ok) break;
-          mbar_arrive(smem_u32(&sm.p_full[sb]));
-          continue;
-        }
-        float x[kCols];
-        if (got) {
-          tc_fence_after();
-#pragma unroll
-          for (int c = 0; c < kCols / 32; ++c) {
-            float(&xc)[32] = *reinterpret_cast<float(*)[32]>(&x[32 * c]);
-            tmem_ld32(tmem + lane_base + F::COL_S + KT * sb + kCols * hf + 32 * c, xc);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < kCols; ++i) x[i] = 0.f;
-        }
-        const int j0 = (u.t0 + t) * KT + kCols * hf;
-        // x stays raw: P = 2^(x sc - m)
-        float tmax = -INFINITY;
-        if (!plain) {
-#pragma unroll
-          for (int i = 0; i < kCols; ++i)
-            if (j0 + i >= vis) x[i] = -INFINITY;
-        }
-#pragma unroll
-        for (int i = 0; i < kCols; ++i) tmax = fmaxf(tmax, x[i]);
-        tmax *= sc;
-        sm.xmax[sb][hf][r] = tmax;
-        if (lane == 0) sm.okx[sb][hf][wq] = got;
-        // the barrier also orders this half's S reads before the other half's P
-        // stores (half 1 writes P over S columns that half 0 reads)
-        tc_fence_before();
-        named_bar(pair_bar, 64);
-        tc_fence_after();
-        tmax = fmaxf(tmax, sm.xmax[sb][hf ^ 1][r]);
-        ok = got && sm.okx[sb][hf ^ 1][wq];
+        ok = __all_sync(0xffffffffu, wait(sm.s_full[sb], (gt >> 1) & 1, abort_flag));
         if (!ok) break;
-        // a row moves its reference max only when the tile max exceeds it by
-        // more than 8 (P <= 2^8 otherwise); O then scales by 2^(old - new)
-        const bool grow = tmax > m_used + 8.f;
-        if (__any_sync(0xffffffffu, grow)) {
-          const float m_new = grow ? tmax : m_used;
-          if (t > 0) {
-            // O holds P V of this unit's earlier tiles: wait for the last, then rescale this half row
-            const bool done = __all_sync(0xffffffffu,
-                                         mbar_wait_or_abort(smem_u32(&sm.o_done), (gt - 1) & 1, abort_flag));
-            if (lane == 0) sm.okr[sb][hf][wq] = done;
-            named_bar(pair_bar, 64);
-            ok = done && sm.okr[sb][hf ^ 1][wq];
+        // keys that every token of the tile sees need no mask (uniform)
+        const int j0 = (u.t0 + t) * KT;
+        const bool plain = j0 + KT <= u.vis0 && j0 + KT <= u.L;
+        const uint32_t ts = tmem + lane_base + F::COL_S + KT * sb;
+        float x[64];
+        float tmax = -INFINITY;
+        auto mask = [&](float* xs, int j, int n) {
+          if (plain) return;
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (i < n && j + i >= vis) xs[i] = -INFINITY;
+        };
+        if (busy) {
+          tc_fence_after();
+          float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll 1
+          for (int c = 0; c < KT; c += 64) {
+            tmem_ld64(ts + c, x);
+            mask(x, j0 + c, 64);
+#pragma unroll
+            for (int i = 0; i < 64; i += 4) {
+              mx[0] = fmaxf(fmaxf(mx[0], x[i]), x[i + 1]);
+              mx[1] = fmaxf(fmaxf(mx[1], x[i + 2]), x[i + 3]);
+            }
+          }
+          // x stays raw: P = 2^(x sc - m)
+          tmax = fmaxf(mx[0], mx[1]) * sc;
+        }
+        // the reference after tile gt - 1 (of a unit's first tile only the order counts)
+        if (gt > 0) ok = __all_sync(0xffffffffu, wait(sm.m_ready[(gt - 1) & 1][wq], ((gt - 1) >> 1) & 1, abort_flag));
+        if (!ok) break;
+        const float m_old = t > 0 ? sm.m[r] : -INFINITY;
+        // a row moves it only when the tile's maximum exceeds it by more than 8
+        // (P <= 2^8 otherwise); O then scales by 2^(old - new)
+        const bool grow = tmax > m_old + 8.f;
+        const float m_new = grow ? tmax : m_old;
+        sm.m[r] = m_new;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sm.m_ready[gt & 1][wq]));
+        if (busy) {
+          if (t > 0 && __any_sync(0xffffffffu, grow)) {
+            // O holds P V of this unit's earlier tiles: wait for the last, then rescale the row
+            ok = __all_sync(0xffffffffu, wait(sm.pv_done[(gt - 1) & 1], ((gt - 1) >> 1) & 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
-            const float alpha = grow ? ex2(m_used - m_new) : 1.f;
+            const float alpha = grow ? ex2(m_old - m_new) : 1.f;
 #pragma unroll 1
-            for (int c = 0; c < D / 64; ++c) {
+            for (int c = 0; c < D / 32; ++c) {
               float v[32];
-              tmem_ld32(tmem + lane_base + F::COL_O + (D / 2) * hf + 32 * c, v);
+              tmem_ld32(tmem + lane_base + F::COL_O + 32 * c, v);
 #pragma unroll
               for (int i = 0; i < 32; ++i) v[i] *= alpha;
-              tmem_st32(tmem + lane_base + F::COL_O + (D / 2) * hf + 32 * c, v);
+              tmem_st32(tmem + lane_base + F::COL_O + 32 * c, v);
             }
-            l *= alpha;
           }
-          m_used = m_new;
-        }
-        uint32_t pk[kPk];
-        f32x2 sum2 = pk2(0.f, 0.f);
-        // a row whose scores so far are all -inf has no reference yet: its P is 0
-        const float nm = (m_used == -INFINITY && !plain) ? 0.f : kBias - m_used;
-        const f32x2 sc2 = pk2(sc, sc), nm2 = pk2(nm, nm);
+          if (m_new != m_used) {
+            l *= m_used == -INFINITY ? 1.f : ex2(m_used - m_new);  // without a reference l is 0 or NaN
+            m_used = m_new;
+          }
+          // a row whose scores so far are all -inf has no reference yet: its P is 0
+          const float nm = (m_used == -INFINITY && !plain) ? 0.f : kBias - m_used;
+          const f32x2 sc2 = pk2(sc, sc), nm2 = pk2(nm, nm);
+          f32x2 sum2[2] = {pk2(0.f, 0.f), pk2(0.f, 0.f)};
+          float(&xa)[32] = *reinterpret_cast<float(*)[32]>(&x[0]);
+          float(&xb)[32] = *reinterpret_cast<float(*)[32]>(&x[32]);
+          // 32 columns of S to 16 of P, over columns that have been read
+          auto weigh = [&](float(&xs)[32], int c) {
+            mask(xs, j0 + c, 32);
+            uint32_t pk[16];
 #pragma unroll
-        for (int i = 0; i < kPk; ++i) {
-          float e0, e1;
-          upk2(fma2(pk2(x[2 * i], x[2 * i + 1]), sc2, nm2), e0, e1);
-          const float p0 = ex2(e0), p1 = ex2(e1);
-          sum2 = add2(sum2, pk2(p0, p1));
-          pk[i] = pack2<BF>(p0, p1);
+            for (int i = 0; i < 16; ++i) {
+              float e0, e1;
+              upk2(fma2(pk2(xs[2 * i], xs[2 * i + 1]), sc2, nm2), e0, e1);
+              const float p0 = ex2(e0), p1 = ex2(e1);
+              sum2[i & 1] = add2(sum2[i & 1], pk2(p0, p1));
+              pk[i] = pack2<BF>(p0, p1);
+            }
+            tmem_st16_async(ts + c / 2, pk);
+          };
+          tmem_ld32_async(ts, xa);
+          tmem_ld_wait(xa);
+#pragma unroll 1
+          for (int c = 0; c < KT; c += 64) {
+            tmem_ld32_async(ts + c + 32, xb);
+            weigh(xa, c);
+            tmem_ld_wait(xb);
+            if (c + 64 < KT) tmem_ld32_async(ts + c + 64, xa);
+            weigh(xb, c + 32);
+            tmem_ld_wait(xa);
+          }
+          tmem_st_wait();
+          float s0, s1;
+          upk2(add2(sum2[0], sum2[1]), s0, s1);
+          l += s0 + s1;
         }
-        float s0, s1;
-        upk2(sum2, s0, s1);
-        l += s0 + s1;
-        // P (pairs) over columns [kPk hf, kPk hf + kPk) of its own S buffer
-#pragma unroll
-        for (int c = 0; c < kPk / 16; ++c) {
-          const uint32_t(&pc)[16] = *reinterpret_cast<const uint32_t(*)[16]>(&pk[16 * c]);
-          tmem_st16(tmem + lane_base + F::COL_S + KT * sb + kPk * hf + 16 * c, pc);
-        }
-        held = plain || clean_v(u, t, gt);
+        ok = plain || clean_v(u, t, gt);
+        if (!ok) break;
         tc_fence_before();
-        if (held) mbar_arrive(smem_u32(&sm.p_full[sb]));
+        warp_arrive<PAIR>(sm.p_full[sb]);  // spare rows: whatever P holds stays in them
       }
       if (!ok) break;
+      sm.ml[ui & 1][wg][r] = make_float2(m_used, l);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sm.l_ready));
       g += T;
-      // every S MMA of this unit has been consumed: the next unit's Q may go in
+      // once every S MMA of this unit has retired the next unit's Q may go in
+      ok = __all_sync(0xffffffffu, wait(sm.s_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag));
+      if (!ok) break;
+      tc_fence_after();
       more = next_live(p);
       if (more) load_q(p);
       // ---- epilogue: wait for this unit's last P V, then O (or its partial) out
-      const bool got =
-          __all_sync(0xffffffffu, held && mbar_wait_or_abort(smem_u32(&sm.o_full), ui & 1, abort_flag));
+      ok = __all_sync(0xffffffffu, wait(sm.l_ready, ui & 1, abort_flag) && wait(sm.o_full, ui & 1, abort_flag));
       tc_fence_after();
-      if (busy) {
-        sm.lsum[hf][r] = l;
-        if (lane == 0) sm.oke[hf][wq] = got;
-        named_bar(pair_bar, 64);
-        l = sm.lsum[0][r] + sm.lsum[1][r];
-        ok = got && sm.oke[hf ^ 1][wq];
-      } else {
-        ok = got;
+      if (ok) {
+        const float2 x0 = sm.ml[ui & 1][0][r], x1 = sm.ml[ui & 1][1][r];
+        m_used = fmaxf(x0.x, x1.x);  // references never fall: the later one, which O is scaled by
+        l = m_used == -INFINITY ? x0.y + x1.y : x0.y * ex2(x0.x - m_used) + x1.y * ex2(x1.x - m_used);
       }
       if (ok && busy) {
-        const int64_t prow = ((int64_t)(2 * blockIdx.x + (u.slot < 0 ? 0 : u.slot))) * kRows + r;
+        const int64_t prow = (int64_t)(2 * worker + max(u.slot, 0)) * (kRows * CG) + R;
         const float inv = l == 0.f ? 0.f : 1.f / l;
         unsigned char* orow = static_cast<unsigned char*>(a.o) +
-                              ((int64_t)(u.tok0 + tok) * a.o_st + (int64_t)(u.h * P.G + g_) * a.o_sh) * 2 + hf * D;
+                              ((int64_t)(u.tok0 + tok) * a.o_st + (int64_t)(u.h * P.G + g_) * a.o_sh) * 2 + wg * D;
         const bool odd = sm.odd[ui & 7] == ui + 1;
 #pragma unroll 1
         for (int c = 0; c < D / 64; ++c) {
           float v[32];
-          tmem_ld32(tmem + lane_base + F::COL_O + (D / 2) * hf + 32 * c, v);
+          tmem_ld32(tmem + lane_base + F::COL_O + (D / 2) * wg + 32 * c, v);
           if (odd) {
             // the masked tiles' non-finite values, for the rows that see their keys
             for (int j = max(0, min(u.vis0, u.t1 * KT) / KT * KT); j < min(u.t1 * KT, vis); ++j) {
               if (j < u.t0 * KT) continue;
               const int64_t s = a.kv_indices[sm.kv[u.b] + j];
               if (s < 0 || s >= a.n_slots) continue;
-              const uint16_t* vr = static_cast<const uint16_t*>(a.v_cache) + s * a.kv_st + u.h * a.kv_sh + (D / 2) * hf + 32 * c;
+              const uint16_t* vr = static_cast<const uint16_t*>(a.v_cache) + s * a.kv_st + u.h * a.kv_sh + (D / 2) * wg + 32 * c;
               for (int i = 0; i < 32; ++i) {
                 const float y = unpack<BF>(vr[i]);
                 if (!(fabsf(y) < INFINITY)) {
@@ -718,12 +838,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                                   pack2<BF>(v[8 * q + 4] * inv, v[8 * q + 5] * inv),
                                   pack2<BF>(v[8 * q + 6] * inv, v[8 * q + 7] * inv));
           } else {
-            float4* dst = reinterpret_cast<float4*>(P.ws_o + prow * D + (D / 2) * hf + 32 * c);
+            float4* dst = reinterpret_cast<float4*>(P.ws_o + prow * D + (D / 2) * wg + 32 * c);
 #pragma unroll
             for (int q = 0; q < 8; ++q) dst[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
           }
         }
-        if (u.slot >= 0 && hf == 0 && row_ok) {
+        if (u.slot >= 0 && wg == 0 && row_ok) {
           P.ws_ml[2 * prow] = m_used;
           P.ws_ml[2 * prow + 1] = l;
         }
@@ -731,36 +851,38 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok) {
         if (u.slot >= 0) {
           slots_used |= 1 << u.slot;
-          if (tid == 0)
-            P.ws_meta[2 * blockIdx.x + u.slot] = make_int4(1 | (u.last ? 2 : 0), u.tok0, u.ntok, u.h);
+          if (tid == 0 && rank == 0)
+            P.ws_meta[2 * worker + u.slot] = make_int4(1 | (u.last ? 2 : 0), u.tok0, u.ntok, u.h);
         }
         // O may now be overwritten by the next unit's first P V
         tc_fence_before();
-        mbar_arrive(smem_u32(&sm.o_free));
+        warp_arrive<PAIR>(sm.o_free);
       }
       ++ui;
     }
-    if (tid == 0)
+    if (tid == 0 && rank == 0)
       for (int s = 0; s < 2; ++s)
-        if (!(slots_used >> s & 1)) P.ws_meta[2 * blockIdx.x + s] = make_int4(0, 0, 0, 0);
+        if (!(slots_used >> s & 1)) P.ws_meta[2 * worker + s] = make_int4(0, 0, 0, 0);
     if (!ok && !*abort_flag) set_abort(sm, status);
   }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync();  // nothing of the other CTA's arrives here any more
   if (warp == kCtlWarp) {
     tc_fence_after();
-    tmem_dealloc(tmem, kTmemCols);
+    if (PAIR) tmem_dealloc_2(tmem, kTmemCols);
+    else tmem_dealloc(tmem, kTmemCols);
   }
 }
 
-// Merge the partials of the unit that CTA c begins and leaves unfinished: its
-// own, then the continuing slots of the CTAs after it up to the unit's last.
+// Merge the partials of the unit that worker c begins and leaves unfinished: its
+// own, then the continuing slots of the workers after it up to the unit's last.
 //   o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s
 constexpr int kMergeThreads = 256, kMergeY = 8;
 template <bool BF, int D>
 __global__ void __launch_bounds__(kMergeThreads) chunk_attn_merge(const __grid_constant__ Params P) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  constexpr int kLanes = D / 4, kPass = kMergeThreads / kLanes;
+  constexpr int kLanes = D / 4, kPass = kMergeThreads / kLanes, kSlotRows = kRows * Cfg<D>::CG;
   __shared__ int list[kMergeThreads + 1], flags[kMergeThreads], n_list;
   const int c = blockIdx.x, grid = gridDim.x;
   const int4 meta = P.ws_meta[2 * c + 1];
@@ -785,12 +907,12 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_attn_merge(const __grid_c
   for (int r = blockIdx.y * kPass + threadIdx.x / kLanes; r < rows; r += kMergeY * kPass) {
     float M = -INFINITY;
 #pragma unroll 4
-    for (int k = 0; k < n; ++k) M = fmaxf(M, P.ws_ml[2 * ((int64_t)list[k] * kRows + r)]);
+    for (int k = 0; k < n; ++k) M = fmaxf(M, P.ws_ml[2 * ((int64_t)list[k] * kSlotRows + r)]);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float L = 0.f;
 #pragma unroll 4
     for (int k = 0; k < n; ++k) {
-      const int64_t prow = (int64_t)list[k] * kRows + r;
+      const int64_t prow = (int64_t)list[k] * kSlotRows + r;
       const float2 ml = reinterpret_cast<const float2*>(P.ws_ml)[prow];
       const float4 v = reinterpret_cast<const float4*>(P.ws_o + prow * D)[e];
       // a sum of 0: the row sees none of these keys (a NaN sum goes on)
@@ -838,21 +960,22 @@ int check_args(const dft_chunk_attn_args* a) {
   return DFT_OK;
 }
 
-// one CTA per SM; the merge keeps a flag per CTA
-int grid_size() {
-  const int n = gtile::sm_count();
+// one CTA per SM; the merge keeps a flag per worker
+int worker_count(int D) {
+  const int n = gtile::sm_count() / (D == 256 ? Cfg<256>::CG : 1);
   return n < kMergeThreads ? n : kMergeThreads;
 }
 
 struct Workspace {
   int64_t o, ml, meta, total;
 };
-Workspace workspace(const dft_chunk_attn_args* a, int grid) {
+Workspace workspace(const dft_chunk_attn_args* a, int workers) {
+  const int64_t slots = 2 * (int64_t)workers, rows = slots * kRows * (a->D == 256 ? Cfg<256>::CG : 1);
   Workspace w;
   w.meta = 0;
-  w.ml = up256(2 * (int64_t)grid * sizeof(int4));
-  w.o = w.ml + up256(2 * (int64_t)grid * kRows * 2 * sizeof(float));
-  w.total = w.o + 2 * (int64_t)grid * kRows * a->D * sizeof(float);
+  w.ml = up256(slots * sizeof(int4));
+  w.o = w.ml + up256(rows * 2 * sizeof(float));
+  w.total = w.o + rows * a->D * sizeof(float);
   return w;
 }
 
@@ -869,18 +992,29 @@ bool encode(CUtensorMap* m, const dft_chunk_attn_args* a, const void* base, bool
 }
 
 template <bool BF, int D>
-int launch(const Params& P, int grid, const CUtensorMap& k_map, const CUtensorMap& v_map, int32_t* status,
+int launch(const Params& P, int workers, const CUtensorMap& k_map, const CUtensorMap& v_map, int32_t* status,
            cudaStream_t st) {
   DFT_CUDA_CHECK(cudaFuncSetAttribute(chunk_attn_kernel<BF, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)smem_bytes<D>()));
-  chunk_attn_kernel<BF, D><<<(unsigned)grid, kThreads, smem_bytes<D>(), st>>>(k_map, v_map, P, status);
-  DFT_LAUNCH_CHECK();
   cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[1];
   memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3((unsigned)grid, kMergeY);
+  cfg.gridDim = dim3((unsigned)(workers * Cfg<D>::CG));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem_bytes<D>();
+  cfg.stream = st;
+  cfg.attrs = attr;
+  if (Cfg<D>::kPair) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+  }
+  DFT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, chunk_attn_kernel<BF, D>, k_map, v_map, P, status));
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((unsigned)workers, kMergeY);
   cfg.blockDim = dim3(kMergeThreads);
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
@@ -894,7 +1028,7 @@ int launch(const Params& P, int grid, const CUtensorMap& k_map, const CUtensorMa
 extern "C" int64_t dft_chunk_attn_workspace_bytes(const dft_chunk_attn_args* a) {
   if (check_args(a)) return -1;
   if (a->B == 0 || a->T == 0) return 0;
-  return workspace(a, grid_size()).total;
+  return workspace(a, worker_count(a->D)).total;
 }
 
 extern "C" int dft_chunk_attn(const dft_chunk_attn_args* a, void* ws, int32_t* dev_status, void* stream) {
@@ -902,13 +1036,13 @@ extern "C" int dft_chunk_attn(const dft_chunk_attn_args* a, void* ws, int32_t* d
   if (rc) return rc;
   if (a->B == 0 || a->T == 0) return DFT_OK;
   if (!ws || !al16(ws)) return DFT_ERR_INVALID;
-  const int grid = grid_size();
-  const Workspace w = workspace(a, grid);
+  const int workers = worker_count(a->D);
+  const Workspace w = workspace(a, workers);
   Params P;
   memset(&P, 0, sizeof(P));
   P.a = *a;
   P.G = a->Hq / a->Hkv;
-  P.TQ = kRows / P.G;
+  P.TQ = kRows * (a->D == 256 ? Cfg<256>::CG : 1) / P.G;
   const bool inner = (a->Hkv - 1) * a->kv_sh + a->D <= a->kv_st;
   P.x_head = inner ? (int)a->kv_sh : 0;
   P.row_head = inner ? 0 : (int)(a->kv_sh / a->kv_st);
@@ -920,7 +1054,7 @@ extern "C" int dft_chunk_attn(const dft_chunk_attn_args* a, void* ws, int32_t* d
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool bf = a->dtype == DFT_BF16;
 #define DFT_GO(D_) \
-  return bf ? launch<true, D_>(P, grid, k_map, v_map, dev_status, st) : launch<false, D_>(P, grid, k_map, v_map, dev_status, st)
+  return bf ? launch<true, D_>(P, workers, k_map, v_map, dev_status, st) : launch<false, D_>(P, workers, k_map, v_map, dev_status, st)
   if (a->D == 64) DFT_GO(64);
   if (a->D == 128) DFT_GO(128);
   DFT_GO(256);
