@@ -148,17 +148,6 @@ __device__ __forceinline__ void set_abort(Small& sm, int32_t* status) {
 __device__ __forceinline__ bool wait(uint64_t& bar, uint32_t parity, const volatile int* abort) {
   return mbar_try(smem_u32(&bar), parity) || mbar_wait_or_abort(smem_u32(&bar), parity, abort);
 }
-// The same for barriers that the pair's other CTA arrives on.
-template <bool PAIR>
-__device__ __forceinline__ bool wait_pair(uint64_t& bar, uint32_t parity, const volatile int* abort) {
-  if (!PAIR) return wait(bar, parity, abort);
-  if (mbar_try_cluster(smem_u32(&bar), parity)) return true;
-  const long long t0 = clock64();
-  while (!mbar_try_cluster(smem_u32(&bar), parity)) {
-    if (*abort || clock64() - t0 > 2000000000ll) return false;
-  }
-  return true;
-}
 // Arrive, once per warp and after all of its lanes, on the barrier of the CTA
 // that issues the MMAs.
 template <bool PAIR>
@@ -376,12 +365,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       while (ok && next_piece(sm, P, w, w1, p)) {
         const int T = p.t1 - p.t0;
         if (T == 0) continue;
-        ok = all(wait_pair<PAIR>(sm.q_ready, ui & 1, abort_flag));
+        ok = all(wait(sm.q_ready, ui & 1, abort_flag));
         for (int t = 0; ok && t <= T; ++t) {
           if (t < T) {
             const int gt = g + t, st = gt % kStages, sb = gt & 1;
             bool got = wait(sm.k_full[st], (gt / kStages) & 1, abort_flag);
-            if (PAIR) got = got && wait_pair<PAIR>(sm.k_peer[st], (gt / kStages) & 1, abort_flag);
+            if (PAIR) got = got && wait(sm.k_peer[st], (gt / kStages) & 1, abort_flag);
             if (got && gt >= 2) got = wait(sm.pv_done[sb], (gt / 2 - 1) & 1, abort_flag);  // P of tile gt - 2 is read
             ok = all(got);
             if (!ok) break;
@@ -403,10 +392,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (t >= 1) {
             const int gu = g + t - 1, st = gu % kStages, pb = gu & 1;
             bool got = wait(sm.v_full[st], (gu / kStages) & 1, abort_flag);
-            if (PAIR) got = got && wait_pair<PAIR>(sm.v_peer[st], (gu / kStages) & 1, abort_flag);
+            if (PAIR) got = got && wait(sm.v_peer[st], (gu / kStages) & 1, abort_flag);
             // the first P V of a unit overwrites O: the previous unit's epilogue has read it
-            if (got && t == 1 && ui > 0) got = wait_pair<PAIR>(sm.o_free, (ui - 1) & 1, abort_flag);
-            ok = all(got && wait_pair<PAIR>(sm.p_full[pb], (gu >> 1) & 1, abort_flag));
+            if (got && t == 1 && ui > 0) got = wait(sm.o_free, (ui - 1) & 1, abort_flag);
+            ok = all(got && wait(sm.p_full[pb], (gu >> 1) & 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
             if (sm.v_mixed[st]) fence_async_smem();

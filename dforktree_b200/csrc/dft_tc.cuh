@@ -316,22 +316,15 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
+// No cluster-scope release: with it a fence of the thread's every access came
+// before each arrival.  What these arrivals hand over is ordered by tcgen05 and
+// proxy fences.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+// one word into the cluster's other CTA, seen there by whoever acquires after a later arrival
 __device__ __forceinline__ void st_cluster(uint32_t cluster_addr, uint32_t v) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
-}
-__device__ __forceinline__ bool mbar_try_cluster(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
+  asm volatile("st.shared::cluster.u32 [%0], %1;\n\tfence.acq_rel.cluster;" ::"r"(cluster_addr), "r"(v) : "memory");
 }
 // Issued by the lane with `lead` set (elect_lane), in code that the whole warp
 // runs: descriptors then stay in uniform registers.  Under a branch of one lane
