@@ -59,16 +59,19 @@ namespace {
 
 constexpr int kMaxB = 1024;
 constexpr int kRows = 128;        // query rows of a CTA
-constexpr int KT = 128;           // keys per tile
 constexpr int kSoftmax = 256;     // two warpgroups, a thread per query row in each
-constexpr int kCtlWarp = 8, kProdWarp0 = 9, kProdWarps = 3, kProducers = 32 * kProdWarps;
+constexpr int kCtlWarp = 8, kProdWarp0 = 9, kProdWarps = 3;
 constexpr int kThreads = 384;     // twelve warps leave 168 registers a thread
 constexpr uint32_t kTmemCols = 512;
+constexpr int kMaxStages = 12;
 // A unit's fixed cost in keys (query load, first tile's latency, output), and
 // the least share of a worker: under it a cut costs more than it spreads.
 constexpr int kUnitKeys = 256;
 constexpr int kMinShare = 384;
 
+#ifndef DFT_KT
+#define DFT_KT(D) 128
+#endif
 template <int N>
 using Int = std::integral_constant<int, N>;
 
@@ -76,7 +79,9 @@ template <int D>
 struct Cfg {
   static constexpr bool kPair = D == 256;
   static constexpr int CG = kPair ? 2 : 1;                    // CTAs of a worker
-  static constexpr int kStages = kPair ? 2 : D == 128 ? 3 : 6;
+  static constexpr int KT = DFT_KT(D);                        // keys per tile
+  static constexpr int NB = KT == 64 ? 4 : 2;                 // S / P buffers
+  static constexpr int kStages = (D == 64 ? 6 : kPair ? 2 : 3) * (128 / KT);
   static constexpr int KR = KT / CG, KC = D / 64;             // K rows and 64-dim chunks in this CTA
   static constexpr int VC = D / 64 / CG;                      // V chunks in this CTA (all KT rows)
   static constexpr uint32_t kKBytes = KR * KC * 128, kVBytes = KT * VC * 128;
@@ -84,14 +89,14 @@ struct Cfg {
   static constexpr uint32_t OFF_V = kStages * kKBytes, OFF_Q = OFF_V + kStages * kVBytes;
   static constexpr uint32_t OFF_SMALL = OFF_Q + kQBytes;
   static constexpr uint32_t COL_O = 0, COL_Q = D, COL_S = kPair ? D : D + D / 2;  // S / P buffer b at COL_S + KT b
-  static_assert(COL_S + 2 * KT <= kTmemCols, "TMEM");
+  static_assert(COL_S + NB * KT <= kTmemCols, "TMEM");
 };
 
 struct Small {
   uint64_t q_ready;
-  uint64_t k_full[6], k_empty[6], v_full[6], v_empty[6];
-  uint64_t k_peer[2], v_peer[2];  // the other CTA's half of the stage (rank 0 of a pair)
-  uint64_t s_full[2], p_full[2], pv_done[2];
+  uint64_t k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages];
+  uint64_t k_peer[kMaxStages], v_peer[kMaxStages];  // the other CTA's part of the stage (rank 0 of a pair)
+  uint64_t s_full[4], p_full[4], pv_done[4];
   uint64_t m_ready[2][4];   // [tile & 1][row warp]: the tile's reference is in m
   uint64_t l_ready, o_full, o_free, mma_done;
   uint32_t tmem_base;
@@ -102,14 +107,13 @@ struct Small {
   int64_t warp_sum[kThreads / 32];
   int64_t pre[kMaxB + 1];   // cost of the requests before b
   int qo[kMaxB + 1], kv[kMaxB + 1];
-  int slots[kProdWarps][KT];
-  int k_mixed[6], v_mixed[6];  // [stage]: the CTA's part holds rows copied by cp.async
+  int slots[kProdWarps][128];
+  int k_mixed[kMaxStages], v_mixed[kMaxStages];  // [stage]: the CTA's part holds rows copied by cp.async
 };
 
 struct Params {
   dft_chunk_attn_args a;
   int G, TQ;                // q-heads per kv-head, tokens per query tile
-  int x_head, row_head;     // kv-head h starts at column h * x_head, row h * row_head of the tensor map
   float* ws_o;              // [2 workers][rows][D] partial O: slot 2c continues a unit, 2c + 1 begins one
   float* ws_ml;             // [2 workers][rows][2] partial (m, l)
   int4* ws_meta;            // [2 workers] (flags, first token row, tokens, kv-head); flags 1: used, 2: the unit's last
@@ -159,13 +163,6 @@ __device__ __forceinline__ void warp_arrive(uint64_t& bar) {
   }
 }
 
-// 64 columns of this thread's TMEM lane
-__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
-  tmem_ld32_async(taddr, &v[0]);
-  tmem_ld32_async(taddr + 32, &v[32]);
-  tmem_ld_wait(v);
-}
-
 // -------------------------------------------------------------- schedule --
 // Request b: n tokens in nt query tiles, L keys.  Tile i ends at token e =
 // min((i + 1) TQ, n) and reads the keys its last token sees, clamp(L - n + e,
@@ -206,6 +203,7 @@ struct Piece {
 };
 
 // The next piece of the line from w, w < w1, that has something to do.
+template <int KT>
 __device__ __forceinline__ bool next_piece(const Small& sm, const Params& P, int64_t& w, int64_t w1, Piece& p) {
   while (w < w1) {
     int lo = 0, hi = P.a.B;  // pre[lo] <= w < pre[hi]
@@ -253,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                       const __grid_constant__ Params P, int32_t* status) {
   using F = Cfg<D>;
   constexpr bool PAIR = F::kPair;
-  constexpr int kStages = F::kStages, CG = F::CG;
+  constexpr int KT = F::KT, NB = F::NB, kAhead = NB - 1, kStages = F::kStages, CG = F::CG;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   Small& sm = *reinterpret_cast<Small*>(smem + F::OFF_SMALL);
@@ -270,18 +268,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       mbar_init(smem_u32(&sm.q_ready), kSoftmax / 32 * CG);
       for (int i = 0; i < kStages; ++i) {
-        mbar_init(smem_u32(&sm.k_full[i]), kProducers + 1);
-        mbar_init(smem_u32(&sm.k_empty[i]), 1);
-        mbar_init(smem_u32(&sm.v_full[i]), kProducers + 1);
-        mbar_init(smem_u32(&sm.v_empty[i]), 1);
-      }
-      for (int i = 0; i < 2; ++i) {
         mbar_init(smem_u32(&sm.k_peer[i]), 1);
         mbar_init(smem_u32(&sm.v_peer[i]), 1);
+        mbar_init(smem_u32(&sm.k_full[i]), 64 + 1);
+        mbar_init(smem_u32(&sm.k_empty[i]), 1);
+        mbar_init(smem_u32(&sm.v_full[i]), 64 + 1);
+        mbar_init(smem_u32(&sm.v_empty[i]), 1);
+      }
+      for (int i = 0; i < 4; ++i) {
         mbar_init(smem_u32(&sm.s_full[i]), 1);
         mbar_init(smem_u32(&sm.p_full[i]), kSoftmax / 64 * CG);
         mbar_init(smem_u32(&sm.pv_done[i]), 1);
-        for (int j = 0; j < 4; ++j) mbar_init(smem_u32(&sm.m_ready[i][j]), 1);
+        mbar_init(smem_u32(&sm.m_ready[0][i]), 1);
+        mbar_init(smem_u32(&sm.m_ready[1][i]), 1);
       }
       mbar_init(smem_u32(&sm.l_ready), kSoftmax / 32);
       mbar_init(smem_u32(&sm.o_full), 1);
@@ -362,16 +361,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t q_base = k_base + F::OFF_Q;
       int g = 0, ui = 0;
       bool ok = true;
-      while (ok && next_piece(sm, P, w, w1, p)) {
+      while (ok && next_piece<KT>(sm, P, w, w1, p)) {
         const int T = p.t1 - p.t0;
         if (T == 0) continue;
         ok = all(wait(sm.q_ready, ui & 1, abort_flag));
-        for (int t = 0; ok && t <= T; ++t) {
+        for (int t = 0; ok && t < T + kAhead; ++t) {
           if (t < T) {
-            const int gt = g + t, st = gt % kStages, sb = gt & 1;
+            const int gt = g + t, st = gt % kStages, sb = gt % NB;
             bool got = wait(sm.k_full[st], (gt / kStages) & 1, abort_flag);
             if (PAIR) got = got && wait(sm.k_peer[st], (gt / kStages) & 1, abort_flag);
-            if (got && gt >= 2) got = wait(sm.pv_done[sb], (gt / 2 - 1) & 1, abort_flag);  // P of tile gt - 2 is read
+            if (got && gt >= NB) got = wait(sm.pv_done[sb], (gt / NB - 1) & 1, abort_flag);  // P of tile gt - NB is read
             ok = all(got);
             if (!ok) break;
             tc_fence_after();
@@ -380,7 +379,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t ds = __shfl_sync(0xffffffffu, tmem + F::COL_S + KT * sb, 0);
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
-              const uint64_t bd = sw128_desc(kb + (k >> 2) * (F::KR * 128) + (k & 3) * 32);
+              // 8-key groups KC KB apart, a group's 64-dim chunks 1 KB apart
+              const uint64_t bd = sw128_desc(kb + (k >> 2) * 1024 + (k & 3) * 32, 16, F::KC * 1024);
               if (PAIR)
                 mma_ss<CG>(lead, ds, sw128_desc(q_base + (k >> 2) * (kRows * 128) + (k & 3) * 32), bd, id_s, k > 0);
               else
@@ -389,28 +389,28 @@ __global__ void __launch_bounds__(kThreads, 1)
             commit(sm.k_empty[st]);
             commit(sm.s_full[sb]);
           }
-          if (t >= 1) {
-            const int gu = g + t - 1, st = gu % kStages, pb = gu & 1;
+          if (t >= kAhead) {
+            const int gu = g + t - kAhead, st = gu % kStages, pb = gu % NB;
             bool got = wait(sm.v_full[st], (gu / kStages) & 1, abort_flag);
             if (PAIR) got = got && wait(sm.v_peer[st], (gu / kStages) & 1, abort_flag);
             // the first P V of a unit overwrites O: the previous unit's epilogue has read it
-            if (got && t == 1 && ui > 0) got = wait(sm.o_free, (ui - 1) & 1, abort_flag);
-            ok = all(got && wait(sm.p_full[pb], (gu >> 1) & 1, abort_flag));
+            if (got && t == kAhead && ui > 0) got = wait(sm.o_free, (ui - 1) & 1, abort_flag);
+            ok = all(got && wait(sm.p_full[pb], (gu / NB) & 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
             if (sm.v_mixed[st]) fence_async_smem();
             const uint32_t vb = __shfl_sync(0xffffffffu, v_base + st * F::kVBytes, 0);
             const uint32_t ps = __shfl_sync(0xffffffffu, tmem + F::COL_S + KT * pb, 0);
-            const uint32_t keep = __shfl_sync(0xffffffffu, t > 1 ? 1u : 0u, 0);
+            const uint32_t keep = __shfl_sync(0xffffffffu, t > kAhead ? 1u : 0u, 0);
 #pragma unroll
             for (int k = 0; k < KT / 16; ++k) {
-              // V [keys x dims] is MN-major: 64-dim chunks KT rows apart, 8-key groups 1 KB apart
-              const uint64_t bd = sw128_desc(vb + k * 16 * 128, KT * 128, 1024);
+              // V [keys x dims] is MN-major: of 16 keys, 64-dim chunks 2 KB apart, 8-key groups 1 KB apart
+              const uint64_t bd = sw128_desc(vb + k * F::VC * 2048, 2048, 1024);
               mma_ts<CG>(lead, tmem + F::COL_O, ps + 8 * k, bd, id_o, k > 0 ? 1u : keep);
             }
             commit(sm.v_empty[st]);
             commit(sm.pv_done[pb]);
-            if (t == T) commit(sm.o_full);
+            if (t == T + kAhead - 1) commit(sm.o_full);
           }
         }
         g += T;
@@ -423,18 +423,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       // rank 1 of a pair: tell rank 0 of this CTA's halves as they land
       int g = 0;
       bool ok = true;
-      while (ok && next_piece(sm, P, w, w1, p)) {
+      while (ok && next_piece<KT>(sm, P, w, w1, p)) {
         const int T = p.t1 - p.t0;
         for (int gt = g; ok && gt < g + T; ++gt) {
           const int st = gt % kStages;
           ok = wait(sm.k_full[st], (gt / kStages) & 1, abort_flag);
           if (!ok) break;
           if (sm.k_mixed[st]) fence_async_smem();
-          mbar_arrive_cluster(map_rank(smem_u32(&sm.k_peer[st & 1]), 0));
+          mbar_arrive_cluster(map_rank(smem_u32(&sm.k_peer[st]), 0));
           ok = wait(sm.v_full[st], (gt / kStages) & 1, abort_flag);
           if (!ok) break;
           if (sm.v_mixed[st]) fence_async_smem();
-          mbar_arrive_cluster(map_rank(smem_u32(&sm.v_peer[st & 1]), 0));
+          mbar_arrive_cluster(map_rank(smem_u32(&sm.v_peer[st]), 0));
         }
         g += T;
       }
@@ -447,18 +447,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Code is kept short (loops rolled, K and V through one body): unrolled, the
     // roles' instructions together starved the warps of each other's.
     constexpr int kPer = KT / 32;
-    const int pt = tid - kProdWarp0 * 32, pw = warp - kProdWarp0;
+    // Warp 0 sends K's boxes, warp 1 V's; of rows copied by cp.async each does two
+    // turns of three and warp 2 the third, for both.
+    const int pw = warp - kProdWarp0;
     const uint64_t pol_first = l2_evict_first(), pol_keep = l2_evict_normal();
     const uint32_t lead = elect_lane();
     int* slots = sm.slots[pw];  // the tile's slots, this warp's copy
     int g = 0;
     bool ok = true;
-    while (ok && next_piece(sm, P, w, w1, p)) {
+    while (ok && next_piece<KT>(sm, P, w, w1, p)) {
       const int T = p.t1 - p.t0;
       if (T == 0) continue;
       const int32_t* idx = a.kv_indices + sm.kv[p.b];
       const uint64_t pol = p.once ? pol_first : pol_keep;
-      const int x0 = p.h * P.x_head, row0 = p.h * P.row_head;
       int s[kPer];  // slots of keys lane + 32 q of a tile; -1 past the request's end
       auto fetch = [&](int tile) {
 #pragma unroll
@@ -495,8 +496,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (t + 1 < T) fetch(p.t0 + t + 1);
         const int live = min(KT / 16, (p.L - j0 + 15) / 16);  // groups with a key; the rest stay as they are
 #pragma unroll 1
-        for (int v = 0; v < 2; ++v) {
-          // K: this CTA's rows, all chunks; V: all rows, this CTA's chunks; chunks ng * 16 rows apart
+        for (int v = pw & 1; v < (pw == 0 ? 1 : 2); ++v) {
+          // K: this CTA's rows, all chunks; V: all rows, this CTA's chunks
           const int ng = v ? KT / 16 : F::KR / 16, nc = v ? F::VC : F::KC;
           const int g0 = v ? 0 : rank * (F::KR / 16), c0 = v ? rank * F::VC : 0;
           uint64_t& full = v ? sm.v_full[st] : sm.k_full[st];
@@ -507,33 +508,43 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t bar = smem_u32(&full);
           const uint32_t dst = v ? v_base + st * F::kVBytes : k_base + st * F::kKBytes;
           const uint32_t mine = boxes >> g0 & ((1u << ng) - 1);
-          if (pt == 0) {
+          if (pw < 2 && lane == 0) {
             // groups with a key that go by cp.async: their readers need a proxy fence
             (v ? sm.v_mixed : sm.k_mixed)[st] = __popc(mine) < max(0, min(ng, live - g0));
             mbar_expect_tx(bar, __popc(mine) * 16 * nc * 128);
           }
-          const CUtensorMap* map = v ? &v_map : &k_map;
           const unsigned char* base =
               static_cast<const unsigned char*>(v ? a.v_cache : a.k_cache) + ((int64_t)p.h * a.kv_sh + 64 * c0) * 2;
-#pragma unroll 1
-          for (int i = 0; i < min(ng, live - g0); ++i) {
-            if (mine >> i & 1) {
-              if (i % kProdWarps == pw) {
-                const int row = slots[16 * (g0 + i)] + row0;
-#pragma unroll 1
-                for (int c = 0; c < nc; ++c)
-                  tma_load_2d(lead, dst + c * (ng * 2048) + i * 2048, map, x0 + 64 * (c0 + c), row, bar, pol);
-              }
-              continue;
-            }
-            // 16 rows of 8 nc pieces of 16 bytes, 32 pieces a turn
-            const int shift = nc == 4 ? 5 : nc == 2 ? 4 : 3;
+          const int n_groups = min(ng, live - g0);
+          if (pw < 2) {
 #pragma unroll 2
-            for (int turn = pw; turn < nc * 4; turn += kProdWarps) {
-              const int u = turn * 32 + lane, row = u >> shift, col = u & ((1 << shift) - 1), r = 16 * i + row;
+            for (int i = 0; i < n_groups; ++i) {
+              if (!(mine >> i & 1)) continue;
+              const int row = slots[16 * (g0 + i)];
+              const uint32_t at = dst + i * nc * 2048;
+              if (v) {
+                tma_load_4d(lead, at, &v_map, 0, row, c0, p.h, bar, pol);
+              } else {
+                tma_load_4d(lead, at, &k_map, 0, row, 0, p.h, bar, pol);
+                tma_load_4d(lead, at + F::KC * 1024, &k_map, 0, row + 8, 0, p.h, bar, pol);
+              }
+            }
+          }
+          if (__popc(mine) < n_groups) {
+            // rows of 8 nc pieces of 16 bytes, 32 pieces a turn
+            const int shift = nc == 4 ? 5 : nc == 2 ? 4 : 3, turns = n_groups * nc * 4;
+            // turns 3 q + {0, 1} are warp 0's or 1's, 3 q + 2 warp 2's
+#pragma unroll 4
+            for (int x = 0; x < turns; ++x) {
+              const int turn = pw == 2 ? 3 * x + 2 : x + (x >> 1);
+              if (turn >= turns) break;
+              const int u = turn * 32 + lane, r = u >> shift, col = u & ((1 << shift) - 1);
               const int slot = slots[16 * g0 + r];
-              cp_async16(dst + (col >> 3) * (ng * 2048) + r * 128 + (((uint32_t)(col ^ r) & 7) << 4),
-                         base + (slot < 0 ? 0 : (int64_t)slot * a.kv_st * 2 + col * 16), slot < 0 ? 0u : 16u, pol);
+              const uint32_t at = v ? (r >> 4) * (nc * 2048) + (col >> 3) * 2048 + (r & 15) * 128
+                                    : (r >> 3) * (nc * 1024) + (col >> 3) * 1024 + (r & 7) * 128;
+              if (!(mine >> (r >> 4) & 1))
+                cp_async16(dst + at + (((uint32_t)(col ^ r) & 7) << 4),
+                           base + (slot < 0 ? 0 : (int64_t)slot * a.kv_st * 2 + col * 16), slot < 0 ? 0u : 16u, pol);
             }
           }
           cp_async_arrive_noinc(bar);
@@ -603,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     // pieces without keys give zero rows; true when u then holds a piece with some
     auto next_live = [&](Piece& u) {
-      while (next_piece(sm, P, w, w1, u)) {
+      while (next_piece<KT>(sm, P, w, w1, u)) {
         if (u.t1 > u.t0) return true;
         if (tok < u.ntok) {
           uint4* orow = reinterpret_cast<uint4*>(static_cast<unsigned char*>(a.o) +
@@ -629,8 +640,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c = 0; c < F::VC; ++c) {
 #pragma unroll
         for (int i = 0; i < KT * 8; i += kSoftmax / 2) {
-          const int at = i + (tid & 127);
-          uint4* q = reinterpret_cast<uint4*>(vb + c * (KT * 128)) + at;
+          const int at = i + (tid & 127);  // row at >> 3
+          uint4* q = reinterpret_cast<uint4*>(vb + (at >> 7) * (F::VC * 2048) + c * 2048) + (at & 127);
           if (at >= live * 8) {
             *q = make_uint4(0u, 0u, 0u, 0u);
           } else if (scan) {
@@ -668,8 +679,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool busy = rank * kRows + wq * 32 < u.ntok * P.G;        // the warp holds rows
       float m_used = -INFINITY, l = 0.f;  // this warpgroup's reference and part of the sum
       for (int t = (g ^ wg) & 1; ok && t < T; t += 2) {
-        const int gt = g + t, sb = gt & 1;
-        ok = __all_sync(0xffffffffu, wait(sm.s_full[sb], (gt >> 1) & 1, abort_flag));
+        const int gt = g + t, sb = gt % NB;
+        ok = __all_sync(0xffffffffu, wait(sm.s_full[sb], (gt / NB) & 1, abort_flag));
         if (!ok) break;
         // keys that every token of the tile sees need no mask (uniform)
         const int j0 = (u.t0 + t) * KT;
@@ -685,10 +696,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         if (busy) {
           tc_fence_after();
+          tmem_ld32_async(ts, &x[0]);
+          tmem_ld32_async(ts + 32, &x[32]);
+        }
+        // the reference after tile gt - 1 (of a unit's first tile only the order counts)
+        if (gt > 0) ok = __all_sync(0xffffffffu, wait(sm.m_ready[(gt - 1) & 1][wq], ((gt - 1) >> 1) & 1, abort_flag));
+        const float m_old = t > 0 ? sm.m[r] : -INFINITY;
+        if (busy) {
           float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll 1
+#pragma unroll
           for (int c = 0; c < KT; c += 64) {
-            tmem_ld64(ts + c, x);
+            if (c) {
+              tmem_ld32_async(ts + c, &x[0]);
+              tmem_ld32_async(ts + c + 32, &x[32]);
+            }
+            tmem_ld_wait(x);
             mask(x, j0 + c, 64);
 #pragma unroll
             for (int i = 0; i < 64; i += 4) {
@@ -699,21 +721,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           // x stays raw: P = 2^(x sc - m)
           tmax = fmaxf(mx[0], mx[1]) * sc;
         }
-        // the reference after tile gt - 1 (of a unit's first tile only the order counts)
-        if (gt > 0) ok = __all_sync(0xffffffffu, wait(sm.m_ready[(gt - 1) & 1][wq], ((gt - 1) >> 1) & 1, abort_flag));
         if (!ok) break;
-        const float m_old = t > 0 ? sm.m[r] : -INFINITY;
         // a row moves it only when the tile's maximum exceeds it by more than 8
         // (P <= 2^8 otherwise); O then scales by 2^(old - new)
         const bool grow = tmax > m_old + 8.f;
         const float m_new = grow ? tmax : m_old;
-        sm.m[r] = m_new;
-        __syncwarp();
+        const bool moves = __any_sync(0xffffffffu, grow);
+        if (moves || t == 0) {
+          sm.m[r] = m_new;
+          __syncwarp();
+        }
         if (lane == 0) mbar_arrive(smem_u32(&sm.m_ready[gt & 1][wq]));
         if (busy) {
-          if (t > 0 && __any_sync(0xffffffffu, grow)) {
+          if (t > 0 && moves) {
             // O holds P V of this unit's earlier tiles: wait for the last, then rescale the row
-            ok = __all_sync(0xffffffffu, wait(sm.pv_done[(gt - 1) & 1], ((gt - 1) >> 1) & 1, abort_flag));
+            ok = __all_sync(0xffffffffu, wait(sm.pv_done[(gt - 1) % NB], ((gt - 1) / NB) & 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
             const float alpha = grow ? ex2(m_old - m_new) : 1.f;
@@ -726,8 +748,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               tmem_st32(tmem + lane_base + F::COL_O + 32 * c, v);
             }
           }
-          if (m_new != m_used) {
-            l *= m_used == -INFINITY ? 1.f : ex2(m_used - m_new);  // without a reference l is 0 or NaN
+          if (__any_sync(0xffffffffu, m_new != m_used)) {
+            if (m_new != m_used) l *= m_used == -INFINITY ? 1.f : ex2(m_used - m_new);  // without a reference l is 0 or NaN
             m_used = m_new;
           }
           // a row whose scores so far are all -inf has no reference yet: its P is 0
@@ -738,7 +760,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           float(&xb)[32] = *reinterpret_cast<float(*)[32]>(&x[32]);
           // 32 columns of S to 16 of P, over columns that have been read
           auto weigh = [&](float(&xs)[32], int c) {
-            mask(xs, j0 + c, 32);
             uint32_t pk[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -750,16 +771,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tmem_st16_async(ts + c / 2, pk);
           };
-          tmem_ld32_async(ts, xa);
-          tmem_ld_wait(xa);
-#pragma unroll 1
-          for (int c = 0; c < KT; c += 64) {
-            tmem_ld32_async(ts + c + 32, xb);
-            weigh(xa, c);
-            tmem_ld_wait(xb);
-            if (c + 64 < KT) tmem_ld32_async(ts + c + 64, xa);
-            weigh(xb, c + 32);
+          if (KT == 64) {  // the tile's scores are still in x, masked
+            weigh(xa, 0);
+            weigh(xb, 32);
+          } else {
+            tmem_ld32_async(ts, xa);
             tmem_ld_wait(xa);
+#pragma unroll 1
+            for (int c = 0; c < KT; c += 64) {
+              tmem_ld32_async(ts + c + 32, xb);
+              mask(xa, j0 + c, 32);
+              weigh(xa, c);
+              tmem_ld_wait(xb);
+              if (c + 64 < KT) tmem_ld32_async(ts + c + 64, xa);
+              mask(xb, j0 + c + 32, 32);
+              weigh(xb, c + 32);
+              tmem_ld_wait(xa);
+            }
           }
           tmem_st_wait();
           float s0, s1;
@@ -777,7 +805,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(smem_u32(&sm.l_ready));
       g += T;
       // once every S MMA of this unit has retired the next unit's Q may go in
-      ok = __all_sync(0xffffffffu, wait(sm.s_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag));
+      ok = __all_sync(0xffffffffu, wait(sm.s_full[(g - 1) % NB], ((g - 1) / NB) & 1, abort_flag));
       if (!ok) break;
       tc_fence_after();
       more = next_live(p);
@@ -940,12 +968,8 @@ int check_args(const dft_chunk_attn_args* a) {
   if (a->q_st < 0 || a->q_sh < 0 || (a->T > 1 && a->o_st < a->D) || (a->Hq > 1 && a->o_sh < a->D) ||
       a->kv_st < a->D || (a->Hkv > 1 && a->kv_sh < a->D))
     return DFT_ERR_INVALID;
-  // the cache as rows of one 2-D tensor map: a head is a column offset where a
-  // slot's heads lie inside its stride, a row offset where heads are outermost
-  const int64_t span = (a->Hkv - 1) * a->kv_sh + a->D;
-  if (span > a->kv_st && a->kv_sh % a->kv_st) return DFT_ERR_UNSUPPORTED;
-  const int64_t rows = span <= a->kv_st ? a->n_slots : a->n_slots + (a->Hkv - 1) * (a->kv_sh / a->kv_st);
-  if (rows > 0x7FFFFFFF || span > 0x7FFFFFFF || a->kv_st >= ((int64_t)1 << 38)) return DFT_ERR_UNSUPPORTED;
+  if (a->kv_st >= ((int64_t)1 << 38) || a->kv_sh >= ((int64_t)1 << 38) || a->n_slots > 0x7FFFFFFF)
+    return DFT_ERR_UNSUPPORTED;
   return DFT_OK;
 }
 
@@ -968,14 +992,14 @@ Workspace workspace(const dft_chunk_attn_args* a, int workers) {
   return w;
 }
 
-bool encode(CUtensorMap* m, const dft_chunk_attn_args* a, const void* base, bool inner) {
-  const cuuint64_t dims[2] = {(cuuint64_t)(inner ? (a->Hkv - 1) * a->kv_sh + a->D : a->D),
-                              (cuuint64_t)(inner ? a->n_slots : a->n_slots + (a->Hkv - 1) * (a->kv_sh / a->kv_st))};
-  const cuuint64_t strides[1] = {(cuuint64_t)a->kv_st * 2};
-  const cuuint32_t box[2] = {64, 16}, estr[2] = {1, 1};
+// the cache as (64 dims, slots, 64-dim chunks, heads): any slot and head stride
+bool encode(CUtensorMap* m, const dft_chunk_attn_args* a, const void* base, int rows, int chunks) {
+  const cuuint64_t dims[4] = {64, (cuuint64_t)a->n_slots, (cuuint64_t)a->D / 64, (cuuint64_t)a->Hkv};
+  const cuuint64_t strides[3] = {(cuuint64_t)a->kv_st * 2, 128, (cuuint64_t)a->kv_sh * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)rows, (cuuint32_t)chunks, 1}, estr[4] = {1, 1, 1, 1};
   return gtile::encode_fn() &&
          gtile::encode_fn()(m, a->dtype == DFT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                            2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -1032,14 +1056,13 @@ extern "C" int dft_chunk_attn(const dft_chunk_attn_args* a, void* ws, int32_t* d
   P.a = *a;
   P.G = a->Hq / a->Hkv;
   P.TQ = kRows * (a->D == 256 ? Cfg<256>::CG : 1) / P.G;
-  const bool inner = (a->Hkv - 1) * a->kv_sh + a->D <= a->kv_st;
-  P.x_head = inner ? (int)a->kv_sh : 0;
-  P.row_head = inner ? 0 : (int)(a->kv_sh / a->kv_st);
   P.ws_meta = reinterpret_cast<int4*>(static_cast<char*>(ws) + w.meta);
   P.ws_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + w.ml);
   P.ws_o = reinterpret_cast<float*>(static_cast<char*>(ws) + w.o);
   CUtensorMap k_map, v_map;
-  if (!encode(&k_map, a, a->k_cache, inner) || !encode(&v_map, a, a->v_cache, inner)) return DFT_ERR_UNSUPPORTED;
+  if (!encode(&k_map, a, a->k_cache, 8, a->D / 64) ||
+      !encode(&v_map, a, a->v_cache, 16, a->D == 256 ? Cfg<256>::VC : a->D / 64))
+    return DFT_ERR_UNSUPPORTED;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool bf = a->dtype == DFT_BF16;
 #define DFT_GO(D_) \

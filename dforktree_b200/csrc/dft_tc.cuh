@@ -92,22 +92,13 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, int c
 
 // issued by the lane with `lead` set, in code that the whole warp runs (several
 // lanes issuing, or one under a branch, took about 200 cycles a copy)
-__device__ __forceinline__ void tma_load_2d(uint32_t lead, uint32_t dst, const void* map, int c0, int c1, uint32_t bar,
-                                            uint64_t policy) {
+__device__ __forceinline__ void tma_load_4d(uint32_t lead, uint32_t dst, const void* map, int c0, int c1, int c2,
+                                            int c3, uint32_t bar, uint64_t policy) {
   asm volatile(
-      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
-      "@q cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
-      "[%0], [%1, {%2, %3}], [%4], %5;\n\t}\n" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar), "l"(policy), "r"(lead)
-      : "memory");
-}
-__device__ __forceinline__ void tma_load_3d(uint32_t lead, uint32_t dst, const void* map, int c0, int c1, int c2,
-                                            uint32_t bar, uint64_t policy) {
-  asm volatile(
-      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %7, 0;\n\t"
-      "@q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
-      "[%0], [%1, {%2, %3, %4}], [%5], %6;\n\t}\n" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar), "l"(policy), "r"(lead)
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %8, 0;\n\t"
+      "@q cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
+      "[%0], [%1, {%2, %3, %4, %5}], [%6], %7;\n\t}\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar), "l"(policy), "r"(lead)
       : "memory");
 }
 __device__ __forceinline__ uint64_t l2_evict_normal() {
