@@ -452,6 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int pw = warp - kProdWarp0;
     const uint64_t pol_first = l2_evict_first(), pol_keep = l2_evict_normal();
     const uint32_t lead = elect_lane();
+    const uint64_t pitch = (uint32_t)a.kv_st * 2u;  // bytes, below 2^32
     int* slots = sm.slots[pw];  // the tile's slots, this warp's copy
     int g = 0;
     bool ok = true;
@@ -460,12 +461,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (T == 0) continue;
       const int32_t* idx = a.kv_indices + sm.kv[p.b];
       const uint64_t pol = p.once ? pol_first : pol_keep;
-      int s[kPer];  // slots of keys lane + 32 q of a tile; -1 past the request's end
+      int s[kPer];  // slots of keys lane + 32 q of a tile; past the request's end, of its last
       auto fetch = [&](int tile) {
 #pragma unroll
         for (int q = 0; q < kPer; ++q) {
           const int j = tile * KT + 32 * q + lane;
-          s[q] = j < p.L ? __ldg(idx + j) : -1;
+          s[q] = __ldg(idx + min(j, p.L - 1));
         }
       };
       fetch(p.t0);
@@ -479,15 +480,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int q = 0; q < kPer; ++q) {
           const int j = j0 + 32 * q + lane;
           int cur = s[q];
-          if (j < p.L && (cur < 0 || (int64_t)cur >= a.n_slots)) {
+          if (cur < 0 || (int64_t)cur >= a.n_slots) {
             bad = true;
             cur = 0;
           }
           slots[32 * q + lane] = cur;
-          // keys past the end go along with their group's box; a group without a key has none
+          // keys past the end go along with their group's box
           const int first = __shfl_sync(0xffffffffu, cur, lane & 16);
           const uint32_t with = __ballot_sync(
-              0xffffffffu, first >= 0 && (int64_t)first + 16 <= a.n_slots && (j >= p.L || cur == first + (lane & 15)));
+              0xffffffffu, (int64_t)first + 16 <= a.n_slots && (j >= p.L || cur == first + (lane & 15)));
           boxes |= (with & 0xFFFFu) == 0xFFFFu ? 1u << (2 * q) : 0u;
           boxes |= (with >> 16) == 0xFFFFu ? 2u << (2 * q) : 0u;
         }
@@ -507,15 +508,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           const uint32_t bar = smem_u32(&full);
           const uint32_t dst = v ? v_base + st * F::kVBytes : k_base + st * F::kKBytes;
-          const uint32_t mine = boxes >> g0 & ((1u << ng) - 1);
+          const int n_groups = min(ng, live - g0);  // may be negative
+          const uint32_t mine = n_groups > 0 ? boxes >> g0 & ((1u << n_groups) - 1) : 0u;
           if (pw < 2 && lane == 0) {
             // groups with a key that go by cp.async: their readers need a proxy fence
-            (v ? sm.v_mixed : sm.k_mixed)[st] = __popc(mine) < max(0, min(ng, live - g0));
+            (v ? sm.v_mixed : sm.k_mixed)[st] = __popc(mine) < n_groups;
             mbar_expect_tx(bar, __popc(mine) * 16 * nc * 128);
           }
           const unsigned char* base =
               static_cast<const unsigned char*>(v ? a.v_cache : a.k_cache) + ((int64_t)p.h * a.kv_sh + 64 * c0) * 2;
-          const int n_groups = min(ng, live - g0);
           if (pw < 2) {
 #pragma unroll 2
             for (int i = 0; i < n_groups; ++i) {
@@ -531,21 +532,34 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           if (__popc(mine) < n_groups) {
-            // rows of 8 nc pieces of 16 bytes, 32 pieces a turn
-            const int shift = nc == 4 ? 5 : nc == 2 ? 4 : 3, turns = n_groups * nc * 4;
-            // turns 3 q + {0, 1} are warp 0's or 1's, 3 q + 2 warp 2's
-#pragma unroll 4
-            for (int x = 0; x < turns; ++x) {
-              const int turn = pw == 2 ? 3 * x + 2 : x + (x >> 1);
-              if (turn >= turns) break;
-              const int u = turn * 32 + lane, r = u >> shift, col = u & ((1 << shift) - 1);
-              const int slot = slots[16 * g0 + r];
-              const uint32_t at = v ? (r >> 4) * (nc * 2048) + (col >> 3) * 2048 + (r & 15) * 128
-                                    : (r >> 3) * (nc * 1024) + (col >> 3) * 1024 + (r & 7) * 128;
-              if (!(mine >> (r >> 4) & 1))
-                cp_async16(dst + at + (((uint32_t)(col ^ r) & 7) << 4),
-                           base + (slot < 0 ? 0 : (int64_t)slot * a.kv_st * 2 + col * 16), slot < 0 ? 0u : 16u, pol);
-            }
+            // a group's 16 rows of 8 NC pieces of 16 bytes, 32 pieces a turn
+            auto copy = [&](auto nc_, auto v_) {
+              constexpr int NC = decltype(nc_)::value, kRow = 32 / (8 * NC);  // rows a turn
+              constexpr bool V = decltype(v_)::value;
+              const int lr = lane / (8 * NC), col = lane % (8 * NC);
+              const unsigned char* src = base + col * 16;
+              const uint32_t to = dst + (col >> 3) * (V ? 2048 : 1024) + lr * 128, swz = ((col ^ lr) & 7) << 4;
+              auto turn = [&](int i, int q) {
+                const int row = q * kRow;  // and lr
+                cp_async16(to + i * (NC * 2048) + (V ? row * 128 : (row >> 3) * (NC * 1024) + (row & 7) * 128) +
+                               (swz ^ ((row & 7) << 4)),
+                           src + (uint64_t)(uint32_t)slots[16 * (g0 + i) + row + lr] * pitch, 16u, pol);
+              };
+#pragma unroll 1
+              for (int i = 0; i < n_groups; ++i) {
+                if (mine >> i & 1) continue;
+                if (pw == 2) {
+#pragma unroll
+                  for (int q = 2; q < 4 * NC; q += 3) turn(i, q);
+                } else {
+#pragma unroll
+                  for (int q = 0; q < 4 * NC; ++q)
+                    if (q % 3 != 2) turn(i, q);
+                }
+              }
+            };
+            if (v) copy(Int<F::VC>(), Int<1>());
+            else copy(Int<F::KC>(), Int<0>());
           }
           cp_async_arrive_noinc(bar);
         }
@@ -968,7 +982,7 @@ int check_args(const dft_chunk_attn_args* a) {
   if (a->q_st < 0 || a->q_sh < 0 || (a->T > 1 && a->o_st < a->D) || (a->Hq > 1 && a->o_sh < a->D) ||
       a->kv_st < a->D || (a->Hkv > 1 && a->kv_sh < a->D))
     return DFT_ERR_INVALID;
-  if (a->kv_st >= ((int64_t)1 << 38) || a->kv_sh >= ((int64_t)1 << 38) || a->n_slots > 0x7FFFFFFF)
+  if (a->kv_st >= ((int64_t)1 << 31) || a->kv_sh >= ((int64_t)1 << 38) || a->n_slots > 0x7FFFFFFF)
     return DFT_ERR_UNSUPPORTED;
   return DFT_OK;
 }
