@@ -20,15 +20,14 @@
 //         copy, 5 us per 64 KB)
 //   S     = Q K^T    kind::f16, fp32 in TMEM; Q from TMEM, or from shared memory
 //         for a pair
-//   P     = 2^(S sm_scale log2e - m), a thread per row; the reference m moves
+//   P     = 2^(S sm_scale log2e - m), two threads per row; the reference m moves
 //         (and O is rescaled in TMEM) only when the maximum grows by more than
 //         8, so P <= 2^8; rounded to the 16-bit type over its own S (the second
 //         product's operand has V's type), summed unrounded
 //   O    += P V      P from TMEM, V as an MN-major operand
-// Two softmax warpgroups take the tiles in turn, each with twice a tile's MMA
-// time to hide its latencies in; m goes from one to the other through shared
-// memory as soon as a tile's maximum is known.  S / P are double-buffered and
-// the S MMA runs a tile ahead of the P V MMA.
+// S / P are double-buffered and the S MMA runs a tile ahead of the P V MMA.  S of
+// tile t+2 waits for P V of tile t, so a tile's softmax latency counts twice: a
+// warpgroup per tile, in turn, took 3000 cycles a tile, both on one tile 1600.
 //
 // Work is split by keys, not by unit: unit costs (keys + a fixed part) are laid
 // out on one line, and worker c (a CTA, a pair) takes the c-th share of it,
@@ -59,7 +58,7 @@ namespace {
 
 constexpr int kMaxB = 1024;
 constexpr int kRows = 128;        // query rows of a CTA
-constexpr int kSoftmax = 256;     // two warpgroups, a thread per query row in each
+constexpr int kSoftmax = 256;     // two threads per query row, in warps w and w + 4
 constexpr int kCtlWarp = 8, kProdWarp0 = 9, kProdWarps = 3;
 constexpr int kThreads = 384;     // twelve warps leave 168 registers a thread
 constexpr uint32_t kTmemCols = 512;
@@ -95,19 +94,22 @@ struct Cfg {
 struct Small {
   uint64_t q_ready;
   uint64_t k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages];
-  uint64_t k_peer[kMaxStages], v_peer[kMaxStages];  // the other CTA's part of the stage (rank 0 of a pair)
+  uint64_t k_copied[kMaxStages], v_copied[kMaxStages];  // rank 1 of a pair: its cp.async rows of the stage
   uint64_t s_full[4], p_full[4], pv_done[4];
-  uint64_t m_ready[2][4];   // [tile & 1][row warp]: the tile's reference is in m
-  uint64_t l_ready, o_full, o_free, mma_done;
+  uint64_t v_here[4];       // rank 1 of a pair: [S buffer] the tile's V is in (its boxes complete on rank 0)
+  uint64_t o_full, o_free, mma_done;
   uint32_t tmem_base;
   int abort;
   int odd[8];               // [piece & 7] = piece + 1 when one of its masked tiles held a non-finite value
-  float m[kRows];           // the reference after the last tile whose maximum is known
-  float2 ml[2][2][kRows];   // [piece & 1][warpgroup] its reference and its part of the row sum
+  float xmax[2][2][kRows];  // [tile parity][half][row] tile max exchange between a row's two threads
+  float lsum[2][kRows];     // [half][row] final row sums
+  int okx[2][2][4];         // [tile parity][half][row warp] wait outcomes, shared by a row's two warps
+  int okr[2][2][4];         // the same for the rescale's wait
+  int oke[2][4];            // [half][row warp] the epilogue's wait
   int64_t warp_sum[kThreads / 32];
   int64_t pre[kMaxB + 1];   // cost of the requests before b
   int qo[kMaxB + 1], kv[kMaxB + 1];
-  int slots[kProdWarps][128];
+  int4 slots[kProdWarps][32];
   int k_mixed[kMaxStages], v_mixed[kMaxStages];  // [stage]: the CTA's part holds rows copied by cp.async
 };
 
@@ -268,21 +270,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       mbar_init(smem_u32(&sm.q_ready), kSoftmax / 32 * CG);
       for (int i = 0; i < kStages; ++i) {
-        mbar_init(smem_u32(&sm.k_peer[i]), 1);
-        mbar_init(smem_u32(&sm.v_peer[i]), 1);
-        mbar_init(smem_u32(&sm.k_full[i]), 64 + 1);
+        // 64 producers' cp.async and an expect_tx; from rank 1 an expect_tx and, once its cp.async are in, an arrival
+        mbar_init(smem_u32(&sm.k_copied[i]), 64);
+        mbar_init(smem_u32(&sm.v_copied[i]), 64);
+        mbar_init(smem_u32(&sm.k_full[i]), 64 + 1 + 2 * (CG - 1));
         mbar_init(smem_u32(&sm.k_empty[i]), 1);
-        mbar_init(smem_u32(&sm.v_full[i]), 64 + 1);
+        mbar_init(smem_u32(&sm.v_full[i]), 64 + 1 + 2 * (CG - 1));
         mbar_init(smem_u32(&sm.v_empty[i]), 1);
       }
       for (int i = 0; i < 4; ++i) {
         mbar_init(smem_u32(&sm.s_full[i]), 1);
-        mbar_init(smem_u32(&sm.p_full[i]), kSoftmax / 64 * CG);
+        mbar_init(smem_u32(&sm.p_full[i]), kSoftmax / 32 * CG);
         mbar_init(smem_u32(&sm.pv_done[i]), 1);
-        mbar_init(smem_u32(&sm.m_ready[0][i]), 1);
-        mbar_init(smem_u32(&sm.m_ready[1][i]), 1);
+        mbar_init(smem_u32(&sm.v_here[i]), 1);
       }
-      mbar_init(smem_u32(&sm.l_ready), kSoftmax / 32);
       mbar_init(smem_u32(&sm.o_full), 1);
       mbar_init(smem_u32(&sm.o_free), kSoftmax / 32 * CG);
       mbar_init(smem_u32(&sm.mma_done), 1);
@@ -369,7 +370,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (t < T) {
             const int gt = g + t, st = gt % kStages, sb = gt % NB;
             bool got = wait(sm.k_full[st], (gt / kStages) & 1, abort_flag);
-            if (PAIR) got = got && wait(sm.k_peer[st], (gt / kStages) & 1, abort_flag);
             if (got && gt >= NB) got = wait(sm.pv_done[sb], (gt / NB - 1) & 1, abort_flag);  // P of tile gt - NB is read
             ok = all(got);
             if (!ok) break;
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (t >= kAhead) {
             const int gu = g + t - kAhead, st = gu % kStages, pb = gu % NB;
             bool got = wait(sm.v_full[st], (gu / kStages) & 1, abort_flag);
-            if (PAIR) got = got && wait(sm.v_peer[st], (gu / kStages) & 1, abort_flag);
+            if (PAIR && got && lead) mbar_arrive_cluster(map_rank(smem_u32(&sm.v_here[pb]), 1));
             // the first P V of a unit overwrites O: the previous unit's epilogue has read it
             if (got && t == kAhead && ui > 0) got = wait(sm.o_free, (ui - 1) & 1, abort_flag);
             ok = all(got && wait(sm.p_full[pb], (gu / NB) & 1, abort_flag));
@@ -420,21 +420,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       // every MMA issued above has retired before TMEM is freed
       commit(sm.mma_done);
     } else if (lane == 0) {
-      // rank 1 of a pair: tell rank 0 of this CTA's halves as they land
+      // rank 1 of a pair: its boxes complete on rank 0's barriers by themselves;
+      // tell rank 0 of the stages that hold cp.async rows as those land
       int g = 0;
       bool ok = true;
       while (ok && next_piece<KT>(sm, P, w, w1, p)) {
         const int T = p.t1 - p.t0;
         for (int gt = g; ok && gt < g + T; ++gt) {
           const int st = gt % kStages;
-          ok = wait(sm.k_full[st], (gt / kStages) & 1, abort_flag);
+          ok = wait(sm.k_copied[st], (gt / kStages) & 1, abort_flag);
           if (!ok) break;
-          if (sm.k_mixed[st]) fence_async_smem();
-          mbar_arrive_cluster(map_rank(smem_u32(&sm.k_peer[st]), 0));
-          ok = wait(sm.v_full[st], (gt / kStages) & 1, abort_flag);
+          if (sm.k_mixed[st]) {
+            fence_async_smem();
+            mbar_arrive_cluster(map_rank(smem_u32(&sm.k_full[st]), 0));
+          }
+          ok = wait(sm.v_copied[st], (gt / kStages) & 1, abort_flag);
           if (!ok) break;
-          if (sm.v_mixed[st]) fence_async_smem();
-          mbar_arrive_cluster(map_rank(smem_u32(&sm.v_peer[st]), 0));
+          if (sm.v_mixed[st]) {
+            fence_async_smem();
+            mbar_arrive_cluster(map_rank(smem_u32(&sm.v_full[st]), 0));
+          }
         }
         g += T;
       }
@@ -446,14 +451,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------- producers: paged K/V tiles
     // Code is kept short (loops rolled, K and V through one body): unrolled, the
     // roles' instructions together starved the warps of each other's.
-    constexpr int kPer = KT / 32;
-    // Warp 0 sends K's boxes, warp 1 V's; of rows copied by cp.async each does two
+    static_assert(KT == 128, "four slots a lane");
+    // Warps 0 and 2 send K's boxes, warp 1 V's; of rows copied by cp.async each does two
     // turns of three and warp 2 the third, for both.
     const int pw = warp - kProdWarp0;
     const uint64_t pol_first = l2_evict_first(), pol_keep = l2_evict_normal();
     const uint32_t lead = elect_lane();
     const uint64_t pitch = (uint32_t)a.kv_st * 2u;  // bytes, below 2^32
-    int* slots = sm.slots[pw];  // the tile's slots, this warp's copy
+    const int* slots = reinterpret_cast<const int*>(sm.slots[pw]);  // the tile's slots, this warp's copy
     int g = 0;
     bool ok = true;
     while (ok && next_piece<KT>(sm, P, w, w1, p)) {
@@ -461,38 +466,34 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (T == 0) continue;
       const int32_t* idx = a.kv_indices + sm.kv[p.b];
       const uint64_t pol = p.once ? pol_first : pol_keep;
-      int s[kPer];  // slots of keys lane + 32 q of a tile; past the request's end, of its last
+      int s[4];  // slots of keys 4 lane + q of a tile; past the request's end, of its last
       auto fetch = [&](int tile) {
 #pragma unroll
-        for (int q = 0; q < kPer; ++q) {
-          const int j = tile * KT + 32 * q + lane;
-          s[q] = __ldg(idx + min(j, p.L - 1));
-        }
+        for (int q = 0; q < 4; ++q) s[q] = __ldg(idx + min(tile * KT + 4 * lane + q, p.L - 1));
       };
       fetch(p.t0);
 #pragma unroll 1
       for (int t = 0; t < T; ++t) {
         const int gt = g + t, st = gt % kStages, j0 = (p.t0 + t) * KT;
-        uint32_t boxes = 0;  // bit i: the 16 slots of group i are consecutive
+        const int j = j0 + 4 * lane;
         bool bad = false;
-        __syncwarp();
 #pragma unroll
-        for (int q = 0; q < kPer; ++q) {
-          const int j = j0 + 32 * q + lane;
-          int cur = s[q];
-          if (cur < 0 || (int64_t)cur >= a.n_slots) {
-            bad = true;
-            cur = 0;
-          }
-          slots[32 * q + lane] = cur;
-          // keys past the end go along with their group's box
-          const int first = __shfl_sync(0xffffffffu, cur, lane & 16);
-          const uint32_t with = __ballot_sync(
-              0xffffffffu, (int64_t)first + 16 <= a.n_slots && (j >= p.L || cur == first + (lane & 15)));
-          boxes |= (with & 0xFFFFu) == 0xFFFFu ? 1u << (2 * q) : 0u;
-          boxes |= (with >> 16) == 0xFFFFu ? 2u << (2 * q) : 0u;
+        for (int q = 0; q < 4; ++q) {
+          const bool out = s[q] < 0 || (int64_t)s[q] >= a.n_slots;
+          if (out) s[q] = 0;
+          bad |= out;
         }
         if (bad) raise_status(status, DFT_DEV_BAD_INDEX);
+        __syncwarp();
+        sm.slots[pw][lane] = make_int4(s[0], s[1], s[2], s[3]);
+        // boxes: bit 4 i set where the 16 slots of group i are consecutive; keys past the end go along
+        const int first = __shfl_sync(0xffffffffu, s[0], lane & 28);
+        bool run = (int64_t)first + 16 <= a.n_slots;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) run &= j + q >= p.L || s[q] == first + 4 * (lane & 3) + q;
+        uint32_t boxes = __ballot_sync(0xffffffffu, run);
+        boxes &= boxes >> 1;
+        boxes = boxes & boxes >> 2 & 0x11111111u;
         __syncwarp();
         if (t + 1 < T) fetch(p.t0 + t + 1);
         const int live = min(KT / 16, (p.L - j0 + 15) / 16);  // groups with a key; the rest stay as they are
@@ -506,28 +507,34 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = __all_sync(0xffffffffu, wait(v ? sm.v_empty[st] : sm.k_empty[st], (gt / kStages - 1) & 1, abort_flag));
             if (!ok) break;
           }
-          const uint32_t bar = smem_u32(&full);
+          // rank 0's barrier takes both CTAs' boxes, a rank 1's own its cp.async
+          const uint32_t bar = PAIR ? map_rank(smem_u32(&full), 0) : smem_u32(&full);
+          const uint32_t copied = rank ? smem_u32(v ? &sm.v_copied[st] : &sm.k_copied[st]) : smem_u32(&full);
           const uint32_t dst = v ? v_base + st * F::kVBytes : k_base + st * F::kKBytes;
           const int n_groups = min(ng, live - g0);  // may be negative
-          const uint32_t mine = n_groups > 0 ? boxes >> g0 & ((1u << n_groups) - 1) : 0u;
+          const uint32_t mine = n_groups > 0 ? boxes >> 4 * g0 & (0xFFFFFFFFu >> (32 - 4 * n_groups)) : 0u;
           if (pw < 2 && lane == 0) {
             // groups with a key that go by cp.async: their readers need a proxy fence
-            (v ? sm.v_mixed : sm.k_mixed)[st] = __popc(mine) < n_groups;
-            mbar_expect_tx(bar, __popc(mine) * 16 * nc * 128);
+            const bool mixed = __popc(mine) < n_groups;
+            (v ? sm.v_mixed : sm.k_mixed)[st] = mixed;
+            mbar_expect_tx_cluster<PAIR>(bar, __popc(mine) * 16 * nc * 128);
+            if (PAIR && rank && !mixed) mbar_arrive_cluster(bar);
           }
+          __syncwarp();
           const unsigned char* base =
               static_cast<const unsigned char*>(v ? a.v_cache : a.k_cache) + ((int64_t)p.h * a.kv_sh + 64 * c0) * 2;
-          if (pw < 2) {
+          // K's boxes by warps 0 and 2 in turn, V's by warp 1
+          if (pw < 2 || !v) {
 #pragma unroll 2
-            for (int i = 0; i < n_groups; ++i) {
-              if (!(mine >> i & 1)) continue;
+            for (int i = pw >> 1; i < n_groups; i += v ? 1 : 2) {
+              if (!(mine >> 4 * i & 1)) continue;
               const int row = slots[16 * (g0 + i)];
               const uint32_t at = dst + i * nc * 2048;
               if (v) {
-                tma_load_4d(lead, at, &v_map, 0, row, c0, p.h, bar, pol);
+                tma_load_4d<CG>(lead, at, &v_map, 0, row, c0, p.h, bar, pol);
               } else {
-                tma_load_4d(lead, at, &k_map, 0, row, 0, p.h, bar, pol);
-                tma_load_4d(lead, at + F::KC * 1024, &k_map, 0, row + 8, 0, p.h, bar, pol);
+                tma_load_4d<CG>(lead, at, &k_map, 0, row, 0, p.h, bar, pol);
+                tma_load_4d<CG>(lead, at + F::KC * 1024, &k_map, 0, row + 8, 0, p.h, bar, pol);
               }
             }
           }
@@ -547,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               };
 #pragma unroll 1
               for (int i = 0; i < n_groups; ++i) {
-                if (mine >> i & 1) continue;
+                if (mine >> 4 * i & 1) continue;
                 if (pw == 2) {
 #pragma unroll
                   for (int q = 2; q < 4 * NC; q += 3) turn(i, q);
@@ -561,7 +568,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (v) copy(Int<F::VC>(), Int<1>());
             else copy(Int<F::KC>(), Int<0>());
           }
-          cp_async_arrive_noinc(bar);
+          cp_async_arrive_noinc(copied);
         }
         if (!ok) {
           g += t;
@@ -574,17 +581,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     // The last copies land before the block's shared memory goes, whatever
     // became of their readers; after an abort tile g may have its K on the way.
     cp_async_wait_all();
-    for (int gt = max(0, g - kStages); gt < g; ++gt) {
-      mbar_wait(smem_u32(&sm.k_full[gt % kStages]), (gt / kStages) & 1);
-      mbar_wait(smem_u32(&sm.v_full[gt % kStages]), (gt / kStages) & 1);
+    if (rank == 0) {
+      for (int gt = max(0, g - kStages); gt < g; ++gt) {
+        mbar_wait(smem_u32(&sm.k_full[gt % kStages]), (gt / kStages) & 1);
+        mbar_wait(smem_u32(&sm.v_full[gt % kStages]), (gt / kStages) & 1);
+      }
+      if (!ok) mbar_wait(smem_u32(&sm.k_full[g % kStages]), (g / kStages) & 1);
     }
-    if (!ok) mbar_wait(smem_u32(&sm.k_full[g % kStages]), (g / kStages) & 1);
   } else {
-    // ------------- softmax, a thread per row; output, by halves of the columns
+    // ------------- softmax and output, two threads per row, one half of the columns each
     constexpr float kBias = BF ? 0.f : 6.f; // float16 P: up to 2^14, so that small weights stay clear of its smallest step
     const int r = (warp & 3) * 32 + lane;   // TMEM lane
     const int R = rank * kRows + r;         // query row of the tile
-    const int wg = warp >> 2;               // this warpgroup's tiles: gt & 1 == wg; its half of O's and Q's columns
+    const int wg = warp >> 2;               // half of S's, O's and Q's columns
+    const int pair_bar = 1 + (warp & 3);    // named barrier of warps w and w + 4 (same rows)
     const int wq = warp & 3;
     const int tok = R / P.G, g_ = R - tok * P.G;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
@@ -645,7 +655,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto clean_v = [&](const Piece& u, int t, int gt) -> bool {
       constexpr uint32_t kExp = BF ? 0x7F807F80u : 0x7C007C00u, kOne = BF ? 0x00800080u : 0x04000400u;
       const int j0 = (u.t0 + t) * KT, st = gt % kStages;
-      if (!__all_sync(0xffffffffu, wait(sm.v_full[st], (gt / kStages) & 1, abort_flag))) return false;
+      if (!__all_sync(0xffffffffu, rank ? wait(sm.v_here[gt % NB], (gt / NB) & 1, abort_flag)
+                                        : wait(sm.v_full[st], (gt / kStages) & 1, abort_flag)))
+        return false;
       const int live = min(KT, u.L - j0);          // rows of real keys
       const bool scan = u.vis0 < j0 + live;        // some token does not see them all
       unsigned char* vb = smem + F::OFF_V + st * F::kVBytes;
@@ -653,8 +665,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
       for (int c = 0; c < F::VC; ++c) {
 #pragma unroll
-        for (int i = 0; i < KT * 8; i += kSoftmax / 2) {
-          const int at = i + (tid & 127);  // row at >> 3
+        for (int i = 0; i < KT * 8; i += kSoftmax) {
+          const int at = i + tid;  // row at >> 3
           uint4* q = reinterpret_cast<uint4*>(vb + (at >> 7) * (F::VC * 2048) + c * 2048) + (at & 127);
           if (at >= live * 8) {
             *q = make_uint4(0u, 0u, 0u, 0u);
@@ -691,146 +703,120 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int T = u.t1 - u.t0;
       const int vis = max(0, min(u.L, u.vis0 + (row_ok ? tok : 0)));  // keys this row sees: j < vis
       const bool busy = rank * kRows + wq * 32 < u.ntok * P.G;        // the warp holds rows
-      float m_used = -INFINITY, l = 0.f;  // this warpgroup's reference and part of the sum
-      for (int t = (g ^ wg) & 1; ok && t < T; t += 2) {
-        const int gt = g + t, sb = gt % NB;
-        ok = __all_sync(0xffffffffu, wait(sm.s_full[sb], (gt / NB) & 1, abort_flag));
-        if (!ok) break;
+      // A row's two warps meet at the same named barriers in the same order;
+      // every early exit is decided from outcomes both have exchanged there.
+      float m_used = -INFINITY, l = 0.f;
+      bool held = true;  // false: the last tile's V never came; told to the other warp at the next barrier
+#pragma unroll 1
+      for (int t = 0; t < T; ++t) {
+        const int gt = g + t, sb = gt % NB, par = gt & 1;
+        const bool got = __all_sync(0xffffffffu, held && wait(sm.s_full[sb], (gt / NB) & 1, abort_flag));
         // keys that every token of the tile sees need no mask (uniform)
         const int j0 = (u.t0 + t) * KT;
         const bool plain = j0 + KT <= u.vis0 && j0 + KT <= u.L;
+        if (!busy) {  // spare rows: whatever P holds stays in them
+          ok = got && (plain || clean_v(u, t, gt));
+          if (!ok) break;
+          warp_arrive<PAIR>(sm.p_full[sb]);
+          continue;
+        }
         const uint32_t ts = tmem + lane_base + F::COL_S + KT * sb;
         float x[64];
-        float tmax = -INFINITY;
-        auto mask = [&](float* xs, int j, int n) {
-          if (plain) return;
+        tc_fence_after();
+        tmem_ld32_async(ts + 64 * wg, &x[0]);
+        tmem_ld32_async(ts + 64 * wg + 32, &x[32]);
+        tmem_ld_wait(x);
+        if (!plain) {
+          const int c0 = vis - j0 - 64 * wg;  // columns of this half that the row sees
 #pragma unroll
           for (int i = 0; i < 64; ++i)
-            if (i < n && j + i >= vis) xs[i] = -INFINITY;
-        };
-        if (busy) {
-          tc_fence_after();
-          tmem_ld32_async(ts, &x[0]);
-          tmem_ld32_async(ts + 32, &x[32]);
+            if (i >= c0) x[i] = -INFINITY;
         }
-        // the reference after tile gt - 1 (of a unit's first tile only the order counts)
-        if (gt > 0) ok = __all_sync(0xffffffffu, wait(sm.m_ready[(gt - 1) & 1][wq], ((gt - 1) >> 1) & 1, abort_flag));
-        const float m_old = t > 0 ? sm.m[r] : -INFINITY;
-        if (busy) {
-          float mx[2] = {-INFINITY, -INFINITY};
+        float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < KT; c += 64) {
-            if (c) {
-              tmem_ld32_async(ts + c, &x[0]);
-              tmem_ld32_async(ts + c + 32, &x[32]);
-            }
-            tmem_ld_wait(x);
-            mask(x, j0 + c, 64);
-#pragma unroll
-            for (int i = 0; i < 64; i += 4) {
-              mx[0] = fmaxf(fmaxf(mx[0], x[i]), x[i + 1]);
-              mx[1] = fmaxf(fmaxf(mx[1], x[i + 2]), x[i + 3]);
-            }
-          }
-          // x stays raw: P = 2^(x sc - m)
-          tmax = fmaxf(mx[0], mx[1]) * sc;
+        for (int i = 0; i < 64; i += 4) {
+          mx[0] = fmaxf(fmaxf(mx[0], x[i]), x[i + 1]);
+          mx[1] = fmaxf(fmaxf(mx[1], x[i + 2]), x[i + 3]);
         }
+        // x stays raw: P = 2^(x sc - m)
+        float tmax = fmaxf(mx[0], mx[1]) * sc;
+        sm.xmax[par][wg][r] = tmax;
+        if (lane == 0) sm.okx[par][wg][wq] = got;
+        // the barrier also orders this half's S reads before the other half's P
+        // stores (half 1 writes P over S columns that half 0 reads)
+        tc_fence_before();
+        named_bar(pair_bar, 64);
+        tc_fence_after();
+        tmax = fmaxf(tmax, sm.xmax[par][wg ^ 1][r]);
+        ok = got && sm.okx[par][wg ^ 1][wq];
         if (!ok) break;
-        // a row moves it only when the tile's maximum exceeds it by more than 8
-        // (P <= 2^8 otherwise); O then scales by 2^(old - new)
-        const bool grow = tmax > m_old + 8.f;
-        const float m_new = grow ? tmax : m_old;
-        const bool moves = __any_sync(0xffffffffu, grow);
-        if (moves || t == 0) {
-          sm.m[r] = m_new;
-          __syncwarp();
-        }
-        if (lane == 0) mbar_arrive(smem_u32(&sm.m_ready[gt & 1][wq]));
-        if (busy) {
-          if (t > 0 && moves) {
-            // O holds P V of this unit's earlier tiles: wait for the last, then rescale the row
-            ok = __all_sync(0xffffffffu, wait(sm.pv_done[(gt - 1) % NB], ((gt - 1) / NB) & 1, abort_flag));
+        // a row moves its reference only when the tile's maximum exceeds it by
+        // more than 8 (P <= 2^8 otherwise); O then scales by 2^(old - new)
+        const bool grow = tmax > m_used + 8.f;
+        if (__any_sync(0xffffffffu, grow)) {
+          const float m_new = grow ? tmax : m_used;
+          if (t > 0) {
+            // O holds P V of this unit's earlier tiles: wait for the last, then rescale this half row
+            const bool done = __all_sync(0xffffffffu, wait(sm.pv_done[(gt - 1) % NB], ((gt - 1) / NB) & 1, abort_flag));
+            if (lane == 0) sm.okr[par][wg][wq] = done;
+            named_bar(pair_bar, 64);
+            ok = done && sm.okr[par][wg ^ 1][wq];
             if (!ok) break;
             tc_fence_after();
-            const float alpha = grow ? ex2(m_old - m_new) : 1.f;
+            const float alpha = grow ? ex2(m_used - m_new) : 1.f;
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
+            for (int c = 0; c < D / 2; c += 32) {
               float v[32];
-              tmem_ld32(tmem + lane_base + F::COL_O + 32 * c, v);
+              tmem_ld32(tmem + lane_base + F::COL_O + (D / 2) * wg + c, v);
 #pragma unroll
               for (int i = 0; i < 32; ++i) v[i] *= alpha;
-              tmem_st32(tmem + lane_base + F::COL_O + 32 * c, v);
+              tmem_st32(tmem + lane_base + F::COL_O + (D / 2) * wg + c, v);
             }
+            l *= alpha;
           }
-          if (__any_sync(0xffffffffu, m_new != m_used)) {
-            if (m_new != m_used) l *= m_used == -INFINITY ? 1.f : ex2(m_used - m_new);  // without a reference l is 0 or NaN
-            m_used = m_new;
-          }
-          // a row whose scores so far are all -inf has no reference yet: its P is 0
-          const float nm = (m_used == -INFINITY && !plain) ? 0.f : kBias - m_used;
-          const f32x2 sc2 = pk2(sc, sc), nm2 = pk2(nm, nm);
-          f32x2 sum2[2] = {pk2(0.f, 0.f), pk2(0.f, 0.f)};
-          float(&xa)[32] = *reinterpret_cast<float(*)[32]>(&x[0]);
-          float(&xb)[32] = *reinterpret_cast<float(*)[32]>(&x[32]);
-          // 32 columns of S to 16 of P, over columns that have been read
-          auto weigh = [&](float(&xs)[32], int c) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              float e0, e1;
-              upk2(fma2(pk2(xs[2 * i], xs[2 * i + 1]), sc2, nm2), e0, e1);
-              const float p0 = ex2(e0), p1 = ex2(e1);
-              sum2[i & 1] = add2(sum2[i & 1], pk2(p0, p1));
-              pk[i] = pack2<BF>(p0, p1);
-            }
-            tmem_st16_async(ts + c / 2, pk);
-          };
-          if (KT == 64) {  // the tile's scores are still in x, masked
-            weigh(xa, 0);
-            weigh(xb, 32);
-          } else {
-            tmem_ld32_async(ts, xa);
-            tmem_ld_wait(xa);
-#pragma unroll 1
-            for (int c = 0; c < KT; c += 64) {
-              tmem_ld32_async(ts + c + 32, xb);
-              mask(xa, j0 + c, 32);
-              weigh(xa, c);
-              tmem_ld_wait(xb);
-              if (c + 64 < KT) tmem_ld32_async(ts + c + 64, xa);
-              mask(xb, j0 + c + 32, 32);
-              weigh(xb, c + 32);
-              tmem_ld_wait(xa);
-            }
-          }
-          tmem_st_wait();
-          float s0, s1;
-          upk2(add2(sum2[0], sum2[1]), s0, s1);
-          l += s0 + s1;
+          m_used = m_new;
         }
-        ok = plain || clean_v(u, t, gt);
-        if (!ok) break;
+        // a row whose scores so far are all -inf has no reference yet: its P is 0
+        const float nm = (m_used == -INFINITY && !plain) ? 0.f : kBias - m_used;
+        const f32x2 sc2 = pk2(sc, sc), nm2 = pk2(nm, nm);
+        f32x2 sum2[2] = {pk2(0.f, 0.f), pk2(0.f, 0.f)};
+#pragma unroll
+        for (int c = 0; c < 64; c += 32) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float e0, e1;
+            upk2(fma2(pk2(x[c + 2 * i], x[c + 2 * i + 1]), sc2, nm2), e0, e1);
+            const float p0 = ex2(e0), p1 = ex2(e1);
+            sum2[i & 1] = add2(sum2[i & 1], pk2(p0, p1));
+            pk[i] = pack2<BF>(p0, p1);
+          }
+          tmem_st16_async(ts + 32 * wg + c / 2, pk);
+        }
+        float s0, s1;
+        upk2(add2(sum2[0], sum2[1]), s0, s1);
+        l += s0 + s1;
+        held = plain || clean_v(u, t, gt);
+        tmem_st_wait();
         tc_fence_before();
-        warp_arrive<PAIR>(sm.p_full[sb]);  // spare rows: whatever P holds stays in them
+        if (held) warp_arrive<PAIR>(sm.p_full[sb]);
       }
       if (!ok) break;
-      sm.ml[ui & 1][wg][r] = make_float2(m_used, l);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sm.l_ready));
       g += T;
-      // once every S MMA of this unit has retired the next unit's Q may go in
-      ok = __all_sync(0xffffffffu, wait(sm.s_full[(g - 1) % NB], ((g - 1) / NB) & 1, abort_flag));
-      if (!ok) break;
-      tc_fence_after();
+      // every S MMA of this unit has been consumed: the next unit's Q may go in
       more = next_live(p);
       if (more) load_q(p);
       // ---- epilogue: wait for this unit's last P V, then O (or its partial) out
-      ok = __all_sync(0xffffffffu, wait(sm.l_ready, ui & 1, abort_flag) && wait(sm.o_full, ui & 1, abort_flag));
+      const bool got = __all_sync(0xffffffffu, held && wait(sm.o_full, ui & 1, abort_flag));
       tc_fence_after();
-      if (ok) {
-        const float2 x0 = sm.ml[ui & 1][0][r], x1 = sm.ml[ui & 1][1][r];
-        m_used = fmaxf(x0.x, x1.x);  // references never fall: the later one, which O is scaled by
-        l = m_used == -INFINITY ? x0.y + x1.y : x0.y * ex2(x0.x - m_used) + x1.y * ex2(x1.x - m_used);
+      if (busy) {
+        sm.lsum[wg][r] = l;
+        if (lane == 0) sm.oke[wg][wq] = got;
+        named_bar(pair_bar, 64);
+        l = sm.lsum[0][r] + sm.lsum[1][r];
+        ok = got && sm.oke[wg ^ 1][wq];
+      } else {
+        ok = got;
       }
       if (ok && busy) {
         const int64_t prow = (int64_t)(2 * worker + max(u.slot, 0)) * (kRows * CG) + R;

@@ -92,14 +92,24 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, int c
 
 // issued by the lane with `lead` set, in code that the whole warp runs (several
 // lanes issuing, or one under a branch, took about 200 cycles a copy)
+// CG = 2: bar may lie in the other CTA of the pair.
+template <int CG>
 __device__ __forceinline__ void tma_load_4d(uint32_t lead, uint32_t dst, const void* map, int c0, int c1, int c2,
                                             int c3, uint32_t bar, uint64_t policy) {
-  asm volatile(
-      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %8, 0;\n\t"
-      "@q cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
-      "[%0], [%1, {%2, %3, %4, %5}], [%6], %7;\n\t}\n" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar), "l"(policy), "r"(lead)
-      : "memory");
+  if (CG == 2)
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t.reg .b32 l;\n\tand.b32 l, %8, 1;\n\tsetp.ne.b32 q, l, 0;\n\t"
+        "@q cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2"
+        ".L2::cache_hint [%0], [%1, {%2, %3, %4, %5}], [%6], %7;\n\t}\n" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar), "l"(policy), "r"(lead)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t.reg .b32 l;\n\tand.b32 l, %8, 1;\n\tsetp.ne.b32 q, l, 0;\n\t"
+        "@q cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
+        "[%0], [%1, {%2, %3, %4, %5}], [%6], %7;\n\t}\n" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar), "l"(policy), "r"(lead)
+        : "memory");
 }
 __device__ __forceinline__ uint64_t l2_evict_normal() {
   uint64_t p;
@@ -312,6 +322,13 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
 // proxy fences.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void mbar_expect_tx_cluster(uint32_t bar, uint32_t bytes) {
+  if (PAIR)
+    asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+  else
+    mbar_expect_tx(bar, bytes);
 }
 // one word into the cluster's other CTA, seen there by whoever acquires after a later arrival
 __device__ __forceinline__ void st_cluster(uint32_t cluster_addr, uint32_t v) {
