@@ -13,8 +13,8 @@
 // x 16 from TMEM, bound by reading A); Q in shared memory leaves a CTA alone no
 // room for two 128 KB tiles.  Per tile of 128 keys, one pass with a running
 // maximum and sum:
-//   K, V  by slot, 16 keys at a time, into separate rings of stages by three
-//         producer warps: where the 16 slots are consecutive (pages of 16 and
+//   K, V  by slot, 16 keys at a time, into separate rings of stages by one
+//         producer warp each: where the 16 slots are consecutive (pages of 16 and
 //         more) one TMA box of 16 cache rows x 64 dims per copy, else 16-byte
 //         cp.async row by row (a gather of four rows per TMA copy took 39 ns a
 //         copy, 5 us per 64 KB)
@@ -59,7 +59,7 @@ namespace {
 constexpr int kMaxB = 1024;
 constexpr int kRows = 128;        // query rows of a CTA
 constexpr int kSoftmax = 256;     // two threads per query row, in warps w and w + 4
-constexpr int kCtlWarp = 8, kProdWarp0 = 9, kProdWarps = 3;
+constexpr int kCtlWarp = 8, kProdWarp0 = 9, kTellWarp = 11;  // a producer warp for K, one for V
 constexpr int kThreads = 384;     // twelve warps leave 168 registers a thread
 constexpr uint32_t kTmemCols = 512;
 constexpr int kMaxStages = 12;
@@ -109,7 +109,7 @@ struct Small {
   int64_t warp_sum[kThreads / 32];
   int64_t pre[kMaxB + 1];   // cost of the requests before b
   int qo[kMaxB + 1], kv[kMaxB + 1];
-  int4 slots[kProdWarps][32];
+  int4 slots[2][32];
   int k_mixed[kMaxStages], v_mixed[kMaxStages];  // [stage]: the CTA's part holds rows copied by cp.async
 };
 
@@ -270,12 +270,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       mbar_init(smem_u32(&sm.q_ready), kSoftmax / 32 * CG);
       for (int i = 0; i < kStages; ++i) {
-        // 64 producers' cp.async and an expect_tx; from rank 1 an expect_tx and, once its cp.async are in, an arrival
-        mbar_init(smem_u32(&sm.k_copied[i]), 64);
-        mbar_init(smem_u32(&sm.v_copied[i]), 64);
-        mbar_init(smem_u32(&sm.k_full[i]), 64 + 1 + 2 * (CG - 1));
+        // a warp's cp.async and an expect_tx; from rank 1 an expect_tx and, once its cp.async are in, an arrival
+        mbar_init(smem_u32(&sm.k_copied[i]), 32);
+        mbar_init(smem_u32(&sm.v_copied[i]), 32);
+        mbar_init(smem_u32(&sm.k_full[i]), 32 + 1 + 2 * (CG - 1));
         mbar_init(smem_u32(&sm.k_empty[i]), 1);
-        mbar_init(smem_u32(&sm.v_full[i]), 64 + 1 + 2 * (CG - 1));
+        mbar_init(smem_u32(&sm.v_full[i]), 32 + 1 + 2 * (CG - 1));
         mbar_init(smem_u32(&sm.v_empty[i]), 1);
       }
       for (int i = 0; i < 4; ++i) {
@@ -350,6 +350,29 @@ __global__ void __launch_bounds__(kThreads, 1)
   int64_t w = w0;
   Piece p;
 
+  // Rank 1 of a pair: its boxes complete on rank 0's barriers by themselves; one
+  // thread for K and one for V (each may run ahead of the other) arrives there
+  // for the stage's cp.async rows once those are in, if there are any.  It does so
+  // for every tile: a stage is not reused before, so its parity keeps its meaning.
+  auto tell = [&](uint64_t* copied, uint64_t* full, int* mixed) {
+    if (lane == 0) {
+      int g = 0;
+      bool ok = true;
+      while (ok && next_piece<KT>(sm, P, w, w1, p)) {
+        const int T = p.t1 - p.t0;
+        for (int gt = g; ok && gt < g + T; ++gt) {
+          const int st = gt % kStages;
+          ok = wait(copied[st], (gt / kStages) & 1, abort_flag);
+          if (!ok) break;
+          if (mixed[st]) fence_async_smem();
+          mbar_arrive_cluster(map_rank(smem_u32(&full[st]), 0));
+        }
+        g += T;
+      }
+      if (!ok && !*abort_flag) set_abort(sm, status);
+    }
+    __syncwarp();
+  };
   if (warp == kCtlWarp) {
     if (rank == 0) {
       // ---------------------------------------------------- control: MMAs
@@ -419,175 +442,142 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok && lane == 0 && !*abort_flag) set_abort(sm, status);
       // every MMA issued above has retired before TMEM is freed
       commit(sm.mma_done);
-    } else if (lane == 0) {
-      // rank 1 of a pair: its boxes complete on rank 0's barriers by themselves;
-      // tell rank 0 of the stages that hold cp.async rows as those land
+    } else {
+      tell(sm.k_copied, sm.k_full, sm.k_mixed);
+    }
+    if (lane == 0 && !mbar_wait(smem_u32(&sm.mma_done), 0)) raise_status(status, DFT_DEV_TIMEOUT);
+    __syncwarp();
+  } else if (warp == kTellWarp) {
+    if (rank) tell(sm.v_copied, sm.v_full, sm.v_mixed);
+  } else if (warp >= kProdWarp0) {
+    // ------------------------------------------- producers: paged K/V tiles
+    // A dependent instruction costs a lone warp 4 to 6 cycles, so what a tile
+    // takes is counted in instructions: K and V have code and a warp each (one
+    // body for both, three warps sharing its rows, took 2700 cycles a tile).
+    auto produce = [&](auto v_) {
+      constexpr bool V = decltype(v_)::value;
+      // K: this CTA's rows, all chunks; V: all rows, this CTA's chunks
+      constexpr int NG = V ? KT / 16 : F::KR / 16, NC = V ? F::VC : F::KC;
+      const int g0 = V ? 0 : rank * NG, c0 = V ? rank * NC : 0;
+      uint64_t* full = V ? sm.v_full : sm.k_full;
+      uint64_t* empty = V ? sm.v_empty : sm.k_empty;
+      uint64_t* copied = V ? sm.v_copied : sm.k_copied;
+      int* mixed = V ? sm.v_mixed : sm.k_mixed;
+      const uint32_t ring = V ? v_base : k_base;
+      constexpr uint32_t kStageBytes = V ? F::kVBytes : F::kKBytes;
+      const uint64_t pol_first = l2_evict_first(), pol_keep = l2_evict_normal();
+      const uint64_t pitch = (uint32_t)a.kv_st * 2u;  // bytes, below 2^32
+      const uint32_t lead = elect_lane();
+      int4* slots = sm.slots[V];
       int g = 0;
       bool ok = true;
       while (ok && next_piece<KT>(sm, P, w, w1, p)) {
         const int T = p.t1 - p.t0;
-        for (int gt = g; ok && gt < g + T; ++gt) {
-          const int st = gt % kStages;
-          ok = wait(sm.k_copied[st], (gt / kStages) & 1, abort_flag);
-          if (!ok) break;
-          if (sm.k_mixed[st]) {
-            fence_async_smem();
-            mbar_arrive_cluster(map_rank(smem_u32(&sm.k_full[st]), 0));
-          }
-          ok = wait(sm.v_copied[st], (gt / kStages) & 1, abort_flag);
-          if (!ok) break;
-          if (sm.v_mixed[st]) {
-            fence_async_smem();
-            mbar_arrive_cluster(map_rank(smem_u32(&sm.v_full[st]), 0));
-          }
-        }
-        g += T;
-      }
-      if (!ok && !*abort_flag) set_abort(sm, status);
-    }
-    if (lane == 0 && !mbar_wait(smem_u32(&sm.mma_done), 0)) raise_status(status, DFT_DEV_TIMEOUT);
-    __syncwarp();
-  } else if (warp >= kProdWarp0) {
-    // ------------------------------------------- producers: paged K/V tiles
-    // Code is kept short (loops rolled, K and V through one body): unrolled, the
-    // roles' instructions together starved the warps of each other's.
-    static_assert(KT == 128, "four slots a lane");
-    // Warps 0 and 2 send K's boxes, warp 1 V's; of rows copied by cp.async each does two
-    // turns of three and warp 2 the third, for both.
-    const int pw = warp - kProdWarp0;
-    const uint64_t pol_first = l2_evict_first(), pol_keep = l2_evict_normal();
-    const uint32_t lead = elect_lane();
-    const uint64_t pitch = (uint32_t)a.kv_st * 2u;  // bytes, below 2^32
-    const int* slots = reinterpret_cast<const int*>(sm.slots[pw]);  // the tile's slots, this warp's copy
-    int g = 0;
-    bool ok = true;
-    while (ok && next_piece<KT>(sm, P, w, w1, p)) {
-      const int T = p.t1 - p.t0;
-      if (T == 0) continue;
-      const int32_t* idx = a.kv_indices + sm.kv[p.b];
-      const uint64_t pol = p.once ? pol_first : pol_keep;
-      int s[4];  // slots of keys 4 lane + q of a tile; past the request's end, of its last
-      auto fetch = [&](int tile) {
+        if (T == 0) continue;
+        const int32_t* idx = a.kv_indices + sm.kv[p.b];
+        const uint64_t pol = p.once ? pol_first : pol_keep;
+        int s[4];  // slots of keys 4 lane + q of a tile; past the request's end, of its last
+        auto fetch = [&](int tile) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) s[q] = __ldg(idx + min(tile * KT + 4 * lane + q, p.L - 1));
-      };
-      fetch(p.t0);
+          for (int q = 0; q < 4; ++q) s[q] = __ldg(idx + min(tile * KT + 4 * lane + q, p.L - 1));
+        };
+        fetch(p.t0);
 #pragma unroll 1
-      for (int t = 0; t < T; ++t) {
-        const int gt = g + t, st = gt % kStages, j0 = (p.t0 + t) * KT;
-        const int j = j0 + 4 * lane;
-        bool bad = false;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const bool out = s[q] < 0 || (int64_t)s[q] >= a.n_slots;
-          if (out) s[q] = 0;
-          bad |= out;
-        }
-        if (bad) raise_status(status, DFT_DEV_BAD_INDEX);
-        __syncwarp();
-        sm.slots[pw][lane] = make_int4(s[0], s[1], s[2], s[3]);
-        // boxes: bit 4 i set where the 16 slots of group i are consecutive; keys past the end go along
-        const int first = __shfl_sync(0xffffffffu, s[0], lane & 28);
-        bool run = (int64_t)first + 16 <= a.n_slots;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) run &= j + q >= p.L || s[q] == first + 4 * (lane & 3) + q;
-        uint32_t boxes = __ballot_sync(0xffffffffu, run);
-        boxes &= boxes >> 1;
-        boxes = boxes & boxes >> 2 & 0x11111111u;
-        __syncwarp();
-        if (t + 1 < T) fetch(p.t0 + t + 1);
-        const int live = min(KT / 16, (p.L - j0 + 15) / 16);  // groups with a key; the rest stay as they are
-#pragma unroll 1
-        for (int v = pw & 1; v < (pw == 0 ? 1 : 2); ++v) {
-          // K: this CTA's rows, all chunks; V: all rows, this CTA's chunks
-          const int ng = v ? KT / 16 : F::KR / 16, nc = v ? F::VC : F::KC;
-          const int g0 = v ? 0 : rank * (F::KR / 16), c0 = v ? rank * F::VC : 0;
-          uint64_t& full = v ? sm.v_full[st] : sm.k_full[st];
+        for (int t = 0; t < T; ++t) {
+          const int gt = g + t, st = gt % kStages, j0 = (p.t0 + t) * KT;
+          int4 c = make_int4(s[0], s[1], s[2], s[3]);
+          if (t + 1 < T) fetch(p.t0 + t + 1);
+          const uint32_t n_slots = (uint32_t)a.n_slots;
+          if ((uint32_t)c.x >= n_slots || (uint32_t)c.y >= n_slots || (uint32_t)c.z >= n_slots ||
+              (uint32_t)c.w >= n_slots) {
+            raise_status(status, DFT_DEV_BAD_INDEX);
+            c = make_int4((uint32_t)c.x < n_slots ? c.x : 0, (uint32_t)c.y < n_slots ? c.y : 0,
+                          (uint32_t)c.z < n_slots ? c.z : 0, (uint32_t)c.w < n_slots ? c.w : 0);
+          }
+          // boxes: bit 4 i set where the 16 slots of group i are consecutive; keys past the end go along
+          const int first = __shfl_sync(0xffffffffu, c.x, lane & 28), at0 = first + 4 * (lane & 3);
+          const int left = p.L - j0 - 4 * lane;
+          uint32_t boxes = __ballot_sync(
+              0xffffffffu, (uint32_t)first + 16 <= n_slots && (left <= 0 || c.x == at0) && (left <= 1 || c.y == at0 + 1) &&
+                               (left <= 2 || c.z == at0 + 2) && (left <= 3 || c.w == at0 + 3));
+          boxes &= boxes >> 1;
+          boxes = boxes & boxes >> 2 & 0x11111111u;
+          // groups with a key; the others' rows stay as they are
+          const int n = min(NG, (p.L - j0 + 15) / 16 - g0);
+          const uint32_t mine = n > 0 ? boxes >> 4 * g0 & (0xFFFFFFFFu >> (32 - 4 * n)) : 0u;
           if (gt >= kStages) {
-            ok = __all_sync(0xffffffffu, wait(v ? sm.v_empty[st] : sm.k_empty[st], (gt / kStages - 1) & 1, abort_flag));
-            if (!ok) break;
-          }
-          // rank 0's barrier takes both CTAs' boxes, a rank 1's own its cp.async
-          const uint32_t bar = PAIR ? map_rank(smem_u32(&full), 0) : smem_u32(&full);
-          const uint32_t copied = rank ? smem_u32(v ? &sm.v_copied[st] : &sm.k_copied[st]) : smem_u32(&full);
-          const uint32_t dst = v ? v_base + st * F::kVBytes : k_base + st * F::kKBytes;
-          const int n_groups = min(ng, live - g0);  // may be negative
-          const uint32_t mine = n_groups > 0 ? boxes >> 4 * g0 & (0xFFFFFFFFu >> (32 - 4 * n_groups)) : 0u;
-          if (pw < 2 && lane == 0) {
-            // groups with a key that go by cp.async: their readers need a proxy fence
-            const bool mixed = __popc(mine) < n_groups;
-            (v ? sm.v_mixed : sm.k_mixed)[st] = mixed;
-            mbar_expect_tx_cluster<PAIR>(bar, __popc(mine) * 16 * nc * 128);
-            if (PAIR && rank && !mixed) mbar_arrive_cluster(bar);
-          }
-          __syncwarp();
-          const unsigned char* base =
-              static_cast<const unsigned char*>(v ? a.v_cache : a.k_cache) + ((int64_t)p.h * a.kv_sh + 64 * c0) * 2;
-          // K's boxes by warps 0 and 2 in turn, V's by warp 1
-          if (pw < 2 || !v) {
-#pragma unroll 2
-            for (int i = pw >> 1; i < n_groups; i += v ? 1 : 2) {
-              if (!(mine >> 4 * i & 1)) continue;
-              const int row = slots[16 * (g0 + i)];
-              const uint32_t at = dst + i * nc * 2048;
-              if (v) {
-                tma_load_4d<CG>(lead, at, &v_map, 0, row, c0, p.h, bar, pol);
-              } else {
-                tma_load_4d<CG>(lead, at, &k_map, 0, row, 0, p.h, bar, pol);
-                tma_load_4d<CG>(lead, at + F::KC * 1024, &k_map, 0, row + 8, 0, p.h, bar, pol);
-              }
+            ok = __all_sync(0xffffffffu, wait(empty[st], (gt / kStages - 1) & 1, abort_flag));
+            if (!ok) {
+              g += t;
+              break;
             }
           }
-          if (__popc(mine) < n_groups) {
-            // a group's 16 rows of 8 NC pieces of 16 bytes, 32 pieces a turn
-            auto copy = [&](auto nc_, auto v_) {
-              constexpr int NC = decltype(nc_)::value, kRow = 32 / (8 * NC);  // rows a turn
-              constexpr bool V = decltype(v_)::value;
-              const int lr = lane / (8 * NC), col = lane % (8 * NC);
-              const unsigned char* src = base + col * 16;
-              const uint32_t to = dst + (col >> 3) * (V ? 2048 : 1024) + lr * 128, swz = ((col ^ lr) & 7) << 4;
-              auto turn = [&](int i, int q) {
-                const int row = q * kRow;  // and lr
-                cp_async16(to + i * (NC * 2048) + (V ? row * 128 : (row >> 3) * (NC * 1024) + (row & 7) * 128) +
-                               (swz ^ ((row & 7) << 4)),
-                           src + (uint64_t)(uint32_t)slots[16 * (g0 + i) + row + lr] * pitch, 16u, pol);
-              };
+          // rank 0's barrier takes both CTAs' boxes, a rank 1's own its cp.async
+          const uint32_t bar = PAIR ? map_rank(smem_u32(&full[st]), 0) : smem_u32(&full[st]);
+          const uint32_t dst = ring + st * kStageBytes;
+          const bool copies = __popc(mine) < n;  // their readers need a proxy fence
+          if (lane == 0) {
+            mixed[st] = copies;
+            mbar_expect_tx_cluster<PAIR>(bar, __popc(mine) * 16 * NC * 128);
+          }
+          slots[lane] = c;
+          __syncwarp();
+          auto send = [&](uint32_t go, int i, int row) {
+            const uint32_t at = dst + i * NC * 2048;
+            if (V) {
+              tma_load_4d<CG>(go, at, &v_map, 0, row, c0, p.h, bar, pol);
+            } else {
+              tma_load_4d<CG>(go, at, &k_map, 0, row, 0, p.h, bar, pol);
+              tma_load_4d<CG>(go, at + NC * 1024, &k_map, 0, row + 8, 0, p.h, bar, pol);
+            }
+          };
+          if (lead) {
 #pragma unroll 1
-              for (int i = 0; i < n_groups; ++i) {
-                if (mine >> 4 * i & 1) continue;
-                if (pw == 2) {
+            for (int i = 0; i < n; ++i)
+              if (mine >> 4 * i & 1) send(1, i, reinterpret_cast<const int*>(slots)[16 * (g0 + i)]);
+          }
+          __syncwarp();
+          if (copies) {
+            // a group's 16 rows of 8 NC pieces of 16 bytes, 32 pieces a turn
+            constexpr int kRow = 32 / (8 * NC);  // rows a turn
+            const int lr = lane / (8 * NC), col = lane % (8 * NC);
+            const unsigned char* src = static_cast<const unsigned char*>(V ? a.v_cache : a.k_cache) +
+                                       ((int64_t)p.h * a.kv_sh + 64 * c0) * 2 + col * 16;
+            const uint32_t to = dst + (col >> 3) * (V ? 2048 : 1024) + lr * 128, swz = ((col ^ lr) & 7) << 4;
+            const int* slot = reinterpret_cast<const int*>(slots) + 16 * g0 + lr;
+#pragma unroll 1
+            for (int i = 0; i < n; ++i) {
+              if (mine >> 4 * i & 1) continue;
+              constexpr int kTurns = 4 * NC;
 #pragma unroll
-                  for (int q = 2; q < 4 * NC; q += 3) turn(i, q);
-                } else {
+              for (int q0 = 0; q0 < kTurns; q0 += 4) {
+                int sl[4];
 #pragma unroll
-                  for (int q = 0; q < 4 * NC; ++q)
-                    if (q % 3 != 2) turn(i, q);
+                for (int q = 0; q < 4; ++q) sl[q] = slot[16 * i + (q0 + q) * kRow];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  const int row = (q0 + q) * kRow;  // and lr
+                  cp_async16(to + i * (NC * 2048) + (V ? row * 128 : (row >> 3) * (NC * 1024) + (row & 7) * 128) +
+                                 (swz ^ ((row & 7) << 4)),
+                             src + (uint64_t)(uint32_t)sl[q] * pitch, 16u, pol);
                 }
               }
-            };
-            if (v) copy(Int<F::VC>(), Int<1>());
-            else copy(Int<F::KC>(), Int<0>());
+            }
+            __syncwarp();
           }
-          cp_async_arrive_noinc(copied);
+          cp_async_arrive_noinc(rank ? smem_u32(&copied[st]) : smem_u32(&full[st]));
         }
-        if (!ok) {
-          g += t;
-          break;
-        }
+        if (ok) g += T;
       }
-      if (ok) g += T;
-    }
-    if (!ok && lane == 0 && !*abort_flag) set_abort(sm, status);
-    // The last copies land before the block's shared memory goes, whatever
-    // became of their readers; after an abort tile g may have its K on the way.
-    cp_async_wait_all();
-    if (rank == 0) {
-      for (int gt = max(0, g - kStages); gt < g; ++gt) {
-        mbar_wait(smem_u32(&sm.k_full[gt % kStages]), (gt / kStages) & 1);
-        mbar_wait(smem_u32(&sm.v_full[gt % kStages]), (gt / kStages) & 1);
-      }
-      if (!ok) mbar_wait(smem_u32(&sm.k_full[g % kStages]), (g / kStages) & 1);
-    }
+      if (!ok && lane == 0 && !*abort_flag) set_abort(sm, status);
+      // The last copies land before the block's shared memory goes, whatever
+      // became of their readers (rank 0's barriers take rank 1's boxes too).
+      cp_async_wait_all();
+      if (rank == 0)
+        for (int gt = max(0, g - kStages); gt < g; ++gt) mbar_wait(smem_u32(&full[gt % kStages]), (gt / kStages) & 1);
+    };
+    if (warp == kProdWarp0) produce(Int<0>());
+    else produce(Int<1>());
   } else {
     // ------------- softmax and output, two threads per row, one half of the columns each
     constexpr float kBias = BF ? 0.f : 6.f; // float16 P: up to 2^14, so that small weights stay clear of its smallest step
