@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import threading
 
 import torch
@@ -187,6 +188,36 @@ _lib = None
 _lock = threading.Lock()
 
 
+class Call:
+    """One entry point whose first argument is a struct, called with the
+    struct's fields packed into bytes: `call(fields..., status, stream)`.  A
+    ctypes Structure of twenty fields takes longer to fill than a small kernel
+    to run.  Pointers are ints (0 for none)."""
+
+    _CODE = {i32: "i", i64: "q", f32: "f", vp: "P"}
+
+    def __init__(self, name, cls):
+        fmt = "@" + "".join(self._CODE[t] for _, t in cls._fields_)
+        size = C.sizeof(cls)
+        fmt += f"{size - struct.calcsize(fmt)}x"      # the struct's own tail padding
+        self.name, self.cls, self.pack, self._fn = name, cls, struct.Struct(fmt).pack, None
+        assert struct.calcsize(fmt) == size
+
+    def fn(self):
+        """The C function, with plain pointer arguments."""
+        if self._fn is None:
+            f = lib()[self.name]
+            f.restype = SIGNATURES[self.name][0]
+            f.argtypes = [vp] * len(SIGNATURES[self.name][1])
+            self._fn = f
+        return self._fn
+
+    def __call__(self, fields, *args):
+        rc = (self._fn or self.fn())(self.pack(*fields), *args)
+        if rc != 0:
+            check(rc, self.name)
+
+
 def load(path: str = LIB_PATH):
     """Load the shared library (no device needed) and bind every entry point."""
     global _lib
@@ -230,6 +261,12 @@ def ptr(t) -> int | None:
 
 def stream_handle(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+# the current device's index and a device's current stream, as PyTorch's own
+# compiled code asks for them
+current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or stream_handle
 
 
 def require_cuda(*tensors):

@@ -7,15 +7,19 @@
 // can be captured once and replayed at any lengths.
 #include "dft_common.cuh"
 
+#include <cstring>
+
 using namespace dft;
 
 namespace {
 
 // ================================================================= plan ==
-// Two launches.  plan_kernel is one CTA, a thread per request: needs and
-// offsets are four block-wide prefix sums (pages given back, pages taken, new
-// tokens, keys), then the page moves, spread over the threads by their flat
-// index.  expand_kernel turns the tables into slots over the whole GPU.
+// plan_kernel is one CTA, a thread per request: needs and offsets are four
+// block-wide prefix sums (pages given back, pages taken, new tokens, keys), then
+// the page moves, spread over the threads by their flat index.  The tables then
+// turn into slots: in the same CTA where the maps' capacities are small (a turn
+// of its 1024 threads is 4096 entries, about 0.5 us; a second launch costs 2.5),
+// else by expand_kernel over the whole GPU.
 constexpr int kMaxB = 1024;
 constexpr int kPlanThreads = 1024;
 
@@ -23,6 +27,7 @@ struct PlanShared {
   int64_t warp_sum[4][32];
   int row[kMaxB], need[kMaxB], have[kMaxB];
   int back_off[kMaxB + 1], take_off[kMaxB + 1];
+  int seen[2 * kMaxB];  // hash set of the rows
 };
 
 // inclusive sum over the CTA of four values at once (64-bit: lengths are the
@@ -66,10 +71,70 @@ __device__ __forceinline__ int owner(const int* off, int n, int i) {
   return lo;
 }
 
+// Keys and new tokens to slots; thread `me` of `all`, four entries a turn with
+// one binary search of the offsets (in shared memory).
+__device__ __forceinline__ void expand(const dft_page_plan_args& a, int page_shift, const int* kv, const int* qo, int me,
+                                       int all, int32_t* status) {
+  const int keys = kv[a.B], tokens = qo[a.B];
+  const int in_page = a.page_size - 1;
+  const int64_t step = (int64_t)all * 4;
+  const bool aligned = ((uintptr_t)a.kv_indices & 15) == 0;
+  bool bad = false;
+  auto slot_of = [&](int b, int64_t pos) -> int {
+    const int64_t row = a.rows ? a.rows[b] : b;
+    const int page = a.block_table[row * a.bt_sr + (pos >> page_shift)];
+    const bool ok = page >= 0 && page < a.n_pages;
+    bad |= !ok;
+    return ok ? (page << page_shift) + (int)(pos & in_page) : -1;
+  };
+  for (int64_t i0 = (int64_t)me * 4; i0 < keys; i0 += step) {
+    int b = owner(kv, a.B, (int)i0);
+    const int64_t pos = i0 - kv[b];
+    if (i0 + 3 < kv[b + 1] && page_shift >= 2) {
+      // four keys of one request lie in at most two pages
+      const int s0 = slot_of(b, pos), s3 = (pos & in_page) + 3 <= in_page ? s0 + 3 * (s0 >= 0) : slot_of(b, pos + 3);
+      int s[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const bool here = (pos & in_page) + q <= in_page;
+        s[q] = here ? (s0 < 0 ? -1 : s0 + q) : (s3 < 0 ? -1 : s3 - (3 - q));
+      }
+      if (aligned) {
+        *reinterpret_cast<int4*>(a.kv_indices + i0) = make_int4(s[0], s[1], s[2], s[3]);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) a.kv_indices[i0 + q] = s[q];
+      }
+      continue;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int64_t i = i0 + q;
+      if (i < keys) {
+        while (i >= kv[b + 1]) ++b;
+        a.kv_indices[i] = slot_of(b, i - kv[b]);
+      }
+    }
+  }
+  for (int64_t i = me; i < a.token_capacity; i += all) {
+    int64_t slot = -1, pos = 0;
+    if (i < tokens) {
+      const int b = owner(qo, a.B, (int)i);
+      pos = a.cached[b] + (i - qo[b]);
+      slot = slot_of(b, pos);
+    }
+    a.slot_map[i] = slot;
+    a.positions[i] = pos;
+  }
+  if (bad) raise_status(status, DFT_DEV_BAD_INDEX);
+}
+
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constant__ dft_page_plan_args a,
-                                                            int page_shift, int32_t* status) {
+                                                            int page_shift, int solo, int32_t* status) {
   __shared__ PlanShared sm;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // expand_kernel's blocks wait for this grid's end
   const int b = threadIdx.x;
+  sm.seen[b] = sm.seen[b + kMaxB] = -1;
   const bool live = b < a.B;
   bool bad = false;
   int64_t cached = 0, fresh = 0, row = 0;
@@ -93,12 +158,21 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
   if (bad) cached = fresh = 0, have = need = 0;
   bad |= n_free < 0 || n_free > a.n_pages;
   int64_t v[4] = {have > need ? have - need : 0, need > have ? need - have : 0, fresh, cached + fresh};
-  block_scan4(v, sm);  // also orders sm.row
+  block_scan4(v, sm);  // also orders sm.seen
   int64_t total[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) total[q] = sm.warp_sum[q][31];
-  if (live && !bad)
-    for (int j = 0; j < b; ++j) bad |= sm.row[j] == (int)row;  // a row named twice
+  if (live && !bad) {  // a row named twice: the second to arrive finds the first
+    uint32_t at = (uint32_t)row * 2654435761u >> 21;
+    for (int tries = 0; tries < 2 * kMaxB; ++tries, at = (at + 1) & (2 * kMaxB - 1)) {
+      const int other = atomicCAS(&sm.seen[at], -1, (int)row);
+      if (other == -1) break;
+      if (other == (int)row) {
+        bad = true;
+        break;
+      }
+    }
+  }
   const int64_t depth = n_free + total[0];  // of the stack once everything is given back
   bad |= depth > a.n_pages || total[2] > a.token_capacity || total[3] > a.kv_capacity || total[3] > 0x7FFFFFFF;
   const bool any_bad = __syncthreads_or(bad);
@@ -113,6 +187,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
       a.qo_indptr[b + 1] = 0;
       a.kv_indptr[b + 1] = 0;
     }
+    if (solo)  // the new tokens' maps still say that there are none
+      for (int64_t i = b; i < a.token_capacity; i += kPlanThreads) {
+        a.slot_map[i] = -1;
+        a.positions[i] = 0;
+      }
     return;
   }
   if (threadIdx.x == 0) {
@@ -141,92 +220,75 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
     a.block_table[(int64_t)sm.row[r] * a.bt_sr + sm.have[r] + (i - sm.take_off[r])] =
         a.free_pages[(int)depth - 1 - i];
   }
+  if (!solo) return;
+  // the offsets take the page counts' places
+  int* const qo = sm.back_off;
+  int* const kv = sm.take_off;
+  __syncthreads();
+  if (threadIdx.x == 0) qo[0] = kv[0] = 0;
+  if (live) {
+    qo[b + 1] = (int)v[2];
+    kv[b + 1] = (int)v[3];
+  }
+  __syncthreads();
+  expand(a, page_shift, kv, qo, threadIdx.x, kPlanThreads, status);
 }
 
-// Keys and new tokens to slots, grid-stride over both; the offsets sit in
-// shared memory, one binary search per run of four entries.
 constexpr int kExpandThreads = 256;
+constexpr int64_t kSoloEntries = 16384;  // of either map: up to this plan_kernel writes them itself
 
 __global__ void __launch_bounds__(kExpandThreads) expand_kernel(const __grid_constant__ dft_page_plan_args a,
                                                                 int page_shift, int32_t* status) {
   __shared__ int kv[kMaxB + 1], qo[kMaxB + 1];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   for (int i = threadIdx.x; i <= a.B; i += kExpandThreads) {
     kv[i] = a.kv_indptr[i];
     qo[i] = a.qo_indptr[i];
   }
   __syncthreads();
-  const int keys = kv[a.B], tokens = qo[a.B];
-  const int in_page = a.page_size - 1;
-  const int64_t step = (int64_t)gridDim.x * kExpandThreads * 4;
-  bool bad = false;
-  auto slot_of = [&](int b, int64_t pos) -> int {
-    const int64_t row = a.rows ? a.rows[b] : b;
-    const int page = a.block_table[row * a.bt_sr + (pos >> page_shift)];
-    const bool ok = page >= 0 && page < a.n_pages;
-    bad |= !ok;
-    return ok ? (page << page_shift) + (int)(pos & in_page) : -1;
-  };
-  const int64_t first = ((int64_t)blockIdx.x * kExpandThreads + threadIdx.x) * 4;
-  for (int64_t i0 = first; i0 < keys; i0 += step) {
-    int b = owner(kv, a.B, (int)i0);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int64_t i = i0 + q;
-      if (i < keys) {
-        while (i >= kv[b + 1]) ++b;
-        a.kv_indices[i] = slot_of(b, i - kv[b]);
-      }
-    }
-  }
-  for (int64_t i0 = first; i0 < a.token_capacity; i0 += step) {
-    int b = i0 < tokens ? owner(qo, a.B, (int)i0) : 0;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int64_t i = i0 + q;
-      if (i < tokens) {
-        while (i >= qo[b + 1]) ++b;
-        const int64_t pos = a.cached[b] + (i - qo[b]);
-        a.slot_map[i] = slot_of(b, pos);
-        a.positions[i] = pos;
-      } else if (i < a.token_capacity) {
-        a.slot_map[i] = -1;
-        a.positions[i] = 0;
-      }
-    }
-  }
-  if (bad) raise_status(status, DFT_DEV_BAD_INDEX);
+  expand(a, page_shift, kv, qo, blockIdx.x * kExpandThreads + threadIdx.x, gridDim.x * kExpandThreads, status);
 }
 
 // =============================================================== append ==
-// A copy: each of K and V is read once and written once, V-byte pieces, one
-// thread per piece and turn.  Bound by HBM at prompt sizes, by the launch for
-// a decode batch.
-constexpr int kAppendThreads = 256;
+// A copy: each of K and V is read once and written once.  A block takes eight
+// tokens, a thread columns of the row (K's pieces of V bytes, then V's): where a
+// column lies in its head is worked out once, and four tokens' pieces are in
+// flight at a time.  Bound by HBM at prompt sizes, by the launch for a decode
+// batch.
+constexpr int kAppendThreads = 256, kAppendTokens = 8, kAppendBatch = 4;
 
 template <typename V>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ dft_kv_append_args a,
                                                                 int32_t* status) {
   constexpr int kElems = sizeof(V) / 2;
   const int per_head = a.D / kElems, per_row = a.Hkv * per_head;
-  const int64_t pieces = a.T * per_row * 2;
-  const uint16_t* src[2] = {static_cast<const uint16_t*>(a.k), static_cast<const uint16_t*>(a.v)};
-  uint16_t* dst[2] = {static_cast<uint16_t*>(a.k_cache), static_cast<uint16_t*>(a.v_cache)};
-  for (int64_t i = (int64_t)blockIdx.x * kAppendThreads + threadIdx.x; i < pieces;
-       i += (int64_t)gridDim.x * kAppendThreads) {
-    const int64_t t = i / (2 * per_row);
-    int c = (int)(i - t * (2 * per_row));
-    const int which = c >= per_row;
-    c -= which * per_row;
-    const int h = c / per_head, e = (c - h * per_head) * kElems;
-    const int64_t slot = a.slot_map[t];
-    if (slot < 0) continue;
-    if (slot >= a.n_slots) {
-      raise_status(status, DFT_DEV_BAD_INDEX);
-      continue;
+  __shared__ int64_t slots[kAppendTokens];
+  for (int64_t t0 = (int64_t)blockIdx.x * kAppendTokens; t0 < a.T; t0 += (int64_t)gridDim.x * kAppendTokens) {
+    const int n = (int)min((int64_t)kAppendTokens, a.T - t0);
+    __syncthreads();
+    if (threadIdx.x < n) {
+      const int64_t slot = a.slot_map[t0 + threadIdx.x];
+      if (slot >= a.n_slots) raise_status(status, DFT_DEV_BAD_INDEX);
+      slots[threadIdx.x] = slot >= a.n_slots ? -1 : slot;
     }
-    const int64_t from = which ? t * a.v_st + h * a.v_sh : t * a.k_st + h * a.k_sh;
-    *reinterpret_cast<V*>(dst[which] + slot * a.kv_st + h * a.kv_sh + e) =
-        *reinterpret_cast<const V*>(src[which] + from + e);
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * per_row; c += kAppendThreads) {
+      const int which = c >= per_row, cc = c - which * per_row;
+      const int h = cc / per_head, e = (cc - h * per_head) * kElems;
+      const int64_t step = which ? a.v_st : a.k_st;
+      const uint16_t* src = static_cast<const uint16_t*>(which ? a.v : a.k) + t0 * step + h * (which ? a.v_sh : a.k_sh) + e;
+      uint16_t* dst = static_cast<uint16_t*>(which ? a.v_cache : a.k_cache) + h * a.kv_sh + e;
+#pragma unroll
+      for (int i0 = 0; i0 < kAppendTokens; i0 += kAppendBatch) {
+        V x[kAppendBatch];
+#pragma unroll
+        for (int i = 0; i < kAppendBatch; ++i)
+          if (i0 + i < n) x[i] = *reinterpret_cast<const V*>(src + (i0 + i) * step);
+#pragma unroll
+        for (int i = 0; i < kAppendBatch; ++i)
+          if (i0 + i < n && slots[i0 + i] >= 0) *reinterpret_cast<V*>(dst + slots[i0 + i] * a.kv_st) = x[i];
+      }
+    }
   }
 }
 
@@ -321,13 +383,25 @@ extern "C" int dft_page_plan(const dft_page_plan_args* a, int32_t* dev_status, v
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   int shift = 0;
   while ((1 << shift) < a->page_size) ++shift;
-  plan_kernel<<<1, kPlanThreads, 0, st>>>(*a, shift, dev_status);
-  DFT_LAUNCH_CHECK();
   const int64_t most = a->kv_capacity > a->token_capacity ? a->kv_capacity : a->token_capacity;
-  int64_t grid = (most + kExpandThreads * 4 - 1) / (kExpandThreads * 4);
-  grid = grid < 1 ? 1 : grid > 148 * 4 ? 148 * 4 : grid;
-  expand_kernel<<<(unsigned)grid, kExpandThreads, 0, st>>>(*a, shift, dev_status);
+  const bool solo = most <= kSoloEntries;
+  plan_kernel<<<1, kPlanThreads, 0, st>>>(*a, shift, solo, dev_status);
   DFT_LAUNCH_CHECK();
+  if (solo) return DFT_OK;
+  int64_t grid = (most + kExpandThreads * 4 - 1) / (kExpandThreads * 4);
+  if (grid > 148 * 8) grid = 148 * 8;
+  // its blocks come up while plan_kernel runs and wait for its end
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kExpandThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  DFT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, expand_kernel, *a, shift, dev_status));
   return DFT_OK;
 }
 
@@ -340,9 +414,8 @@ extern "C" int dft_kv_append(const dft_kv_append_args* a, int32_t* dev_status, v
   const bool wide = al16(a->k) && al16(a->v) && al16(a->k_cache) && al16(a->v_cache) && a->D % 8 == 0 &&
                     a->k_st % 8 == 0 && a->k_sh % 8 == 0 && a->v_st % 8 == 0 && a->v_sh % 8 == 0 &&
                     a->kv_st % 8 == 0 && a->kv_sh % 8 == 0;
-  const int64_t pieces = a->T * a->Hkv * (wide ? a->D / 8 : a->D) * 2;
-  int64_t grid = (pieces + kAppendThreads - 1) / kAppendThreads;
-  if (grid > 148 * 32) grid = 148 * 32;
+  int64_t grid = (a->T + kAppendTokens - 1) / kAppendTokens;
+  if (grid > 65535 * 16) grid = 65535 * 16;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (wide) append_kernel<uint4><<<(unsigned)grid, kAppendThreads, 0, st>>>(*a, dev_status);
   else append_kernel<uint16_t><<<(unsigned)grid, kAppendThreads, 0, st>>>(*a, dev_status);

@@ -519,39 +519,36 @@ def tree_attention(q, k_cache, v_cache, kv_indptr, kv_indices, anc, max_kv_len=N
 
 
 # --------------------------------------------------------- paged KV cache --
+_PAGE_PLAN = L.Call("dft_page_plan", L.PagePlanArgs)
+_KV_APPEND = L.Call("dft_kv_append", L.KvAppendArgs)
+_KV_COMMIT = L.Call("dft_kv_commit", L.KvCommitArgs)
+_CHUNK_ATTN = L.Call("dft_chunk_attn", L.ChunkAttnArgs)
+_CHUNK_ATTN_BYTES = {}      # workspace bytes by (device, head dim): they depend on nothing else
+
+
 def _on_current_device(what, *tensors):
-    """Every tensor on the current CUDA device (the stream's)."""
-    cur = torch.cuda.current_device()
+    """Every tensor on the current CUDA device (the stream's), whose index is
+    returned."""
+    if not torch.cuda.is_initialized():
+        L.lib()
+        torch.cuda.init()
+    cur = L.current_device()
     for t in tensors:
         if t is not None and t.get_device() != cur:
             raise L.DFTError(f"{what}: every tensor must be on the current CUDA device (cuda:{cur}), got one on "
                              f"{t.device}")
+    return cur
 
 
-def _want(what, ok, msg):
-    if not ok:
-        raise L.DFTError(f"{what}: {msg}")
-
-
-def _stride(t, d):
-    """Element stride of dim d; of a dim of size 1, whose stride means nothing,
-    that of a contiguous tensor."""
-    if t.shape[d] != 1:
-        return t.stride(d)
-    n = 1
-    for size in t.shape[d + 1:]:
-        n *= size
-    return n
+def _at(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def _ids(t, dtype):
     return t if t.dtype is dtype and t.is_contiguous() else t.to(dtype).contiguous()
 
 
-def _cache_pair(what, k_cache, v_cache):
-    _want(what, v_cache.shape == k_cache.shape and v_cache.stride() == k_cache.stride() and
-          v_cache.dtype is k_cache.dtype, "k_cache and v_cache must have one shape, dtype and set of strides")
-    _want(what, k_cache.shape[-1] <= 1 or k_cache.stride(-1) == 1, "the cache's head dim must be contiguous")
+_HALF = {torch.bfloat16: L.DFT_BF16, torch.float16: L.DFT_F16}
 
 
 def page_plan_outputs(B, tokens, keys, device):
@@ -575,35 +572,42 @@ def page_plan(cached, fresh, block_table, held, free_pages, n_free, page_size, r
     them made, with room for every slot of the cache.  Returns out.  A plan
     that cannot be made changes no page and yields empty offsets; `status`
     [1] int32 takes the reason."""
-    w = "page_plan"
-    B = cached.numel()
-    n_pages = free_pages.numel()
-    _want(w, fresh.numel() == B and (rows is None or rows.numel() == B), "cached, fresh and rows hold B entries each")
-    _want(w, block_table.dim() == 2 and (block_table.shape[1] <= 1 or block_table.stride(1) == 1),
-          "block_table is [rows, max_pages], its pages contiguous")
-    _want(w, block_table.dtype is torch.int32 and held.dtype is torch.int32 and free_pages.dtype is torch.int32 and
-          n_free.dtype is torch.int32, "block_table, held, free_pages and n_free are int32")
-    _want(w, held.is_contiguous() and free_pages.is_contiguous() and held.numel() == block_table.shape[0] and
-          n_free.numel() == 1, "held [rows] and free_pages are contiguous, n_free holds one count")
-    _want(w, rows is not None or B <= block_table.shape[0], "more requests than table rows")
+    B, n_pages, page_size = cached.numel(), free_pages.numel(), int(page_size)
+    i32, i64 = torch.int32, torch.int64
+    if fresh.numel() != B or (rows is not None and rows.numel() != B):
+        raise L.DFTError("page_plan: cached, fresh and rows hold B entries each")
+    if block_table.dim() != 2:
+        raise L.DFTError("page_plan: block_table is [rows, max_pages]")
+    n_rows, max_pages = block_table.shape
+    pitch, across = block_table.stride()
+    if n_rows == 1:
+        pitch = max_pages
+    if max_pages > 1 and across != 1:
+        raise L.DFTError("page_plan: a row's pages must be contiguous")
+    if not (block_table.dtype is held.dtype is free_pages.dtype is n_free.dtype is i32):
+        raise L.DFTError("page_plan: block_table, held, free_pages and n_free are int32")
+    if not (held.is_contiguous() and free_pages.is_contiguous() and held.numel() == n_rows and n_free.numel() == 1):
+        raise L.DFTError("page_plan: held [rows] and free_pages are contiguous, n_free holds one count")
+    if rows is None and B > n_rows:
+        raise L.DFTError("page_plan: more requests than table rows")
     if out is None:
-        _want(w, tokens is not None, "pass out, or tokens (a bound on the new tokens)")
-        out = page_plan_outputs(B, int(tokens), n_pages * int(page_size), block_table.device)
-    qo, kv, idx, slots, pos = (out[k] for k in ("qo_indptr", "kv_indptr", "kv_indices", "slot_map", "positions"))
-    _want(w, qo.dtype is torch.int32 and kv.dtype is torch.int32 and idx.dtype is torch.int32 and
-          slots.dtype is torch.int64 and pos.dtype is torch.int64, "out: offsets and indices int32, the rest int64")
-    _want(w, qo.numel() == B + 1 and kv.numel() == B + 1 and pos.numel() == slots.numel() and
-          qo.is_contiguous() and kv.is_contiguous() and idx.is_contiguous() and slots.is_contiguous() and
-          pos.is_contiguous(), "out: contiguous, offsets of B + 1 entries, slot_map and positions alike")
-    lib = L.lib()
-    _on_current_device(w, cached, fresh, rows, block_table, held, free_pages, n_free, qo, kv, idx, slots, pos, status)
+        if tokens is None:
+            raise L.DFTError("page_plan: pass out, or tokens (a bound on the new tokens)")
+        out = page_plan_outputs(B, int(tokens), n_pages * page_size, block_table.device)
+    qo, kv, idx, slots, pos = out["qo_indptr"], out["kv_indptr"], out["kv_indices"], out["slot_map"], out["positions"]
+    n_keys, n_tokens = idx.numel(), slots.numel()
+    if not (qo.dtype is kv.dtype is idx.dtype is i32 and slots.dtype is pos.dtype is i64):
+        raise L.DFTError("page_plan: out's offsets and indices are int32, slot_map and positions int64")
+    if not (qo.numel() == kv.numel() == B + 1 and pos.numel() == n_tokens and qo.is_contiguous() and
+            kv.is_contiguous() and idx.is_contiguous() and slots.is_contiguous() and pos.is_contiguous()):
+        raise L.DFTError("page_plan: out holds contiguous offsets of B + 1 entries, slot_map and positions alike")
+    cur = _on_current_device("page_plan", cached, fresh, rows, block_table, held, free_pages, n_free, qo, kv, idx, slots, pos, status)
     cached, fresh = _ids(cached, torch.int64), _ids(fresh, torch.int64)
     rows = None if rows is None else _ids(rows, torch.int64)
-    a = L.PagePlanArgs(B, int(page_size), cached.data_ptr(), fresh.data_ptr(), L.ptr(rows), block_table.data_ptr(),
-                       _stride(block_table, 0), block_table.shape[0], block_table.shape[1], held.data_ptr(),
-                       free_pages.data_ptr(), n_free.data_ptr(), n_pages, qo.data_ptr(), kv.data_ptr(),
-                       idx.data_ptr(), idx.numel(), slots.data_ptr(), pos.data_ptr(), slots.numel())
-    L.check(lib.dft_page_plan(C.byref(a), _status_ptr(status), L.stream_handle()), "dft_page_plan")
+    _PAGE_PLAN((B, page_size, cached.data_ptr(), fresh.data_ptr(), _at(rows), block_table.data_ptr(), pitch, n_rows,
+                max_pages, held.data_ptr(), free_pages.data_ptr(), n_free.data_ptr(), n_pages, qo.data_ptr(),
+                kv.data_ptr(), idx.data_ptr(), n_keys, slots.data_ptr(), pos.data_ptr(), n_tokens), _at(status),
+               L.raw_stream(cur))
     return out
 
 
@@ -611,21 +615,21 @@ def kv_append(k, v, k_cache, v_cache, slot_map, status=None):
     """cache[slot_map[t]] = k[t], v[t]: k, v [T, Hkv, D] (any token and head
     strides), k_cache / v_cache [slots, Hkv, D], slot_map [T] (negative: the row
     is skipped; otherwise distinct).  16-bit types, in place."""
-    w = "kv_append"
-    T, Hkv, D = k.shape
-    _want(w, v.shape == k.shape and k_cache.dim() == 3 and tuple(k_cache.shape[1:]) == (Hkv, D) and
-          slot_map.numel() == T, "k, v [T, Hkv, D], caches [slots, Hkv, D], slot_map [T]")
-    _cache_pair(w, k_cache, v_cache)
-    _want(w, k.dtype is v.dtype and k.dtype is k_cache.dtype and k.dtype in (torch.bfloat16, torch.float16),
-          "k, v and the caches must be alike bfloat16 or float16")
-    _want(w, D <= 1 or (k.stride(2) == 1 and v.stride(2) == 1), "the head dim of k and v must be contiguous")
-    lib = L.lib()
-    _on_current_device(w, k, v, k_cache, v_cache, slot_map, status)
+    shape, rows = k.shape, k_cache.shape
+    T, Hkv, D = shape
+    if not (v.shape == shape and rows == v_cache.shape and len(rows) == 3 and rows[1] == Hkv and rows[2] == D and
+            slot_map.numel() == T):
+        raise L.DFTError("kv_append: k, v [T, Hkv, D], caches [slots, Hkv, D], slot_map [T]")
+    dtype = _HALF.get(k.dtype)
+    if dtype is None or not (k.dtype is v.dtype is k_cache.dtype is v_cache.dtype):
+        raise L.DFTError("kv_append: k, v and the caches must be alike bfloat16 or float16")
+    ks, vs, cs = k.stride(), v.stride(), k_cache.stride()
+    if v_cache.stride() != cs or (D > 1 and not ks[2] == vs[2] == cs[2] == 1):
+        raise L.DFTError("kv_append: k_cache and v_cache need equal strides, and every head dim contiguous elements")
+    cur = _on_current_device("kv_append", k, v, k_cache, v_cache, slot_map, status)
     slot_map = _ids(slot_map, torch.int64)
-    a = L.KvAppendArgs(T, Hkv, D, L.dtype_code(k), k.data_ptr(), _stride(k, 0), _stride(k, 1), v.data_ptr(),
-                       _stride(v, 0), _stride(v, 1), k_cache.data_ptr(), v_cache.data_ptr(), _stride(k_cache, 0),
-                       _stride(k_cache, 1), k_cache.shape[0], slot_map.data_ptr())
-    L.check(lib.dft_kv_append(C.byref(a), _status_ptr(status), L.stream_handle()), "dft_kv_append")
+    _KV_APPEND((T, Hkv, D, dtype, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], k_cache.data_ptr(),
+                v_cache.data_ptr(), cs[0], cs[1], rows[0], slot_map.data_ptr()), _at(status), L.raw_stream(cur))
 
 
 def kv_commit(k_cache, v_cache, kv_indptr, kv_indices, path, accept_len, N, status=None):
@@ -633,22 +637,35 @@ def kv_commit(k_cache, v_cache, kv_indptr, kv_indices, path, accept_len, N, stat
     v_cache [slots, Hkv, D] or [layers, slots, Hkv, D]; the last N keys of each
     request are its tree; path [B, P] and accept_len [B] as accept_greedy
     returns them."""
-    w = "kv_commit"
-    _cache_pair(w, k_cache, v_cache)
-    if k_cache.dim() == 3:
-        k_cache, v_cache = k_cache.unsqueeze(0), v_cache.unsqueeze(0)
-    _want(w, k_cache.dim() == 4 and path.dim() == 2, "caches [layers, slots, Hkv, D], path [B, P]")
-    Ln, slots, Hkv, D = k_cache.shape
+    shape, cs = k_cache.shape, k_cache.stride()
+    if v_cache.shape != shape or v_cache.stride() != cs or len(shape) not in (3, 4) or path.dim() != 2:
+        raise L.DFTError("kv_commit: k_cache and v_cache [layers, slots, Hkv, D] of equal strides, path [B, P]")
+    if len(shape) == 3:
+        shape, cs = (1, *shape), (0, *cs)
+    Ln, slots, Hkv, D = shape
     B, P = path.shape
-    _want(w, accept_len.numel() == B and kv_indptr.numel() == B + 1, "accept_len [B], kv_indptr [B + 1]")
-    lib = L.lib()
-    _on_current_device(w, k_cache, v_cache, kv_indptr, kv_indices, path, accept_len, status)
+    if accept_len.numel() != B or kv_indptr.numel() != B + 1:
+        raise L.DFTError("kv_commit: accept_len [B], kv_indptr [B + 1]")
+    dtype = _HALF.get(k_cache.dtype)
+    if dtype is None or v_cache.dtype is not k_cache.dtype or (D > 1 and cs[3] != 1):
+        raise L.DFTError("kv_commit: the caches must be alike bfloat16 or float16, their head dim contiguous")
+    cur = _on_current_device("kv_commit", k_cache, v_cache, kv_indptr, kv_indices, path, accept_len, status)
     kv_indptr, kv_indices = _ids(kv_indptr, torch.int32), _ids(kv_indices, torch.int32)
     path, accept_len = _ids(path, torch.int64), _ids(accept_len, torch.int64)
-    a = L.KvCommitArgs(Ln, B, int(N), P, Hkv, D, L.dtype_code(k_cache), k_cache.data_ptr(), v_cache.data_ptr(),
-                       _stride(k_cache, 0), _stride(k_cache, 1), _stride(k_cache, 2), slots, kv_indptr.data_ptr(),
-                       kv_indices.data_ptr(), kv_indices.numel(), path.data_ptr(), accept_len.data_ptr())
-    L.check(lib.dft_kv_commit(C.byref(a), _status_ptr(status), L.stream_handle()), "dft_kv_commit")
+    _KV_COMMIT((Ln, B, int(N), P, Hkv, D, dtype, k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2], slots,
+                kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(), path.data_ptr(),
+                accept_len.data_ptr()), _at(status), L.raw_stream(cur))
+
+
+def _chunk_attn_bytes(device, D):
+    """dft_chunk_attn_workspace_bytes for the current device and head dim D."""
+    one = 0x1000        # placeholder pointers: the sizes alone are read
+    a = L.ChunkAttnArgs(1, 1, 1, 1, D, L.DFT_BF16, one, D, D, one, one, D, D, 1, one, one, one, 1, 1.0, one, D, D)
+    need = L.lib().dft_chunk_attn_workspace_bytes(C.byref(a))
+    if need < 0:
+        raise L.DFTError(f"chunk_attention: head dim {D} is not one of 64, 128, 256")
+    _CHUNK_ATTN_BYTES[device, D] = need
+    return need
 
 
 def chunk_attention(q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, sm_scale=None, o=None, workspace=None,
@@ -660,39 +677,48 @@ def chunk_attention(q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, sm_sc
     256}.  Returns o [T, Hq, D]; rows of q outside every request are not
     written (pass o to keep what they hold).  workspace: uint8, at least
     dft_chunk_attn_workspace_bytes, for this call alone; made here if None."""
-    w = "chunk_attention"
-    T, Hq, D = q.shape
-    _want(w, k_cache.dim() == 3 and k_cache.shape[2] == D, "q [T, Hq, D], caches [slots, Hkv, D]")
-    _cache_pair(w, k_cache, v_cache)
-    _want(w, q.dtype is k_cache.dtype and q.dtype in (torch.bfloat16, torch.float16),
-          "q and the caches must be alike bfloat16 or float16")
-    _want(w, q.stride(2) == 1, "the head dim of q must be contiguous")
+    T, Hq, D = shape = q.shape
+    slots, Hkv, cd = rows = k_cache.shape
+    qs, cs = q.stride(), k_cache.stride()
+    if rows != v_cache.shape or cd != D or v_cache.stride() != cs or qs[2] != 1 or cs[2] != 1:
+        raise L.DFTError("chunk_attention: q [T, Hq, D], k_cache and v_cache [slots, Hkv, D] of equal strides, head "
+                         "dims contiguous")
+    dtype = _HALF.get(q.dtype)
+    if dtype is None or not (q.dtype is k_cache.dtype is v_cache.dtype):
+        raise L.DFTError("chunk_attention: q and the caches must be alike bfloat16 or float16")
     if o is None:
-        o = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
+        o = torch.empty(shape, dtype=q.dtype, device=q.device)
+        os = (Hq * D, D)
     else:
-        _want(w, o.shape == q.shape and o.dtype is q.dtype and o.stride(2) == 1,
-              "o must be [T, Hq, D] of q's type, its head dim contiguous")
+        os = o.stride()
+        if o.shape != shape or o.dtype is not q.dtype or os[2] != 1:
+            raise L.DFTError("chunk_attention: o must be [T, Hq, D] of q's type, its head dim contiguous")
     B = qo_indptr.numel() - 1
-    _want(w, B >= 0 and kv_indptr.numel() == B + 1, "qo_indptr and kv_indptr hold B + 1 offsets each")
-    lib = L.lib()
-    _on_current_device(w, q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, o, workspace, status)
+    if B < 0 or kv_indptr.numel() != B + 1:
+        raise L.DFTError("chunk_attention: qo_indptr and kv_indptr hold B + 1 offsets each")
+    cur = _on_current_device("chunk_attention", q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, o, workspace,
+                             status)
     qo_indptr, kv_indptr = _ids(qo_indptr, torch.int32), _ids(kv_indptr, torch.int32)
     kv_indices = _ids(kv_indices, torch.int32)
-    a = L.ChunkAttnArgs(B, T, Hq, k_cache.shape[1], D, L.dtype_code(q), q.data_ptr(), _stride(q, 0), _stride(q, 1),
-                        k_cache.data_ptr(), v_cache.data_ptr(), _stride(k_cache, 0), _stride(k_cache, 1),
-                        k_cache.shape[0], qo_indptr.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(),
-                        kv_indices.numel(), float(D ** -0.5 if sm_scale is None else sm_scale), o.data_ptr(),
-                        _stride(o, 0), _stride(o, 1))
-    need = lib.dft_chunk_attn_workspace_bytes(C.byref(a))
-    if need < 0:
-        raise L.DFTError("chunk_attention: outside what the kernel takes (D in {64, 128, 256}, Hq a multiple of Hkv "
-                         "with at most 128 q-heads each, at most 1024 requests, 16-byte aligned rows, sm_scale > 0)")
-    if need > 0:
-        if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-        else:
-            _want(w, workspace.is_contiguous() and workspace.numel() * workspace.element_size() >= need,
-                  f"workspace needs {need} contiguous bytes")
-    L.check(lib.dft_chunk_attn(C.byref(a), workspace.data_ptr() if need else None, _status_ptr(status),
-                               L.stream_handle()), "dft_chunk_attn")
+    need = _CHUNK_ATTN_BYTES.get((cur, D)) or _chunk_attn_bytes(cur, D)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    elif not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
+        raise L.DFTError(f"chunk_attention: workspace needs {need} contiguous bytes")
+    # strides of dims of size 1 mean nothing
+    q_st, o_st = (Hq * D, Hq * D) if T == 1 else (qs[0], os[0])
+    q_sh, o_sh = (D, D) if Hq == 1 else (qs[1], os[1])
+    kv_sh = D if Hkv == 1 else cs[1]
+    kv_st = Hkv * D if slots == 1 else cs[0]
+    try:
+        _CHUNK_ATTN((B, T, Hq, Hkv, D, dtype, q.data_ptr(), q_st, q_sh, k_cache.data_ptr(), v_cache.data_ptr(), kv_st,
+                     kv_sh, slots, qo_indptr.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(),
+                     kv_indices.numel(), D ** -0.5 if sm_scale is None else sm_scale, o.data_ptr(), o_st, o_sh),
+                    workspace.data_ptr(), _at(status), L.raw_stream(cur))
+    except L.DFTError as e:
+        if e.status == L.DFT_ERR_UNSUPPORTED:
+            raise L.DFTError("chunk_attention: outside what the kernel takes (D in {64, 128, 256}, Hq a multiple of "
+                             "Hkv with at most 128 q-heads each, at most 1024 requests, 16-byte aligned rows)",
+                             e.status) from None
+        raise
     return o

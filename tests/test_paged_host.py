@@ -46,6 +46,12 @@ def test_struct_layouts_match_the_header(tmp_path):
         assert got == int(val), (name, field)
 
 
+@pytest.mark.parametrize("call", [K._PAGE_PLAN, K._KV_APPEND, K._KV_COMMIT, K._CHUNK_ATTN], ids=lambda c: c.name)
+def test_packed_fields_are_the_struct(call):
+    v = [3.5 if t is L.f32 else 1 << 20 | i for i, (_, t) in enumerate(call.cls._fields_)]
+    assert call.pack(*v) == bytes(call.cls(*v))
+
+
 def _plan(**kw):
     d = dict(B=2, page_size=16, cached=FAKE, fresh=FAKE, rows=None, block_table=FAKE, bt_sr=8, n_rows=4, max_pages=8,
              held=FAKE, free_pages=FAKE, n_free=FAKE, n_pages=32, qo_indptr=FAKE, kv_indptr=FAKE, kv_indices=FAKE,
