@@ -59,10 +59,10 @@ namespace {
 constexpr int kMaxB = 1024;
 constexpr int kRows = 128;        // query rows of a CTA
 constexpr int kSoftmax = 256;     // two threads per query row, in warps w and w + 4
-constexpr int kCtlWarp = 8, kProdWarp0 = 9, kTellWarp = 11;  // a producer warp for K, one for V
+constexpr int kCtlWarp = 8, kProdWarp0 = 9, kPlanWarp = 11;  // a producer warp for K, one for V
 constexpr int kThreads = 384;     // twelve warps leave 168 registers a thread
 constexpr uint32_t kTmemCols = 512;
-constexpr int kMaxStages = 12;
+constexpr int kMaxStages = 12, kRing = 4;
 // A unit's fixed cost in keys (query load, first tile's latency, output), and
 // the least share of a worker: under it a cut costs more than it spreads.
 constexpr int kUnitKeys = 256;
@@ -91,13 +91,22 @@ struct Cfg {
   static_assert(COL_S + NB * KT <= kTmemCols, "TMEM");
 };
 
+// A worker's part of one unit: key tiles [t0, t1) of nt.  b < 0: there are no more.
+struct Piece {
+  int b, h, tok0, ntok;  // first token row of q, tokens
+  int vis0, L;           // keys that the first token sees (may be negative), keys of the request
+  int t0, t1;
+  int slot;              // -1: the whole unit; 0 / 1: partial that continues / begins it
+  bool last, once;       // the unit's last tiles; its keys are read by this tile alone
+};
+
 struct Small {
   uint64_t q_ready;
   uint64_t k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages];
-  uint64_t k_copied[kMaxStages], v_copied[kMaxStages];  // rank 1 of a pair: its cp.async rows of the stage
   uint64_t s_full[4], p_full[4], pv_done[4];
   uint64_t v_here[4];       // rank 1 of a pair: [S buffer] the tile's V is in (its boxes complete on rank 0)
   uint64_t o_full, o_free, mma_done;
+  uint64_t ring_full[kRing], ring_empty[kRing];
   uint32_t tmem_base;
   int abort;
   int odd[8];               // [piece & 7] = piece + 1 when one of its masked tiles held a non-finite value
@@ -106,9 +115,11 @@ struct Small {
   int okx[2][2][4];         // [tile parity][half][row warp] wait outcomes, shared by a row's two warps
   int okr[2][2][4];         // the same for the rescale's wait
   int oke[2][4];            // [half][row warp] the epilogue's wait
+  int okt[2][2][4];         // [unit parity][half][row warp] whether the warp goes on to the next unit
   int64_t warp_sum[kThreads / 32];
   int64_t pre[kMaxB + 1];   // cost of the requests before b
   int qo[kMaxB + 1], kv[kMaxB + 1];
+  Piece ring[kRing];           // the worker's pieces as they come, from the plan warp
   int4 slots[2][32];
   int k_mixed[kMaxStages], v_mixed[kMaxStages];  // [stage]: the CTA's part holds rows copied by cp.async
 };
@@ -195,15 +206,6 @@ __device__ __forceinline__ int64_t cost_before(const Req& r, int i, int TQ) {
   return last + (int64_t)i * kUnitKeys + (i - z) * a + TQ * (((int64_t)i * (i + 1) - z * (z + 1)) / 2);
 }
 
-// A worker's part of one unit: key tiles [t0, t1) of nt.
-struct Piece {
-  int b, h, tok0, ntok;  // first token row of q, tokens
-  int vis0, L;           // keys that the first token sees (may be negative), keys of the request
-  int t0, t1;
-  int slot;              // -1: the whole unit; 0 / 1: partial that continues / begins it
-  bool last, once;       // the unit's last tiles; its keys are read by this tile alone
-};
-
 // The next piece of the line from w, w < w1, that has something to do.
 template <int KT>
 __device__ __forceinline__ bool next_piece(const Small& sm, const Params& P, int64_t& w, int64_t w1, Piece& p) {
@@ -271,8 +273,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&sm.q_ready), kSoftmax / 32 * CG);
       for (int i = 0; i < kStages; ++i) {
         // a warp's cp.async and an expect_tx; from rank 1 an expect_tx and, once its cp.async are in, an arrival
-        mbar_init(smem_u32(&sm.k_copied[i]), 32);
-        mbar_init(smem_u32(&sm.v_copied[i]), 32);
         mbar_init(smem_u32(&sm.k_full[i]), 32 + 1 + 2 * (CG - 1));
         mbar_init(smem_u32(&sm.k_empty[i]), 1);
         mbar_init(smem_u32(&sm.v_full[i]), 32 + 1 + 2 * (CG - 1));
@@ -287,6 +287,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&sm.o_full), 1);
       mbar_init(smem_u32(&sm.o_free), kSoftmax / 32 * CG);
       mbar_init(smem_u32(&sm.mma_done), 1);
+      for (int i = 0; i < kRing; ++i) {
+        mbar_init(smem_u32(&sm.ring_full[i]), 1);
+        mbar_init(smem_u32(&sm.ring_empty[i]), kSoftmax / 32 + 2 + (rank == 0));  // the warps that take pieces
+      }
       sm.abort = 0;
       for (int i = 0; i < 8; ++i) sm.odd[i] = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -347,31 +351,23 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int64_t total = sm.pre[a.B];
   const int64_t share = max((int64_t)kMinShare, (total + workers - 1) / workers);
   const int64_t w0 = min(total, share * worker), w1 = min(total, w0 + share);
-  int64_t w = w0;
   Piece p;
 
-  // Rank 1 of a pair: its boxes complete on rank 0's barriers by themselves; one
-  // thread for K and one for V (each may run ahead of the other) arrives there
-  // for the stage's cp.async rows once those are in, if there are any.  It does so
-  // for every tile: a stage is not reused before, so its parity keeps its meaning.
-  auto tell = [&](uint64_t* copied, uint64_t* full, int* mixed) {
-    if (lane == 0) {
-      int g = 0;
-      bool ok = true;
-      while (ok && next_piece<KT>(sm, P, w, w1, p)) {
-        const int T = p.t1 - p.t0;
-        for (int gt = g; ok && gt < g + T; ++gt) {
-          const int st = gt % kStages;
-          ok = wait(copied[st], (gt / kStages) & 1, abort_flag);
-          if (!ok) break;
-          if (mixed[st]) fence_async_smem();
-          mbar_arrive_cluster(map_rank(smem_u32(&full[st]), 0));
-        }
-        g += T;
-      }
-      if (!ok && !*abort_flag) set_abort(sm, status);
+  // The pieces are worked out by one warp for all: at each role the search and
+  // its 64-bit arithmetic were 144 KB of kernel, and every unit's change waited
+  // 8 us for instructions.
+  int taken = 0;
+  const auto take = [&](Piece& x) {
+    const int i = taken % kRing;
+    if (!__all_sync(0xffffffffu, wait(sm.ring_full[i], (taken / kRing) & 1, abort_flag))) {
+      x.b = -2;  // a wait gave up
+      return false;
     }
+    x = sm.ring[i];
     __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&sm.ring_empty[i]));
+    ++taken;
+    return x.b >= 0;
   };
   if (warp == kCtlWarp) {
     if (rank == 0) {
@@ -385,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t q_base = k_base + F::OFF_Q;
       int g = 0, ui = 0;
       bool ok = true;
-      while (ok && next_piece<KT>(sm, P, w, w1, p)) {
+      while (ok && take(p)) {
         const int T = p.t1 - p.t0;
         if (T == 0) continue;
         ok = all(wait(sm.q_ready, ui & 1, abort_flag));
@@ -439,16 +435,39 @@ __global__ void __launch_bounds__(kThreads, 1)
         g += T;
         ++ui;
       }
+      ok = ok && p.b != -2;
       if (!ok && lane == 0 && !*abort_flag) set_abort(sm, status);
       // every MMA issued above has retired before TMEM is freed
       commit(sm.mma_done);
-    } else {
-      tell(sm.k_copied, sm.k_full, sm.k_mixed);
     }
     if (lane == 0 && !mbar_wait(smem_u32(&sm.mma_done), 0)) raise_status(status, DFT_DEV_TIMEOUT);
     __syncwarp();
-  } else if (warp == kTellWarp) {
-    if (rank) tell(sm.v_copied, sm.v_full, sm.v_mixed);
+  } else if (warp == kPlanWarp) {
+    // --------------------------------- plan: pieces, and their Q towards L2
+    int64_t w = w0;
+    bool ok = true, more = true;
+    for (int n = 0; ok && more; ++n) {
+      const int i = n % kRing;
+      if (n >= kRing) ok = __all_sync(0xffffffffu, wait(sm.ring_empty[i], (n / kRing - 1) & 1, abort_flag));
+      if (!ok) break;
+      more = next_piece<KT>(sm, P, w, w1, p);
+      if (!more) p.b = -1;
+      if (lane == 0) {
+        sm.ring[i] = p;
+        mbar_arrive(smem_u32(&sm.ring_full[i]));
+      }
+      if (more && p.t1 > p.t0) {
+        for (int r = lane; r < kRows; r += 32) {
+          const int t = (rank * kRows + r) / P.G, hq = rank * kRows + r - t * P.G;
+          if (t >= p.ntok) break;
+          const unsigned char* row = static_cast<const unsigned char*>(a.q) +
+                                     ((int64_t)(p.tok0 + t) * a.q_st + (int64_t)(p.h * P.G + hq) * a.q_sh) * 2;
+#pragma unroll
+          for (int c = 0; c < 2 * D; c += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + c));
+        }
+      }
+    }
+    if (!ok && lane == 0 && !*abort_flag) set_abort(sm, status);
   } else if (warp >= kProdWarp0) {
     // ------------------------------------------- producers: paged K/V tiles
     // A dependent instruction costs a lone warp 4 to 6 cycles, so what a tile
@@ -461,7 +480,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int g0 = V ? 0 : rank * NG, c0 = V ? rank * NC : 0;
       uint64_t* full = V ? sm.v_full : sm.k_full;
       uint64_t* empty = V ? sm.v_empty : sm.k_empty;
-      uint64_t* copied = V ? sm.v_copied : sm.k_copied;
       int* mixed = V ? sm.v_mixed : sm.k_mixed;
       const uint32_t ring = V ? v_base : k_base;
       constexpr uint32_t kStageBytes = V ? F::kVBytes : F::kKBytes;
@@ -471,7 +489,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       int4* slots = sm.slots[V];
       int g = 0;
       bool ok = true;
-      while (ok && next_piece<KT>(sm, P, w, w1, p)) {
+      // Rank 1 arrives on rank 0's barrier for its copied rows once they are in:
+      // behind the next tile's copies, or the piece's end.  (A stage is not waited
+      // for twice before: what frees tile t+1's has seen tile t-1's arrival.)
+      int owed = -1;  // the stage whose arrival is still to come
+      const auto settle = [&](int behind) {
+        if (owed < 0) return;
+        if (behind) asm volatile("cp.async.wait_group 1;" ::: "memory");
+        else cp_async_wait_all();
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(map_rank(smem_u32(&full[owed]), 0));
+        owed = -1;
+      };
+      while (ok && take(p)) {
         const int T = p.t1 - p.t0;
         if (T == 0) continue;
         const int32_t* idx = a.kv_indices + sm.kv[p.b];
@@ -565,10 +596,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             __syncwarp();
           }
-          cp_async_arrive_noinc(rank ? smem_u32(&copied[st]) : smem_u32(&full[st]));
+          if (rank == 0) {
+            cp_async_arrive_noinc(smem_u32(&full[st]));
+          } else {
+            if (copies) asm volatile("cp.async.commit_group;" ::: "memory");
+            settle(copies);
+            if (copies) owed = st;
+            else if (lane == 0) mbar_arrive_cluster(bar);
+          }
         }
         if (ok) g += T;
+        settle(0);
       }
+      ok = ok && p.b != -2;
       if (!ok && lane == 0 && !*abort_flag) set_abort(sm, status);
       // The last copies land before the block's shared memory goes, whatever
       // became of their readers (rank 0's barriers take rank 1's boxes too).
@@ -626,21 +666,29 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       warp_arrive<PAIR>(sm.q_ready);
     };
-    // pieces without keys give zero rows; true when u then holds a piece with some
+    // A row's two warps meet at the same named barriers in the same order; every
+    // early exit is decided from outcomes that both have exchanged there.
+    bool held = true;  // false: a wait gave up since the last exchange
+    bool ok = true;
+    int g = 0, ui = 0, calls = 0;
+    // the next piece with keys; those without give zero rows
     auto next_live = [&](Piece& u) {
-      while (next_piece<KT>(sm, P, w, w1, u)) {
-        if (u.t1 > u.t0) return true;
+      while (take(u) && u.t1 == u.t0) {
         if (tok < u.ntok) {
           uint4* orow = reinterpret_cast<uint4*>(static_cast<unsigned char*>(a.o) +
                                                  ((int64_t)(u.tok0 + tok) * a.o_st + (int64_t)(u.h * P.G + g_) * a.o_sh) * 2 +
                                                  wg * D);
-#pragma unroll 4
+#pragma unroll 1
           for (int q = 0; q < D / 16; ++q) orow[q] = make_uint4(0u, 0u, 0u, 0u);
         }
       }
-      return false;
+      const int par = calls++ & 1;
+      held = held && u.b != -2;
+      if (lane == 0) sm.okt[par][wg][wq] = held;
+      named_bar(pair_bar, 64);
+      ok = held && sm.okt[par][wg ^ 1][wq];
+      return u.b >= 0;
     };
-    int g = 0, ui = 0;
     // this thread's share of a masked tile's V: rows past the end and non-finite values -> 0
     auto clean_v = [&](const Piece& u, int t, int gt) -> bool {
       constexpr uint32_t kExp = BF ? 0x7F807F80u : 0x7C007C00u, kOne = BF ? 0x00800080u : 0x04000400u;
@@ -654,7 +702,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool any = false;
 #pragma unroll 1
       for (int c = 0; c < F::VC; ++c) {
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < KT * 8; i += kSoftmax) {
           const int at = i + tid;  // row at >> 3
           uint4* q = reinterpret_cast<uint4*>(vb + (at >> 7) * (F::VC * 2048) + c * 2048) + (at & 127);
@@ -684,19 +732,91 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_async_smem();  // these writes before the tensor core's reads
       return true;
     };
-    bool more = next_live(p);
-    if (more) load_q(p);
-    bool ok = true;
-    while (ok && more) {
-      const Piece u = p;
+    // Unit after unit: the next one's Q goes in before the last one's output
+    // comes out, so that its S runs meanwhile.
+    bool pending = false;
+    float m_used = -INFINITY, l = 0.f;
+    Piece u;
+    while (ok) {
+      const bool more = next_live(p);  // every S MMA of unit u has been consumed
+      if (!ok) break;
+      if (more) load_q(p);
+      if (pending) {
+        // ---- epilogue of unit u: wait for its last P V, then O (or its partial) out
+        const bool row_ok = tok < u.ntok, busy = rank * kRows + wq * 32 < u.ntok * P.G;
+        const int vis = max(0, min(u.L, u.vis0 + (row_ok ? tok : 0)));
+        const bool got = __all_sync(0xffffffffu, wait(sm.o_full, ui & 1, abort_flag));
+        tc_fence_after();
+        sm.lsum[wg][r] = l;
+        if (lane == 0) sm.oke[wg][wq] = got;
+        named_bar(pair_bar, 64);
+        l = sm.lsum[0][r] + sm.lsum[1][r];
+        ok = got && sm.oke[wg ^ 1][wq];
+        if (ok && busy) {
+          const int64_t prow = (int64_t)(2 * worker + max(u.slot, 0)) * (kRows * CG) + R;
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          unsigned char* orow = static_cast<unsigned char*>(a.o) +
+                                ((int64_t)(u.tok0 + tok) * a.o_st + (int64_t)(u.h * P.G + g_) * a.o_sh) * 2 + wg * D;
+          const bool odd = sm.odd[ui & 7] == ui + 1;
+#pragma unroll 1
+          for (int c = 0; c < D / 64; ++c) {
+            float v[32];
+            tmem_ld32(tmem + lane_base + F::COL_O + (D / 2) * wg + 32 * c, v);
+            if (odd) {
+              // the masked tiles' non-finite values, for the rows that see their keys
+#pragma unroll 1
+              for (int j = max(u.t0 * KT, max(u.vis0, 0) / KT * KT); j < min(u.t1 * KT, vis); ++j) {
+                const int64_t s = a.kv_indices[sm.kv[u.b] + j];
+                if (s < 0 || s >= a.n_slots) continue;
+                const uint16_t* vr = static_cast<const uint16_t*>(a.v_cache) + s * a.kv_st + u.h * a.kv_sh + (D / 2) * wg + 32 * c;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                  const float y = unpack<BF>(vr[i]);
+                  v[i] += fabsf(y) < INFINITY ? 0.f : y;
+                }
+              }
+            }
+            if (!row_ok) continue;
+            if (u.slot < 0) {
+              uint4* dst = reinterpret_cast<uint4*>(orow + c * 64);
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                dst[q] = make_uint4(pack2<BF>(v[8 * q] * inv, v[8 * q + 1] * inv),
+                                    pack2<BF>(v[8 * q + 2] * inv, v[8 * q + 3] * inv),
+                                    pack2<BF>(v[8 * q + 4] * inv, v[8 * q + 5] * inv),
+                                    pack2<BF>(v[8 * q + 6] * inv, v[8 * q + 7] * inv));
+            } else {
+              float4* dst = reinterpret_cast<float4*>(P.ws_o + prow * D + (D / 2) * wg + 32 * c);
+#pragma unroll
+              for (int q = 0; q < 8; ++q) dst[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+            }
+          }
+          if (u.slot >= 0 && wg == 0 && row_ok) {
+            P.ws_ml[2 * prow] = m_used;
+            P.ws_ml[2 * prow + 1] = l;
+          }
+        }
+        if (ok) {
+          if (u.slot >= 0) {
+            slots_used |= 1 << u.slot;
+            if (tid == 0 && rank == 0)
+              P.ws_meta[2 * worker + u.slot] = make_int4(1 | (u.last ? 2 : 0), u.tok0, u.ntok, u.h);
+          }
+          // O may now be overwritten by the next unit's first P V
+          tc_fence_before();
+          warp_arrive<PAIR>(sm.o_free);
+        }
+        ++ui;
+      }
+      if (!ok || !more) break;
+      u = p;
+      pending = true;
       const bool row_ok = tok < u.ntok;
       const int T = u.t1 - u.t0;
       const int vis = max(0, min(u.L, u.vis0 + (row_ok ? tok : 0)));  // keys this row sees: j < vis
       const bool busy = rank * kRows + wq * 32 < u.ntok * P.G;        // the warp holds rows
-      // A row's two warps meet at the same named barriers in the same order;
-      // every early exit is decided from outcomes both have exchanged there.
-      float m_used = -INFINITY, l = 0.f;
-      bool held = true;  // false: the last tile's V never came; told to the other warp at the next barrier
+      m_used = -INFINITY;
+      l = 0.f;
 #pragma unroll 1
       for (int t = 0; t < T; ++t) {
         const int gt = g + t, sb = gt % NB, par = gt & 1;
@@ -704,169 +824,94 @@ __global__ void __launch_bounds__(kThreads, 1)
         // keys that every token of the tile sees need no mask (uniform)
         const int j0 = (u.t0 + t) * KT;
         const bool plain = j0 + KT <= u.vis0 && j0 + KT <= u.L;
-        if (!busy) {  // spare rows: whatever P holds stays in them
-          ok = got && (plain || clean_v(u, t, gt));
+        if (busy) {  // else spare rows: whatever P holds stays in them
+          const uint32_t ts = tmem + lane_base + F::COL_S + KT * sb;
+          float x[64];
+          tc_fence_after();
+          tmem_ld32_async(ts + 64 * wg, &x[0]);
+          tmem_ld32_async(ts + 64 * wg + 32, &x[32]);
+          tmem_ld_wait(x);
+          if (!plain) {
+            const int c0 = vis - j0 - 64 * wg;  // columns of this half that the row sees
+#pragma unroll
+            for (int i = 0; i < 64; ++i)
+              if (i >= c0) x[i] = -INFINITY;
+          }
+          float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < 64; i += 4) {
+            mx[0] = fmaxf(fmaxf(mx[0], x[i]), x[i + 1]);
+            mx[1] = fmaxf(fmaxf(mx[1], x[i + 2]), x[i + 3]);
+          }
+          // x stays raw: P = 2^(x sc - m)
+          float tmax = fmaxf(mx[0], mx[1]) * sc;
+          sm.xmax[par][wg][r] = tmax;
+          if (lane == 0) sm.okx[par][wg][wq] = got;
+          // the barrier also orders this half's S reads before the other half's P
+          // stores (half 1 writes P over S columns that half 0 reads)
+          tc_fence_before();
+          named_bar(pair_bar, 64);
+          tc_fence_after();
+          tmax = fmaxf(tmax, sm.xmax[par][wg ^ 1][r]);
+          ok = got && sm.okx[par][wg ^ 1][wq];
           if (!ok) break;
-          warp_arrive<PAIR>(sm.p_full[sb]);
-          continue;
-        }
-        const uint32_t ts = tmem + lane_base + F::COL_S + KT * sb;
-        float x[64];
-        tc_fence_after();
-        tmem_ld32_async(ts + 64 * wg, &x[0]);
-        tmem_ld32_async(ts + 64 * wg + 32, &x[32]);
-        tmem_ld_wait(x);
-        if (!plain) {
-          const int c0 = vis - j0 - 64 * wg;  // columns of this half that the row sees
-#pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (i >= c0) x[i] = -INFINITY;
-        }
-        float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int i = 0; i < 64; i += 4) {
-          mx[0] = fmaxf(fmaxf(mx[0], x[i]), x[i + 1]);
-          mx[1] = fmaxf(fmaxf(mx[1], x[i + 2]), x[i + 3]);
-        }
-        // x stays raw: P = 2^(x sc - m)
-        float tmax = fmaxf(mx[0], mx[1]) * sc;
-        sm.xmax[par][wg][r] = tmax;
-        if (lane == 0) sm.okx[par][wg][wq] = got;
-        // the barrier also orders this half's S reads before the other half's P
-        // stores (half 1 writes P over S columns that half 0 reads)
-        tc_fence_before();
-        named_bar(pair_bar, 64);
-        tc_fence_after();
-        tmax = fmaxf(tmax, sm.xmax[par][wg ^ 1][r]);
-        ok = got && sm.okx[par][wg ^ 1][wq];
-        if (!ok) break;
-        // a row moves its reference only when the tile's maximum exceeds it by
-        // more than 8 (P <= 2^8 otherwise); O then scales by 2^(old - new)
-        const bool grow = tmax > m_used + 8.f;
-        if (__any_sync(0xffffffffu, grow)) {
-          const float m_new = grow ? tmax : m_used;
-          if (t > 0) {
-            // O holds P V of this unit's earlier tiles: wait for the last, then rescale this half row
-            const bool done = __all_sync(0xffffffffu, wait(sm.pv_done[(gt - 1) % NB], ((gt - 1) / NB) & 1, abort_flag));
-            if (lane == 0) sm.okr[par][wg][wq] = done;
-            named_bar(pair_bar, 64);
-            ok = done && sm.okr[par][wg ^ 1][wq];
-            if (!ok) break;
-            tc_fence_after();
-            const float alpha = grow ? ex2(m_used - m_new) : 1.f;
+          // a row moves its reference only when the tile's maximum exceeds it by
+          // more than 8 (P <= 2^8 otherwise); O then scales by 2^(old - new)
+          const bool grow = tmax > m_used + 8.f;
+          if (__any_sync(0xffffffffu, grow)) {
+            const float m_new = grow ? tmax : m_used;
+            if (t > 0) {
+              // O holds P V of this unit's earlier tiles: wait for the last, then rescale this half row
+              const bool done = __all_sync(0xffffffffu, wait(sm.pv_done[(gt - 1) % NB], ((gt - 1) / NB) & 1, abort_flag));
+              if (lane == 0) sm.okr[par][wg][wq] = done;
+              named_bar(pair_bar, 64);
+              ok = done && sm.okr[par][wg ^ 1][wq];
+              if (!ok) break;
+              tc_fence_after();
+              const float alpha = grow ? ex2(m_used - m_new) : 1.f;
 #pragma unroll 1
-            for (int c = 0; c < D / 2; c += 32) {
-              float v[32];
-              tmem_ld32(tmem + lane_base + F::COL_O + (D / 2) * wg + c, v);
+              for (int c = 0; c < D / 2; c += 32) {
+                float v[32];
+                tmem_ld32(tmem + lane_base + F::COL_O + (D / 2) * wg + c, v);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] *= alpha;
-              tmem_st32(tmem + lane_base + F::COL_O + (D / 2) * wg + c, v);
+                for (int i = 0; i < 32; ++i) v[i] *= alpha;
+                tmem_st32(tmem + lane_base + F::COL_O + (D / 2) * wg + c, v);
+              }
+              l *= alpha;
             }
-            l *= alpha;
+            m_used = m_new;
           }
-          m_used = m_new;
-        }
-        // a row whose scores so far are all -inf has no reference yet: its P is 0
-        const float nm = (m_used == -INFINITY && !plain) ? 0.f : kBias - m_used;
-        const f32x2 sc2 = pk2(sc, sc), nm2 = pk2(nm, nm);
-        f32x2 sum2[2] = {pk2(0.f, 0.f), pk2(0.f, 0.f)};
+          // a row whose scores so far are all -inf has no reference yet: its P is 0
+          const float nm = (m_used == -INFINITY && !plain) ? 0.f : kBias - m_used;
+          const f32x2 sc2 = pk2(sc, sc), nm2 = pk2(nm, nm);
+          f32x2 sum2[2] = {pk2(0.f, 0.f), pk2(0.f, 0.f)};
 #pragma unroll
-        for (int c = 0; c < 64; c += 32) {
-          uint32_t pk[16];
+          for (int c = 0; c < 64; c += 32) {
+            uint32_t pk[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float e0, e1;
-            upk2(fma2(pk2(x[c + 2 * i], x[c + 2 * i + 1]), sc2, nm2), e0, e1);
-            const float p0 = ex2(e0), p1 = ex2(e1);
-            sum2[i & 1] = add2(sum2[i & 1], pk2(p0, p1));
-            pk[i] = pack2<BF>(p0, p1);
+            for (int i = 0; i < 16; ++i) {
+              float e0, e1;
+              upk2(fma2(pk2(x[c + 2 * i], x[c + 2 * i + 1]), sc2, nm2), e0, e1);
+              const float p0 = ex2(e0), p1 = ex2(e1);
+              sum2[i & 1] = add2(sum2[i & 1], pk2(p0, p1));
+              pk[i] = pack2<BF>(p0, p1);
+            }
+            tmem_st16_async(ts + 32 * wg + c / 2, pk);
           }
-          tmem_st16_async(ts + 32 * wg + c / 2, pk);
+          float s0, s1;
+          upk2(add2(sum2[0], sum2[1]), s0, s1);
+          l += s0 + s1;
+          tmem_st_wait();
         }
-        float s0, s1;
-        upk2(add2(sum2[0], sum2[1]), s0, s1);
-        l += s0 + s1;
-        held = plain || clean_v(u, t, gt);
-        tmem_st_wait();
+        held = got && (plain || clean_v(u, t, gt));
         tc_fence_before();
         if (held) warp_arrive<PAIR>(sm.p_full[sb]);
+        else if (!busy) break;
       }
       if (!ok) break;
       g += T;
-      // every S MMA of this unit has been consumed: the next unit's Q may go in
-      more = next_live(p);
-      if (more) load_q(p);
-      // ---- epilogue: wait for this unit's last P V, then O (or its partial) out
-      const bool got = __all_sync(0xffffffffu, held && wait(sm.o_full, ui & 1, abort_flag));
-      tc_fence_after();
-      if (busy) {
-        sm.lsum[wg][r] = l;
-        if (lane == 0) sm.oke[wg][wq] = got;
-        named_bar(pair_bar, 64);
-        l = sm.lsum[0][r] + sm.lsum[1][r];
-        ok = got && sm.oke[wg ^ 1][wq];
-      } else {
-        ok = got;
-      }
-      if (ok && busy) {
-        const int64_t prow = (int64_t)(2 * worker + max(u.slot, 0)) * (kRows * CG) + R;
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        unsigned char* orow = static_cast<unsigned char*>(a.o) +
-                              ((int64_t)(u.tok0 + tok) * a.o_st + (int64_t)(u.h * P.G + g_) * a.o_sh) * 2 + wg * D;
-        const bool odd = sm.odd[ui & 7] == ui + 1;
-#pragma unroll 1
-        for (int c = 0; c < D / 64; ++c) {
-          float v[32];
-          tmem_ld32(tmem + lane_base + F::COL_O + (D / 2) * wg + 32 * c, v);
-          if (odd) {
-            // the masked tiles' non-finite values, for the rows that see their keys
-            for (int j = max(0, min(u.vis0, u.t1 * KT) / KT * KT); j < min(u.t1 * KT, vis); ++j) {
-              if (j < u.t0 * KT) continue;
-              const int64_t s = a.kv_indices[sm.kv[u.b] + j];
-              if (s < 0 || s >= a.n_slots) continue;
-              const uint16_t* vr = static_cast<const uint16_t*>(a.v_cache) + s * a.kv_st + u.h * a.kv_sh + (D / 2) * wg + 32 * c;
-              for (int i = 0; i < 32; ++i) {
-                const float y = unpack<BF>(vr[i]);
-                if (!(fabsf(y) < INFINITY)) {
-#pragma unroll
-                  for (int e = 0; e < 32; ++e)
-                    if (e == i) v[e] += y;
-                }
-              }
-            }
-          }
-          if (!row_ok) continue;
-          if (u.slot < 0) {
-            uint4* dst = reinterpret_cast<uint4*>(orow + c * 64);
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              dst[q] = make_uint4(pack2<BF>(v[8 * q] * inv, v[8 * q + 1] * inv),
-                                  pack2<BF>(v[8 * q + 2] * inv, v[8 * q + 3] * inv),
-                                  pack2<BF>(v[8 * q + 4] * inv, v[8 * q + 5] * inv),
-                                  pack2<BF>(v[8 * q + 6] * inv, v[8 * q + 7] * inv));
-          } else {
-            float4* dst = reinterpret_cast<float4*>(P.ws_o + prow * D + (D / 2) * wg + 32 * c);
-#pragma unroll
-            for (int q = 0; q < 8; ++q) dst[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-          }
-        }
-        if (u.slot >= 0 && wg == 0 && row_ok) {
-          P.ws_ml[2 * prow] = m_used;
-          P.ws_ml[2 * prow + 1] = l;
-        }
-      }
-      if (ok) {
-        if (u.slot >= 0) {
-          slots_used |= 1 << u.slot;
-          if (tid == 0 && rank == 0)
-            P.ws_meta[2 * worker + u.slot] = make_int4(1 | (u.last ? 2 : 0), u.tok0, u.ntok, u.h);
-        }
-        // O may now be overwritten by the next unit's first P V
-        tc_fence_before();
-        warp_arrive<PAIR>(sm.o_free);
-      }
-      ++ui;
     }
+    ok = ok && p.b != -2;
     if (tid == 0 && rank == 0)
       for (int s = 0; s < 2; ++s)
         if (!(slots_used >> s & 1)) P.ws_meta[2 * worker + s] = make_int4(0, 0, 0, 0);
