@@ -62,7 +62,7 @@ constexpr int kSoftmax = 256;     // two threads per query row, in warps w and w
 constexpr int kCtlWarp = 8, kProdWarp0 = 9, kPlanWarp = 11;  // a producer warp for K, one for V
 constexpr int kThreads = 384;     // twelve warps leave 168 registers a thread
 constexpr uint32_t kTmemCols = 512;
-constexpr int kMaxStages = 12, kRing = 4;
+constexpr int kMaxStages = 4, kRing = 4;
 // A unit's fixed cost in keys (query load, first tile's latency, output), and
 // the least share of a worker: under it a cut costs more than it spreads.
 constexpr int kUnitKeys = 256;
@@ -80,20 +80,21 @@ struct Cfg {
   static constexpr int CG = kPair ? 2 : 1;                    // CTAs of a worker
   static constexpr int KT = DFT_KT(D);                        // keys per tile
   static constexpr int NB = KT == 64 ? 4 : 2;                 // S / P buffers
-  static constexpr int kStages = (D == 64 ? 6 : kPair ? 2 : 3) * (128 / KT);
+  static constexpr int KS = kPair ? 2 : D == 128 ? 3 : 4, VS = D == 64 ? 4 : 2;  // stages of K and of V
   static constexpr int KR = KT / CG, KC = D / 64;             // K rows and 64-dim chunks in this CTA
   static constexpr int VC = D / 64 / CG;                      // V chunks in this CTA (all KT rows)
   static constexpr uint32_t kKBytes = KR * KC * 128, kVBytes = KT * VC * 128;
-  static constexpr uint32_t kQBytes = kPair ? kRows * D * 2 : 0;
-  static constexpr uint32_t OFF_V = kStages * kKBytes, OFF_Q = OFF_V + kStages * kVBytes;
+  static constexpr uint32_t kQBytes = kRows * D * 2;
+  static constexpr uint32_t OFF_V = KS * kKBytes, OFF_Q = OFF_V + VS * kVBytes;
   static constexpr uint32_t OFF_SMALL = OFF_Q + kQBytes;
-  static constexpr uint32_t COL_O = 0, COL_Q = D, COL_S = kPair ? D : D + D / 2;  // S / P buffer b at COL_S + KT b
+  static constexpr uint32_t COL_O = 0, COL_S = D;  // S / P buffer b at COL_S + KT b
   static_assert(COL_S + NB * KT <= kTmemCols, "TMEM");
 };
 
 // A worker's part of one unit: key tiles [t0, t1) of nt.  b < 0: there are no more.
 struct Piece {
   int b, h, tok0, ntok;  // first token row of q, tokens
+  int k0;                // its request's first entry in kv_indices
   int vis0, L;           // keys that the first token sees (may be negative), keys of the request
   int t0, t1;
   int slot;              // -1: the whole unit; 0 / 1: partial that continues / begins it
@@ -103,6 +104,7 @@ struct Piece {
 struct Small {
   uint64_t q_ready;
   uint64_t k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages];
+  uint64_t k_copied[kMaxStages], v_copied[kMaxStages];  // rank 1 of a pair: its cp.async rows of the stage
   uint64_t s_full[4], p_full[4], pv_done[4];
   uint64_t v_here[4];       // rank 1 of a pair: [S buffer] the tile's V is in (its boxes complete on rank 0)
   uint64_t o_full, o_free, mma_done;
@@ -116,7 +118,6 @@ struct Small {
   int okr[2][2][4];         // the same for the rescale's wait
   int oke[2][4];            // [half][row warp] the epilogue's wait
   int okt[2][2][4];         // [unit parity][half][row warp] whether the warp goes on to the next unit
-  int64_t warp_sum[kThreads / 32];
   int64_t pre[kMaxB + 1];   // cost of the requests before b
   int qo[kMaxB + 1], kv[kMaxB + 1];
   Piece ring[kRing];           // the worker's pieces as they come, from the plan warp
@@ -127,6 +128,7 @@ struct Small {
 struct Params {
   dft_chunk_attn_args a;
   int G, TQ;                // q-heads per kv-head, tokens per query tile
+  uint32_t inv_G;           // ceil(2^16 / G): row / G = row * inv_G >> 16 for rows below 256 and G up to 128
   float* ws_o;              // [2 workers][rows][D] partial O: slot 2c continues a unit, 2c + 1 begins one
   float* ws_ml;             // [2 workers][rows][2] partial (m, l)
   int4* ws_meta;            // [2 workers] (flags, first token row, tokens, kv-head); flags 1: used, 2: the unit's last
@@ -206,6 +208,44 @@ __device__ __forceinline__ int64_t cost_before(const Req& r, int i, int TQ) {
   return last + (int64_t)i * kUnitKeys + (i - z) * a + TQ * (((int64_t)i * (i + 1) - z * (z + 1)) / 2);
 }
 
+// The line: offsets to shared memory, and the cost of the requests before each
+// (by one warp; lane i sums a run of requests).  Returns the line's length.
+__device__ __forceinline__ int64_t plan_costs(Small& sm, const Params& P, int32_t* status) {
+  const dft_chunk_attn_args& a = P.a;
+  const int lane = threadIdx.x & 31, per = (a.B + 31) / 32;
+  for (int i = lane; i <= a.B; i += 32) {
+    sm.qo[i] = a.qo_indptr[i];
+    sm.kv[i] = a.kv_indptr[i];
+  }
+  __syncwarp();
+  int64_t sum = 0;
+  bool bad = false;
+#pragma unroll 1
+  for (int b = lane * per; b < min(a.B, (lane + 1) * per); ++b) {
+    const int q0 = sm.qo[b], q1 = sm.qo[b + 1], k0 = sm.kv[b], k1 = sm.kv[b + 1];
+    const bool ok = q0 >= 0 && q0 <= q1 && q1 <= a.T && k0 >= 0 && k0 <= k1 && k1 <= a.n_kv && k1 - k0 <= 0x7FFFFF00;
+    bad |= !ok;
+    sm.pre[b] = sum;  // so far from the lane's first
+    if (ok && q1 > q0) {
+      const Req r = request(sm, b, P.TQ);
+      sum += a.Hkv * cost_before(r, r.nt, P.TQ);
+    }
+  }
+  if (bad && blockIdx.x == 0) raise_status(status, DFT_DEV_BAD_INDEX);
+  int64_t inc = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t o = __shfl_up_sync(0xffffffffu, inc, d);
+    if (lane >= d) inc += o;
+  }
+#pragma unroll 1
+  for (int b = lane * per; b < min(a.B, (lane + 1) * per); ++b) sm.pre[b] += inc - sum;
+  const int64_t total = __shfl_sync(0xffffffffu, inc, 31);
+  if (lane == 0) sm.pre[a.B] = total;
+  __syncwarp();
+  return total;
+}
+
 // The next piece of the line from w, w < w1, that has something to do.
 template <int KT>
 __device__ __forceinline__ bool next_piece(const Small& sm, const Params& P, int64_t& w, int64_t w1, Piece& p) {
@@ -239,6 +279,7 @@ __device__ __forceinline__ bool next_piece(const Small& sm, const Params& P, int
     p.h = h;
     p.tok0 = sm.qo[lo] + i * P.TQ;
     p.ntok = min(P.TQ, r.n - i * P.TQ);
+    p.k0 = sm.kv[lo];
     p.vis0 = r.L - r.n + i * P.TQ + 1;
     p.L = r.L;
     p.last = p.t1 == nt;
@@ -255,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                       const __grid_constant__ Params P, int32_t* status) {
   using F = Cfg<D>;
   constexpr bool PAIR = F::kPair;
-  constexpr int KT = F::KT, NB = F::NB, kAhead = NB - 1, kStages = F::kStages, CG = F::CG;
+  constexpr int KT = F::KT, NB = F::NB, kAhead = NB - 1, CG = F::CG;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   Small& sm = *reinterpret_cast<Small*>(smem + F::OFF_SMALL);
@@ -271,8 +312,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kCtlWarp) {
     if (lane == 0) {
       mbar_init(smem_u32(&sm.q_ready), kSoftmax / 32 * CG);
-      for (int i = 0; i < kStages; ++i) {
+      for (int i = 0; i < kMaxStages; ++i) {
         // a warp's cp.async and an expect_tx; from rank 1 an expect_tx and, once its cp.async are in, an arrival
+        mbar_init(smem_u32(&sm.k_copied[i]), 32);
+        mbar_init(smem_u32(&sm.v_copied[i]), 32);
         mbar_init(smem_u32(&sm.k_full[i]), 32 + 1 + 2 * (CG - 1));
         mbar_init(smem_u32(&sm.k_empty[i]), 1);
         mbar_init(smem_u32(&sm.v_full[i]), 32 + 1 + 2 * (CG - 1));
@@ -289,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&sm.mma_done), 1);
       for (int i = 0; i < kRing; ++i) {
         mbar_init(smem_u32(&sm.ring_full[i]), 1);
-        mbar_init(smem_u32(&sm.ring_empty[i]), kSoftmax / 32 + 2 + (rank == 0));  // the warps that take pieces
+        mbar_init(smem_u32(&sm.ring_empty[i]), kSoftmax / 32 + 3);  // the warps that take pieces
       }
       sm.abort = 0;
       for (int i = 0; i < 8; ++i) sm.odd[i] = 0;
@@ -299,58 +342,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (PAIR) tmem_alloc_2(smem_u32(&sm.tmem_base), kTmemCols);
     else tmem_alloc(smem_u32(&sm.tmem_base), kTmemCols);
   }
-  // offsets and the requests' costs: thread t sums requests [t per, ...)
-  {
-    constexpr int kPer = (kMaxB + kThreads - 1) / kThreads;
-    for (int i = tid; i <= a.B; i += kThreads) {
-      sm.qo[i] = a.qo_indptr[i];
-      sm.kv[i] = a.kv_indptr[i];
-    }
-    __syncthreads();
-    int64_t c[kPer], sum = 0;
-    bool bad = false;
-#pragma unroll
-    for (int q = 0; q < kPer; ++q) {
-      const int b = tid * kPer + q;
-      c[q] = 0;
-      if (b < a.B) {
-        const int q0 = sm.qo[b], q1 = sm.qo[b + 1], k0 = sm.kv[b], k1 = sm.kv[b + 1];
-        const bool ok = q0 >= 0 && q0 <= q1 && q1 <= a.T && k0 >= 0 && k0 <= k1 && k1 <= a.n_kv &&
-                        k1 - k0 <= 0x7FFFFF00;
-        bad |= !ok;
-        if (ok && q1 > q0) {
-          const Req r = request(sm, b, P.TQ);
-          c[q] = a.Hkv * cost_before(r, r.nt, P.TQ);
-        }
-      }
-      sum += c[q];
-    }
-    if (bad && blockIdx.x == 0) raise_status(status, DFT_DEV_BAD_INDEX);
-    int64_t inc = sum;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int64_t o = __shfl_up_sync(0xffffffffu, inc, d);
-      if (lane >= d) inc += o;
-    }
-    if (lane == 31) sm.warp_sum[warp] = inc;
-    __syncthreads();
-    int64_t at = inc - sum;
-    for (int i = 0; i < warp; ++i) at += sm.warp_sum[i];
-#pragma unroll
-    for (int q = 0; q < kPer; ++q) {
-      const int b = tid * kPer + q;
-      if (b <= a.B) sm.pre[b] = at;
-      at += c[q];
-    }
-  }
   tc_fence_before();
   __syncthreads();
-  if (PAIR) cluster_sync();  // the other CTA's barriers are up before anything arrives on them
+  if (PAIR) cluster_arrive();  // this CTA's barriers are up
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // inputs and workspace are the launches before's until here
+  const int64_t total = warp == kPlanWarp ? plan_costs(sm, P, status) : 0;
+  if (PAIR) cluster_wait();    // the other CTA's are too, before anything arrives on them
   tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
-  const int64_t total = sm.pre[a.B];
-  const int64_t share = max((int64_t)kMinShare, (total + workers - 1) / workers);
-  const int64_t w0 = min(total, share * worker), w1 = min(total, w0 + share);
   Piece p;
 
   // The pieces are worked out by one warp for all: at each role the search and
@@ -387,8 +386,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = all(wait(sm.q_ready, ui & 1, abort_flag));
         for (int t = 0; ok && t < T + kAhead; ++t) {
           if (t < T) {
-            const int gt = g + t, st = gt % kStages, sb = gt % NB;
-            bool got = wait(sm.k_full[st], (gt / kStages) & 1, abort_flag);
+            const int gt = g + t, st = gt % F::KS, sb = gt % NB;
+            bool got = wait(sm.k_full[st], (gt / F::KS) & 1, abort_flag);
             if (got && gt >= NB) got = wait(sm.pv_done[sb], (gt / NB - 1) & 1, abort_flag);  // P of tile gt - NB is read
             ok = all(got);
             if (!ok) break;
@@ -396,21 +395,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (sm.k_mixed[st]) fence_async_smem();  // cp.async (generic proxy) writes -> tensor-core reads
             const uint32_t kb = __shfl_sync(0xffffffffu, k_base + st * F::kKBytes, 0);
             const uint32_t ds = __shfl_sync(0xffffffffu, tmem + F::COL_S + KT * sb, 0);
+            // K: 8-key groups KC KB apart, a group's 64-dim chunks 1 KB apart
+            const uint64_t ad = sw128_desc(q_base), bd = sw128_desc(kb, 16, F::KC * 1024);
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              // 8-key groups KC KB apart, a group's 64-dim chunks 1 KB apart
-              const uint64_t bd = sw128_desc(kb + (k >> 2) * 1024 + (k & 3) * 32, 16, F::KC * 1024);
-              if (PAIR)
-                mma_ss<CG>(lead, ds, sw128_desc(q_base + (k >> 2) * (kRows * 128) + (k & 3) * 32), bd, id_s, k > 0);
-              else
-                mma_ts<CG>(lead, ds, tmem + F::COL_Q + 8 * k, bd, id_s, k > 0);
-            }
+            for (int k = 0; k < D / 16; ++k)
+              mma_ss<CG>(lead, ds, ad + ((k >> 2) * (kRows * 128) + (k & 3) * 32) / 16,
+                         bd + ((k >> 2) * 1024 + (k & 3) * 32) / 16, id_s, k > 0);
             commit(sm.k_empty[st]);
             commit(sm.s_full[sb]);
           }
           if (t >= kAhead) {
-            const int gu = g + t - kAhead, st = gu % kStages, pb = gu % NB;
-            bool got = wait(sm.v_full[st], (gu / kStages) & 1, abort_flag);
+            const int gu = g + t - kAhead, st = gu % F::VS, pb = gu % NB;
+            bool got = wait(sm.v_full[st], (gu / F::VS) & 1, abort_flag);
             if (PAIR && got && lead) mbar_arrive_cluster(map_rank(smem_u32(&sm.v_here[pb]), 1));
             // the first P V of a unit overwrites O: the previous unit's epilogue has read it
             if (got && t == kAhead && ui > 0) got = wait(sm.o_free, (ui - 1) & 1, abort_flag);
@@ -421,12 +417,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t vb = __shfl_sync(0xffffffffu, v_base + st * F::kVBytes, 0);
             const uint32_t ps = __shfl_sync(0xffffffffu, tmem + F::COL_S + KT * pb, 0);
             const uint32_t keep = __shfl_sync(0xffffffffu, t > kAhead ? 1u : 0u, 0);
+            // V [keys x dims] is MN-major: of 16 keys, 64-dim chunks 2 KB apart, 8-key groups 1 KB apart
+            const uint64_t bd = sw128_desc(vb, 2048, 1024);
 #pragma unroll
-            for (int k = 0; k < KT / 16; ++k) {
-              // V [keys x dims] is MN-major: of 16 keys, 64-dim chunks 2 KB apart, 8-key groups 1 KB apart
-              const uint64_t bd = sw128_desc(vb + k * F::VC * 2048, 2048, 1024);
-              mma_ts<CG>(lead, tmem + F::COL_O, ps + 8 * k, bd, id_o, k > 0 ? 1u : keep);
-            }
+            for (int k = 0; k < KT / 16; ++k)
+              mma_ts<CG>(lead, tmem + F::COL_O, ps + 8 * k, bd + k * F::VC * 2048 / 16, id_o, k > 0 ? 1u : keep);
             commit(sm.v_empty[st]);
             commit(sm.pv_done[pb]);
             if (t == T + kAhead - 1) commit(sm.o_full);
@@ -439,12 +434,42 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok && lane == 0 && !*abort_flag) set_abort(sm, status);
       // every MMA issued above has retired before TMEM is freed
       commit(sm.mma_done);
+    } else {
+      // Rank 1 of a pair: its boxes complete on rank 0's barriers by themselves.
+      // For the cp.async rows of each stage (none, maybe) this warp arrives there
+      // once they are in.  K and V run apart, so it waits for neither alone; it
+      // arrives for every tile, so a stage is not reused before and its parity
+      // keeps its meaning.
+      int end = 0, next[2] = {0, 0};  // tiles known of, and the next of K and of V
+      bool ok = true, more = true;
+      long long t0 = clock64();
+      while (ok && (more || next[0] < end || next[1] < end)) {
+        if (more && max(next[0], next[1]) == end) {
+          more = take(p);
+          ok = p.b != -2;
+          if (more) end += p.t1 - p.t0;
+        }
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          const int n = v ? F::VS : F::KS, st = next[v] % n;
+          if (next[v] >= end || !__all_sync(0xffffffffu, mbar_test(smem_u32(v ? &sm.v_copied[st] : &sm.k_copied[st]),
+                                                                  (next[v] / n) & 1)))
+            continue;
+          if ((v ? sm.v_mixed : sm.k_mixed)[st]) fence_async_smem();
+          if (lane == 0) mbar_arrive_cluster(map_rank(smem_u32(v ? &sm.v_full[st] : &sm.k_full[st]), 0));
+          ++next[v];
+          t0 = clock64();
+        }
+        ok = ok && __all_sync(0xffffffffu, !*abort_flag && clock64() - t0 < 2000000000ll);
+      }
+      if (!ok && lane == 0 && !*abort_flag) set_abort(sm, status);
     }
     if (lane == 0 && !mbar_wait(smem_u32(&sm.mma_done), 0)) raise_status(status, DFT_DEV_TIMEOUT);
     __syncwarp();
   } else if (warp == kPlanWarp) {
     // --------------------------------- plan: pieces, and their Q towards L2
-    int64_t w = w0;
+    const int64_t share = max((int64_t)kMinShare, (total + workers - 1) / workers), w1 = min(total, share * (worker + 1));
+    int64_t w = min(total, share * worker);
     bool ok = true, more = true;
     for (int n = 0; ok && more; ++n) {
       const int i = n % kRing;
@@ -458,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (more && p.t1 > p.t0) {
         for (int r = lane; r < kRows; r += 32) {
-          const int t = (rank * kRows + r) / P.G, hq = rank * kRows + r - t * P.G;
+          const int t = (int)((rank * kRows + r) * P.inv_G >> 16), hq = rank * kRows + r - t * P.G;
           if (t >= p.ntok) break;
           const unsigned char* row = static_cast<const unsigned char*>(a.q) +
                                      ((int64_t)(p.tok0 + t) * a.q_st + (int64_t)(p.h * P.G + hq) * a.q_sh) * 2;
@@ -476,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto produce = [&](auto v_) {
       constexpr bool V = decltype(v_)::value;
       // K: this CTA's rows, all chunks; V: all rows, this CTA's chunks
-      constexpr int NG = V ? KT / 16 : F::KR / 16, NC = V ? F::VC : F::KC;
+      constexpr int NG = V ? KT / 16 : F::KR / 16, NC = V ? F::VC : F::KC, kStages = V ? F::VS : F::KS;
       const int g0 = V ? 0 : rank * NG, c0 = V ? rank * NC : 0;
       uint64_t* full = V ? sm.v_full : sm.k_full;
       uint64_t* empty = V ? sm.v_empty : sm.k_empty;
@@ -489,23 +514,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       int4* slots = sm.slots[V];
       int g = 0;
       bool ok = true;
-      // Rank 1 arrives on rank 0's barrier for its copied rows once they are in:
-      // behind the next tile's copies, or the piece's end.  (A stage is not waited
-      // for twice before: what frees tile t+1's has seen tile t-1's arrival.)
-      int owed = -1;  // the stage whose arrival is still to come
-      const auto settle = [&](int behind) {
-        if (owed < 0) return;
-        if (behind) asm volatile("cp.async.wait_group 1;" ::: "memory");
-        else cp_async_wait_all();
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(map_rank(smem_u32(&full[owed]), 0));
-        owed = -1;
-      };
       while (ok && take(p)) {
         const int T = p.t1 - p.t0;
         if (T == 0) continue;
-        const int32_t* idx = a.kv_indices + sm.kv[p.b];
+        const int32_t* idx = a.kv_indices + p.k0;
         const uint64_t pol = p.once ? pol_first : pol_keep;
         int s[4];  // slots of keys 4 lane + q of a tile; past the request's end, of its last
         auto fetch = [&](int tile) {
@@ -596,17 +608,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             __syncwarp();
           }
-          if (rank == 0) {
-            cp_async_arrive_noinc(smem_u32(&full[st]));
-          } else {
-            if (copies) asm volatile("cp.async.commit_group;" ::: "memory");
-            settle(copies);
-            if (copies) owed = st;
-            else if (lane == 0) mbar_arrive_cluster(bar);
-          }
+          cp_async_arrive_noinc(smem_u32(rank ? (V ? &sm.v_copied[st] : &sm.k_copied[st]) : &full[st]));
         }
         if (ok) g += T;
-        settle(0);
       }
       ok = ok && p.b != -2;
       if (!ok && lane == 0 && !*abort_flag) set_abort(sm, status);
@@ -626,44 +630,35 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int wg = warp >> 2;               // half of S's, O's and Q's columns
     const int pair_bar = 1 + (warp & 3);    // named barrier of warps w and w + 4 (same rows)
     const int wq = warp & 3;
-    const int tok = R / P.G, g_ = R - tok * P.G;
+    const int tok = (int)(R * P.inv_G >> 16), g_ = R - tok * P.G;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const float sc = a.sm_scale * 1.4426950408889634f;
     // a partial slot that no piece of this CTA fills is marked so
     int slots_used = 0;
-    // Q row half of a piece -> TMEM (packed, D / 4 columns), or shared memory (128B-swizzled); spare rows are zero
+    // A piece's Q -> shared memory (128B-swizzled, 64-dim chunks kRows rows apart):
+    // 16 rows a warp, whole rows in a load (a row per lane took 6000 cycles, a line
+    // looked up for every 16 bytes); spare rows are zero.
     auto load_q = [&](const Piece& u) {
-      const bool row_ok = tok < u.ntok;
-      const uint4* qrow = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(a.q) +
-                                                         ((int64_t)(u.tok0 + (row_ok ? tok : 0)) * a.q_st +
-                                                          (int64_t)(u.h * P.G + (row_ok ? g_ : 0)) * a.q_sh) * 2 +
-                                                         wg * D);
-      if (PAIR) {
-        uint4 x[D / 16];
-#pragma unroll
-        for (int q = 0; q < D / 16; ++q) x[q] = row_ok ? __ldg(qrow + q) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-        for (int q = 0; q < D / 16; ++q) {
-          const int col = wg * (D / 16) + q;  // 16-byte piece of the row
-          *reinterpret_cast<uint4*>(smem + F::OFF_Q + (col >> 3) * (kRows * 128) + r * 128 + (((col ^ r) & 7) << 4)) = x[q];
-        }
-        fence_async_smem();
-      } else {
+      constexpr int kLanes = D / 8, kPass = 32 / kLanes, kTurns = 16 / kPass;  // lanes a row, rows a pass, passes
+      const int col = lane % kLanes;
+      constexpr int kBatch = kTurns < 4 ? kTurns : 4;
 #pragma unroll 1
-        for (int c = 0; c < D / 4; c += 16) {
-          uint32_t v[16];
+      for (int i0 = 0; i0 < kTurns; i0 += kBatch) {
+        uint4 x[kBatch];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint4 x = row_ok ? __ldg(qrow + c / 4 + q) : make_uint4(0u, 0u, 0u, 0u);
-            v[4 * q] = x.x;
-            v[4 * q + 1] = x.y;
-            v[4 * q + 2] = x.z;
-            v[4 * q + 3] = x.w;
-          }
-          tmem_st16(tmem + lane_base + F::COL_Q + (D / 4) * wg + c, v);
+        for (int i = 0; i < kBatch; ++i) {
+          const int row = rank * kRows + warp * 16 + (i0 + i) * kPass + lane / kLanes, t = (int)(row * P.inv_G >> 16);
+          const unsigned char* from = static_cast<const unsigned char*>(a.q) + 16 * col +
+                                      ((int64_t)(u.tok0 + t) * a.q_st + (int64_t)(u.h * P.G + row - t * P.G) * a.q_sh) * 2;
+          x[i] = t < u.ntok ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0u, 0u, 0u, 0u);
         }
-        tc_fence_before();
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int row = warp * 16 + (i0 + i) * kPass + lane / kLanes;
+          *reinterpret_cast<uint4*>(smem + F::OFF_Q + (col >> 3) * (kRows * 128) + row * 128 + (((col ^ row) & 7) << 4)) = x[i];
+        }
       }
+      fence_async_smem();
       warp_arrive<PAIR>(sm.q_ready);
     };
     // A row's two warps meet at the same named barriers in the same order; every
@@ -692,9 +687,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     // this thread's share of a masked tile's V: rows past the end and non-finite values -> 0
     auto clean_v = [&](const Piece& u, int t, int gt) -> bool {
       constexpr uint32_t kExp = BF ? 0x7F807F80u : 0x7C007C00u, kOne = BF ? 0x00800080u : 0x04000400u;
-      const int j0 = (u.t0 + t) * KT, st = gt % kStages;
+      const int j0 = (u.t0 + t) * KT, st = gt % F::VS;
       if (!__all_sync(0xffffffffu, rank ? wait(sm.v_here[gt % NB], (gt / NB) & 1, abort_flag)
-                                        : wait(sm.v_full[st], (gt / kStages) & 1, abort_flag)))
+                                        : wait(sm.v_full[st], (gt / F::VS) & 1, abort_flag)))
         return false;
       const int live = min(KT, u.L - j0);          // rows of real keys
       const bool scan = u.vis0 < j0 + live;        // some token does not see them all
@@ -766,7 +761,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               // the masked tiles' non-finite values, for the rows that see their keys
 #pragma unroll 1
               for (int j = max(u.t0 * KT, max(u.vis0, 0) / KT * KT); j < min(u.t1 * KT, vis); ++j) {
-                const int64_t s = a.kv_indices[sm.kv[u.b] + j];
+                const int64_t s = a.kv_indices[u.k0 + j];
                 if (s < 0 || s >= a.n_slots) continue;
                 const uint16_t* vr = static_cast<const uint16_t*>(a.v_cache) + s * a.kv_st + u.h * a.kv_sh + (D / 2) * wg + 32 * c;
 #pragma unroll
@@ -776,16 +771,35 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
               }
             }
-            if (!row_ok) continue;
             if (u.slot < 0) {
-              uint4* dst = reinterpret_cast<uint4*>(orow + c * 64);
+              // four lanes swap their 16-byte pieces, so that a store writes 64
+              // bytes of 8 rows and not 16 of 32
+              uint32_t y[4][4];
 #pragma unroll
-              for (int q = 0; q < 4; ++q)
-                dst[q] = make_uint4(pack2<BF>(v[8 * q] * inv, v[8 * q + 1] * inv),
-                                    pack2<BF>(v[8 * q + 2] * inv, v[8 * q + 3] * inv),
-                                    pack2<BF>(v[8 * q + 4] * inv, v[8 * q + 5] * inv),
-                                    pack2<BF>(v[8 * q + 6] * inv, v[8 * q + 7] * inv));
-            } else {
+              for (int q = 0; q < 16; ++q) y[q >> 2][q & 3] = pack2<BF>(v[2 * q] * inv, v[2 * q + 1] * inv);
+#pragma unroll
+              for (int d = 1; d < 4; d <<= 1) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  if (q & d) continue;
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    // lanes with bit d of the index set give piece q and take q | d, the others the reverse
+                    const bool hi = lane & d;
+                    const uint32_t get = __shfl_xor_sync(0xffffffffu, hi ? y[q][e] : y[q | d][e], d);
+                    if (hi) y[q][e] = get;
+                    else y[q | d][e] = get;
+                  }
+                }
+              }
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {  // y[q]: piece lane & 3 of the row of lane (lane & ~3) + q
+                unsigned char* to = reinterpret_cast<unsigned char*>(
+                    __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(orow), (lane & 28) + q));
+                if (__shfl_sync(0xffffffffu, (int)row_ok, (lane & 28) + q))
+                  *reinterpret_cast<uint4*>(to + c * 64 + (lane & 3) * 16) = make_uint4(y[q][0], y[q][1], y[q][2], y[q][3]);
+              }
+            } else if (row_ok) {
               float4* dst = reinterpret_cast<float4*>(P.ws_o + prow * D + (D / 2) * wg + 32 * c);
 #pragma unroll
               for (int q = 0; q < 8; ++q) dst[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
@@ -934,6 +948,7 @@ constexpr int kMergeThreads = 256, kMergeY = 8;
 template <bool BF, int D>
 __global__ void __launch_bounds__(kMergeThreads) chunk_attn_merge(const __grid_constant__ Params P) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   constexpr int kLanes = D / 4, kPass = kMergeThreads / kLanes, kSlotRows = kRows * Cfg<D>::CG;
   __shared__ int list[kMergeThreads + 1], flags[kMergeThreads], n_list;
   const int c = blockIdx.x, grid = gridDim.x;
@@ -1045,26 +1060,25 @@ int launch(const Params& P, int workers, const CUtensorMap& k_map, const CUtenso
   DFT_CUDA_CHECK(cudaFuncSetAttribute(chunk_attn_kernel<BF, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)smem_bytes<D>()));
   cudaLaunchConfig_t cfg;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3((unsigned)(workers * Cfg<D>::CG));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem_bytes<D>();
   cfg.stream = st;
   cfg.attrs = attr;
-  if (Cfg<D>::kPair) {
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.numAttrs = 1;
-  }
+  // both kernels come up under the launch before them and wait for its end
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.numAttrs = Cfg<D>::kPair ? 2 : 1;
   DFT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, chunk_attn_kernel<BF, D>, k_map, v_map, P, status));
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3((unsigned)workers, kMergeY);
   cfg.blockDim = dim3(kMergeThreads);
   cfg.stream = st;
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   DFT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, chunk_attn_merge<BF, D>, P));
@@ -1090,6 +1104,7 @@ extern "C" int dft_chunk_attn(const dft_chunk_attn_args* a, void* ws, int32_t* d
   memset(&P, 0, sizeof(P));
   P.a = *a;
   P.G = a->Hq / a->Hkv;
+  P.inv_G = (65535u + P.G) / P.G;
   P.TQ = kRows * (a->D == 256 ? Cfg<256>::CG : 1) / P.G;
   P.ws_meta = reinterpret_cast<int4*>(static_cast<char*>(ws) + w.meta);
   P.ws_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + w.ml);
