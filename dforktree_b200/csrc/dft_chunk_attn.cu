@@ -65,8 +65,8 @@ constexpr uint32_t kTmemCols = 512;
 constexpr int kMaxStages = 4, kRing = 4;
 // A unit's fixed cost in keys (query load, first tile's latency, output), and
 // the least share of a worker: under it a cut costs more than it spreads.
-constexpr int kUnitKeys = 256;
-constexpr int kMinShare = 384;
+constexpr int kUnitKeys = 512;
+constexpr int kMinShare = 256;
 
 #ifndef DFT_KT
 #define DFT_KT(D) 128
@@ -102,7 +102,7 @@ struct Piece {
 };
 
 struct Small {
-  uint64_t q_ready;
+  uint64_t q_ready, q_empty;
   uint64_t k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages];
   uint64_t k_copied[kMaxStages], v_copied[kMaxStages];  // rank 1 of a pair: its cp.async rows of the stage
   uint64_t s_full[4], p_full[4], pv_done[4];
@@ -127,8 +127,8 @@ struct Small {
 
 struct Params {
   dft_chunk_attn_args a;
-  int G, TQ;                // q-heads per kv-head, tokens per query tile
-  uint32_t inv_G;           // ceil(2^16 / G): row / G = row * inv_G >> 16 for rows below 256 and G up to 128
+  int G, TC, TQ;            // q-heads per kv-head, tokens of a query tile per CTA and in all
+  uint32_t inv_G;           // ceil(2^16 / G): row / G = row * inv_G >> 16 for rows below 128 and G up to 128
   float* ws_o;              // [2 workers][rows][D] partial O: slot 2c continues a unit, 2c + 1 begins one
   float* ws_ml;             // [2 workers][rows][2] partial (m, l)
   int4* ws_meta;            // [2 workers] (flags, first token row, tokens, kv-head); flags 1: used, 2: the unit's last
@@ -292,8 +292,8 @@ __device__ __forceinline__ bool next_piece(const Small& sm, const Params& P, int
 
 template <bool BF, int D>
 __global__ void __launch_bounds__(kThreads, 1)
-    chunk_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
-                      const __grid_constant__ Params P, int32_t* status) {
+    chunk_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                      const __grid_constant__ CUtensorMap v_map, const __grid_constant__ Params P, int32_t* status) {
   using F = Cfg<D>;
   constexpr bool PAIR = F::kPair;
   constexpr int KT = F::KT, NB = F::NB, kAhead = NB - 1, CG = F::CG;
@@ -311,7 +311,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp == kCtlWarp) {
     if (lane == 0) {
-      mbar_init(smem_u32(&sm.q_ready), kSoftmax / 32 * CG);
+      mbar_init(smem_u32(&sm.q_ready), CG);
+      mbar_init(smem_u32(&sm.q_empty), 1);
       for (int i = 0; i < kMaxStages; ++i) {
         // a warp's cp.async and an expect_tx; from rank 1 an expect_tx and, once its cp.async are in, an arrival
         mbar_init(smem_u32(&sm.k_copied[i]), 32);
@@ -403,6 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                          bd + ((k >> 2) * 1024 + (k & 3) * 32) / 16, id_s, k > 0);
             commit(sm.k_empty[st]);
             commit(sm.s_full[sb]);
+            if (t == T - 1) commit(sm.q_empty);
           }
           if (t >= kAhead) {
             const int gu = g + t - kAhead, st = gu % F::VS, pb = gu % NB;
@@ -467,30 +469,38 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0 && !mbar_wait(smem_u32(&sm.mma_done), 0)) raise_status(status, DFT_DEV_TIMEOUT);
     __syncwarp();
   } else if (warp == kPlanWarp) {
-    // --------------------------------- plan: pieces, and their Q towards L2
+    // ------------------------------------------ plan: the pieces, and their Q
     const int64_t share = max((int64_t)kMinShare, (total + workers - 1) / workers), w1 = min(total, share * (worker + 1));
     int64_t w = min(total, share * worker);
-    bool ok = true, more = true;
-    for (int n = 0; ok && more; ++n) {
+    const uint64_t pol = l2_evict_first();
+    const uint32_t lead = elect_lane();
+    bool ok = true;
+    int ui = 0;  // pieces whose Q is on its way
+#pragma unroll 1
+    for (int n = 0;; ++n) {
       const int i = n % kRing;
       if (n >= kRing) ok = __all_sync(0xffffffffu, wait(sm.ring_empty[i], (n / kRing - 1) & 1, abort_flag));
       if (!ok) break;
-      more = next_piece<KT>(sm, P, w, w1, p);
+      const bool more = next_piece<KT>(sm, P, w, w1, p);
       if (!more) p.b = -1;
       if (lane == 0) {
         sm.ring[i] = p;
         mbar_arrive(smem_u32(&sm.ring_full[i]));
       }
-      if (more && p.t1 > p.t0) {
-        for (int r = lane; r < kRows; r += 32) {
-          const int t = (int)((rank * kRows + r) * P.inv_G >> 16), hq = rank * kRows + r - t * P.G;
-          if (t >= p.ntok) break;
-          const unsigned char* row = static_cast<const unsigned char*>(a.q) +
-                                     ((int64_t)(p.tok0 + t) * a.q_st + (int64_t)(p.h * P.G + hq) * a.q_sh) * 2;
+      if (!more) break;
+      if (p.t1 == p.t0) continue;
+      // its Q, a box of tokens x G heads per 64 dims, once the piece before has no S
+      // MMA left; rows past the piece's tokens hold what follows and are nobody's
+      if (ui > 0) ok = __all_sync(0xffffffffu, wait(sm.q_empty, (ui - 1) & 1, abort_flag));
+      if (!ok) break;
+      const uint32_t bar = PAIR ? map_rank(smem_u32(&sm.q_ready), 0) : smem_u32(&sm.q_ready);
+      if (lane == 0) mbar_expect_tx_cluster<PAIR>(bar, P.TC * P.G * D * 2);
+      __syncwarp();
 #pragma unroll
-          for (int c = 0; c < 2 * D; c += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + c));
-        }
-      }
+      for (int c = 0; c < D / 64; ++c)
+        tma_load_4d<CG>(lead, smem_u32(smem) + F::OFF_Q + c * (kRows * 128), &q_map, 0, p.h * P.G,
+                        p.tok0 + rank * P.TC, c, bar, pol);
+      ++ui;
     }
     if (!ok && lane == 0 && !*abort_flag) set_abort(sm, status);
   } else if (warp >= kProdWarp0) {
@@ -626,41 +636,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------- softmax and output, two threads per row, one half of the columns each
     constexpr float kBias = BF ? 0.f : 6.f; // float16 P: up to 2^14, so that small weights stay clear of its smallest step
     const int r = (warp & 3) * 32 + lane;   // TMEM lane
-    const int R = rank * kRows + r;         // query row of the tile
     const int wg = warp >> 2;               // half of S's, O's and Q's columns
     const int pair_bar = 1 + (warp & 3);    // named barrier of warps w and w + 4 (same rows)
     const int wq = warp & 3;
-    const int tok = (int)(R * P.inv_G >> 16), g_ = R - tok * P.G;
+    const int rt = (int)(r * P.inv_G >> 16), g_ = r - rt * P.G;  // the row's token in the CTA, and its head
+    const int tok = rt < P.TC ? rank * P.TC + rt : 1 << 20;      // in the piece; rows past the last token are spare
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const float sc = a.sm_scale * 1.4426950408889634f;
     // a partial slot that no piece of this CTA fills is marked so
     int slots_used = 0;
-    // A piece's Q -> shared memory (128B-swizzled, 64-dim chunks kRows rows apart):
-    // 16 rows a warp, whole rows in a load (a row per lane took 6000 cycles, a line
-    // looked up for every 16 bytes); spare rows are zero.
-    auto load_q = [&](const Piece& u) {
-      constexpr int kLanes = D / 8, kPass = 32 / kLanes, kTurns = 16 / kPass;  // lanes a row, rows a pass, passes
-      const int col = lane % kLanes;
-      constexpr int kBatch = kTurns < 4 ? kTurns : 4;
-#pragma unroll 1
-      for (int i0 = 0; i0 < kTurns; i0 += kBatch) {
-        uint4 x[kBatch];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int row = rank * kRows + warp * 16 + (i0 + i) * kPass + lane / kLanes, t = (int)(row * P.inv_G >> 16);
-          const unsigned char* from = static_cast<const unsigned char*>(a.q) + 16 * col +
-                                      ((int64_t)(u.tok0 + t) * a.q_st + (int64_t)(u.h * P.G + row - t * P.G) * a.q_sh) * 2;
-          x[i] = t < u.ntok ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0u, 0u, 0u, 0u);
-        }
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int row = warp * 16 + (i0 + i) * kPass + lane / kLanes;
-          *reinterpret_cast<uint4*>(smem + F::OFF_Q + (col >> 3) * (kRows * 128) + row * 128 + (((col ^ row) & 7) << 4)) = x[i];
-        }
-      }
-      fence_async_smem();
-      warp_arrive<PAIR>(sm.q_ready);
-    };
     // A row's two warps meet at the same named barriers in the same order; every
     // early exit is decided from outcomes that both have exchanged there.
     bool held = true;  // false: a wait gave up since the last exchange
@@ -727,18 +711,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_async_smem();  // these writes before the tensor core's reads
       return true;
     };
-    // Unit after unit: the next one's Q goes in before the last one's output
-    // comes out, so that its S runs meanwhile.
+    // Unit after unit; the next one's Q, K and S come in while the last one's output goes out.
     bool pending = false;
     float m_used = -INFINITY, l = 0.f;
     Piece u;
     while (ok) {
-      const bool more = next_live(p);  // every S MMA of unit u has been consumed
+      const bool more = next_live(p);
       if (!ok) break;
-      if (more) load_q(p);
       if (pending) {
         // ---- epilogue of unit u: wait for its last P V, then O (or its partial) out
-        const bool row_ok = tok < u.ntok, busy = rank * kRows + wq * 32 < u.ntok * P.G;
+        const bool row_ok = tok < u.ntok, busy = wq * 32 < min(P.TC, u.ntok - rank * P.TC) * P.G;
         const int vis = max(0, min(u.L, u.vis0 + (row_ok ? tok : 0)));
         const bool got = __all_sync(0xffffffffu, wait(sm.o_full, ui & 1, abort_flag));
         tc_fence_after();
@@ -748,10 +730,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         l = sm.lsum[0][r] + sm.lsum[1][r];
         ok = got && sm.oke[wg ^ 1][wq];
         if (ok && busy) {
-          const int64_t prow = (int64_t)(2 * worker + max(u.slot, 0)) * (kRows * CG) + R;
+          const int64_t prow = (int64_t)(2 * worker + max(u.slot, 0)) * (kRows * CG) + (row_ok ? tok * P.G + g_ : 0);
           const float inv = l == 0.f ? 0.f : 1.f / l;
-          unsigned char* orow = static_cast<unsigned char*>(a.o) +
-                                ((int64_t)(u.tok0 + tok) * a.o_st + (int64_t)(u.h * P.G + g_) * a.o_sh) * 2 + wg * D;
+          // the rows of this lane's four; its 16 bytes of each 64
+          unsigned char* to[4];
+          bool there[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int rr = (r & ~3) + q, t = (int)(rr * P.inv_G >> 16);
+            there[q] = t < min(P.TC, u.ntok - rank * P.TC);
+            to[q] = static_cast<unsigned char*>(a.o) + wg * D + (lane & 3) * 16 +
+                    ((int64_t)(u.tok0 + rank * P.TC + t) * a.o_st + (int64_t)(u.h * P.G + rr - t * P.G) * a.o_sh) * 2;
+          }
           const bool odd = sm.odd[ui & 7] == ui + 1;
 #pragma unroll 1
           for (int c = 0; c < D / 64; ++c) {
@@ -793,12 +783,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
               }
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {  // y[q]: piece lane & 3 of the row of lane (lane & ~3) + q
-                unsigned char* to = reinterpret_cast<unsigned char*>(
-                    __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(orow), (lane & 28) + q));
-                if (__shfl_sync(0xffffffffu, (int)row_ok, (lane & 28) + q))
-                  *reinterpret_cast<uint4*>(to + c * 64 + (lane & 3) * 16) = make_uint4(y[q][0], y[q][1], y[q][2], y[q][3]);
-              }
+              for (int q = 0; q < 4; ++q)  // y[q]: piece lane & 3 of the q-th of the four rows
+                if (there[q])
+                  *reinterpret_cast<uint4*>(to[q] + c * 64) = make_uint4(y[q][0], y[q][1], y[q][2], y[q][3]);
             } else if (row_ok) {
               float4* dst = reinterpret_cast<float4*>(P.ws_o + prow * D + (D / 2) * wg + 32 * c);
 #pragma unroll
@@ -828,7 +815,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool row_ok = tok < u.ntok;
       const int T = u.t1 - u.t0;
       const int vis = max(0, min(u.L, u.vis0 + (row_ok ? tok : 0)));  // keys this row sees: j < vis
-      const bool busy = rank * kRows + wq * 32 < u.ntok * P.G;        // the warp holds rows
+      const bool busy = wq * 32 < min(P.TC, u.ntok - rank * P.TC) * P.G;  // the warp holds rows
       m_used = -INFINITY;
       l = 0.f;
 #pragma unroll 1
@@ -1018,7 +1005,8 @@ int check_args(const dft_chunk_attn_args* a) {
   if (a->q_st < 0 || a->q_sh < 0 || (a->T > 1 && a->o_st < a->D) || (a->Hq > 1 && a->o_sh < a->D) ||
       a->kv_st < a->D || (a->Hkv > 1 && a->kv_sh < a->D))
     return DFT_ERR_INVALID;
-  if (a->kv_st >= ((int64_t)1 << 31) || a->kv_sh >= ((int64_t)1 << 38) || a->n_slots > 0x7FFFFFFF)
+  if (a->kv_st >= ((int64_t)1 << 31) || a->kv_sh >= ((int64_t)1 << 38) || a->q_st >= ((int64_t)1 << 38) ||
+      a->q_sh >= ((int64_t)1 << 38) || a->n_slots > 0x7FFFFFFF)
     return DFT_ERR_UNSUPPORTED;
   return DFT_OK;
 }
@@ -1042,11 +1030,12 @@ Workspace workspace(const dft_chunk_attn_args* a, int workers) {
   return w;
 }
 
-// the cache as (64 dims, slots, 64-dim chunks, heads): any slot and head stride
-bool encode(CUtensorMap* m, const dft_chunk_attn_args* a, const void* base, int rows, int chunks) {
-  const cuuint64_t dims[4] = {64, (cuuint64_t)a->n_slots, (cuuint64_t)a->D / 64, (cuuint64_t)a->Hkv};
-  const cuuint64_t strides[3] = {(cuuint64_t)a->kv_st * 2, 128, (cuuint64_t)a->kv_sh * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)rows, (cuuint32_t)chunks, 1}, estr[4] = {1, 1, 1, 1};
+// three-level strides in elements under 64 contiguous dims
+bool encode(CUtensorMap* m, const dft_chunk_attn_args* a, const void* base, const int64_t (&size)[3],
+            const int64_t (&stride)[3], const int (&box_)[3]) {
+  const cuuint64_t dims[4] = {64, (cuuint64_t)size[0], (cuuint64_t)size[1], (cuuint64_t)size[2]};
+  const cuuint64_t strides[3] = {(cuuint64_t)stride[0] * 2, (cuuint64_t)stride[1] * 2, (cuuint64_t)stride[2] * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_[0], (cuuint32_t)box_[1], (cuuint32_t)box_[2]}, estr[4] = {1, 1, 1, 1};
   return gtile::encode_fn() &&
          gtile::encode_fn()(m, a->dtype == DFT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                             4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -1055,7 +1044,7 @@ bool encode(CUtensorMap* m, const dft_chunk_attn_args* a, const void* base, int 
 }
 
 template <bool BF, int D>
-int launch(const Params& P, int workers, const CUtensorMap& k_map, const CUtensorMap& v_map, int32_t* status,
+int launch(const Params& P, int workers, const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map, int32_t* status,
            cudaStream_t st) {
   DFT_CUDA_CHECK(cudaFuncSetAttribute(chunk_attn_kernel<BF, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)smem_bytes<D>()));
@@ -1074,7 +1063,7 @@ int launch(const Params& P, int workers, const CUtensorMap& k_map, const CUtenso
   attr[1].val.clusterDim.x = 2;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.numAttrs = Cfg<D>::kPair ? 2 : 1;
-  DFT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, chunk_attn_kernel<BF, D>, k_map, v_map, P, status));
+  DFT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, chunk_attn_kernel<BF, D>, q_map, k_map, v_map, P, status));
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3((unsigned)workers, kMergeY);
   cfg.blockDim = dim3(kMergeThreads);
@@ -1105,18 +1094,23 @@ extern "C" int dft_chunk_attn(const dft_chunk_attn_args* a, void* ws, int32_t* d
   P.a = *a;
   P.G = a->Hq / a->Hkv;
   P.inv_G = (65535u + P.G) / P.G;
-  P.TQ = kRows * (a->D == 256 ? Cfg<256>::CG : 1) / P.G;
+  P.TC = kRows / P.G;
+  P.TQ = P.TC * (a->D == 256 ? Cfg<256>::CG : 1);
   P.ws_meta = reinterpret_cast<int4*>(static_cast<char*>(ws) + w.meta);
   P.ws_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + w.ml);
   P.ws_o = reinterpret_cast<float*>(static_cast<char*>(ws) + w.o);
-  CUtensorMap k_map, v_map;
-  if (!encode(&k_map, a, a->k_cache, 8, a->D / 64) ||
-      !encode(&v_map, a, a->v_cache, 16, a->D == 256 ? Cfg<256>::VC : a->D / 64))
+  // K, V: (slots, 64-dim chunks, heads); Q: (heads, tokens, chunks)
+  const int64_t chunks = a->D / 64;
+  const int vc = a->D == 256 ? Cfg<256>::VC : (int)chunks;
+  CUtensorMap q_map, k_map, v_map;
+  if (!encode(&q_map, a, a->q, {a->Hq, a->T, chunks}, {a->q_sh, a->q_st, 64}, {P.G, P.TC, 1}) ||
+      !encode(&k_map, a, a->k_cache, {a->n_slots, chunks, a->Hkv}, {a->kv_st, 64, a->kv_sh}, {8, (int)chunks, 1}) ||
+      !encode(&v_map, a, a->v_cache, {a->n_slots, chunks, a->Hkv}, {a->kv_st, 64, a->kv_sh}, {16, vc, 1}))
     return DFT_ERR_UNSUPPORTED;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool bf = a->dtype == DFT_BF16;
 #define DFT_GO(D_) \
-  return bf ? launch<true, D_>(P, workers, k_map, v_map, dev_status, st) : launch<false, D_>(P, workers, k_map, v_map, dev_status, st)
+  return bf ? launch<true, D_>(P, workers, q_map, k_map, v_map, dev_status, st) : launch<false, D_>(P, workers, q_map, k_map, v_map, dev_status, st)
   if (a->D == 64) DFT_GO(64);
   if (a->D == 128) DFT_GO(128);
   DFT_GO(256);
