@@ -116,7 +116,6 @@ struct Small {
   float lsum[2][kRows];     // [half][row] final row sums
   int okx[2][2][4];         // [tile parity][half][row warp] wait outcomes, shared by a row's two warps
   int okr[2][2][4];         // the same for the rescale's wait
-  int oke[2][4];            // [half][row warp] the epilogue's wait
   int okt[2][2][4];         // [unit parity][half][row warp] whether the warp goes on to the next unit
   int64_t pre[kMaxB + 1];   // cost of the requests before b
   int qo[kMaxB + 1], kv[kMaxB + 1];
@@ -419,11 +418,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t vb = __shfl_sync(0xffffffffu, v_base + st * F::kVBytes, 0);
             const uint32_t ps = __shfl_sync(0xffffffffu, tmem + F::COL_S + KT * pb, 0);
             const uint32_t keep = __shfl_sync(0xffffffffu, t > kAhead ? 1u : 0u, 0);
+            // P: 64 keys in columns 0 to 31 of its buffer, 64 in 64 to 95.
             // V [keys x dims] is MN-major: of 16 keys, 64-dim chunks 2 KB apart, 8-key groups 1 KB apart
             const uint64_t bd = sw128_desc(vb, 2048, 1024);
 #pragma unroll
             for (int k = 0; k < KT / 16; ++k)
-              mma_ts<CG>(lead, tmem + F::COL_O, ps + 8 * k, bd + k * F::VC * 2048 / 16, id_o, k > 0 ? 1u : keep);
+              mma_ts<CG>(lead, tmem + F::COL_O, ps + 8 * k + (k < 4 ? 0 : 32), bd + k * F::VC * 2048 / 16, id_o, k > 0 ? 1u : keep);
             commit(sm.v_empty[st]);
             commit(sm.pv_done[pb]);
             if (t == T + kAhead - 1) commit(sm.o_full);
@@ -678,29 +678,36 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int live = min(KT, u.L - j0);          // rows of real keys
       const bool scan = u.vis0 < j0 + live;        // some token does not see them all
       unsigned char* vb = smem + F::OFF_V + st * F::kVBytes;
+      constexpr int kTurns = KT * 8 / kSoftmax;  // 16-byte pieces of a chunk for a thread
       bool any = false;
 #pragma unroll 1
       for (int c = 0; c < F::VC; ++c) {
+        uint4 x[kTurns];
+        uint32_t hit = 0;
+        const auto piece = [&](int i) {
+          const int at = i * kSoftmax + tid;  // row at >> 3
+          return reinterpret_cast<uint4*>(vb + (at >> 7) * (F::VC * 2048) + c * 2048) + (at & 127);
+        };
+#pragma unroll
+        for (int i = 0; i < kTurns; ++i) {
+          if (i * kSoftmax + tid >= live * 8) *piece(i) = make_uint4(0u, 0u, 0u, 0u);
+          x[i] = scan ? *piece(i) : make_uint4(0u, 0u, 0u, 0u);
+        }
+        // a half's exponent is all ones iff adding one to it carries out
+#pragma unroll
+        for (int i = 0; i < kTurns; ++i)
+          hit |= ((x[i].x & kExp) + kOne) | ((x[i].y & kExp) + kOne) | ((x[i].z & kExp) + kOne) | ((x[i].w & kExp) + kOne);
+        if (hit & 0x80008000u) {
+          any = true;
+          const auto clean = [&](uint32_t& y) { y &= ~(((((y & kExp) + kOne) & 0x80008000u) >> 15) * 0xFFFFu); };
 #pragma unroll 1
-        for (int i = 0; i < KT * 8; i += kSoftmax) {
-          const int at = i + tid;  // row at >> 3
-          uint4* q = reinterpret_cast<uint4*>(vb + (at >> 7) * (F::VC * 2048) + c * 2048) + (at & 127);
-          if (at >= live * 8) {
-            *q = make_uint4(0u, 0u, 0u, 0u);
-          } else if (scan) {
-            uint4 x = *q;
-            // a half's exponent is all ones iff adding one to it carries out
-            const uint32_t hit = (((x.x & kExp) + kOne) | ((x.y & kExp) + kOne) | ((x.z & kExp) + kOne) |
-                                  ((x.w & kExp) + kOne)) & 0x80008000u;
-            if (hit) {
-              any = true;
-              auto clean = [&](uint32_t& y) { y &= ~(((((y & kExp) + kOne) & 0x80008000u) >> 15) * 0xFFFFu); };
-              clean(x.x);
-              clean(x.y);
-              clean(x.z);
-              clean(x.w);
-              *q = x;
-            }
+          for (int i = 0; i < kTurns; ++i) {
+            uint4 y = *piece(i);
+            clean(y.x);
+            clean(y.y);
+            clean(y.z);
+            clean(y.w);
+            *piece(i) = y;
           }
         }
       }
@@ -722,74 +729,63 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ---- epilogue of unit u: wait for its last P V, then O (or its partial) out
         const bool row_ok = tok < u.ntok, busy = wq * 32 < min(P.TC, u.ntok - rank * P.TC) * P.G;
         const int vis = max(0, min(u.L, u.vis0 + (row_ok ? tok : 0)));
-        const bool got = __all_sync(0xffffffffu, wait(sm.o_full, ui & 1, abort_flag));
-        tc_fence_after();
         sm.lsum[wg][r] = l;
-        if (lane == 0) sm.oke[wg][wq] = got;
         named_bar(pair_bar, 64);
         l = sm.lsum[0][r] + sm.lsum[1][r];
-        ok = got && sm.oke[wg ^ 1][wq];
-        if (ok && busy) {
-          const int64_t prow = (int64_t)(2 * worker + max(u.slot, 0)) * (kRows * CG) + (row_ok ? tok * P.G + g_ : 0);
-          const float inv = l == 0.f ? 0.f : 1.f / l;
-          // the rows of this lane's four; its 16 bytes of each 64
-          unsigned char* to[4];
-          bool there[4];
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int64_t prow = (int64_t)(2 * worker + max(u.slot, 0)) * (kRows * CG) + (row_ok ? tok * P.G + g_ : 0);
+        // the rows of this lane's two; its 16 bytes of each 32
+        unsigned char* to[2];
+        bool there[2];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int rr = (r & ~3) + q, t = (int)(rr * P.inv_G >> 16);
-            there[q] = t < min(P.TC, u.ntok - rank * P.TC);
-            to[q] = static_cast<unsigned char*>(a.o) + wg * D + (lane & 3) * 16 +
-                    ((int64_t)(u.tok0 + rank * P.TC + t) * a.o_st + (int64_t)(u.h * P.G + rr - t * P.G) * a.o_sh) * 2;
-          }
+        for (int q = 0; q < 2; ++q) {
+          const int rr = (r & ~1) + q, t = (int)(rr * P.inv_G >> 16);
+          there[q] = t < min(P.TC, u.ntok - rank * P.TC);
+          to[q] = static_cast<unsigned char*>(a.o) + wg * D + (lane & 1) * 16 +
+                  ((int64_t)(u.tok0 + rank * P.TC + t) * a.o_st + (int64_t)(u.h * P.G + rr - t * P.G) * a.o_sh) * 2;
+        }
+        held = held && __all_sync(0xffffffffu, wait(sm.o_full, ui & 1, abort_flag));
+        tc_fence_after();
+        if (held && busy) {
           const bool odd = sm.odd[ui & 7] == ui + 1;
 #pragma unroll 1
-          for (int c = 0; c < D / 64; ++c) {
-            float v[32];
-            tmem_ld32(tmem + lane_base + F::COL_O + (D / 2) * wg + 32 * c, v);
+          for (int c = 0; c < D / 2; c += 16) {
+            float v[16];
+            tmem_ld16(tmem + lane_base + F::COL_O + (D / 2) * wg + c, v);
             if (odd) {
               // the masked tiles' non-finite values, for the rows that see their keys
 #pragma unroll 1
               for (int j = max(u.t0 * KT, max(u.vis0, 0) / KT * KT); j < min(u.t1 * KT, vis); ++j) {
                 const int64_t s = a.kv_indices[u.k0 + j];
                 if (s < 0 || s >= a.n_slots) continue;
-                const uint16_t* vr = static_cast<const uint16_t*>(a.v_cache) + s * a.kv_st + u.h * a.kv_sh + (D / 2) * wg + 32 * c;
+                const uint16_t* vr = static_cast<const uint16_t*>(a.v_cache) + s * a.kv_st + u.h * a.kv_sh + (D / 2) * wg + c;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
+                for (int i = 0; i < 16; ++i) {
                   const float y = unpack<BF>(vr[i]);
                   v[i] += fabsf(y) < INFINITY ? 0.f : y;
                 }
               }
             }
             if (u.slot < 0) {
-              // four lanes swap their 16-byte pieces, so that a store writes 64
-              // bytes of 8 rows and not 16 of 32
-              uint32_t y[4][4];
+              // two lanes swap 16-byte pieces, so that a store writes 32 bytes of 16
+              // rows and not 16 of 32
+              uint32_t y[2][4];
 #pragma unroll
-              for (int q = 0; q < 16; ++q) y[q >> 2][q & 3] = pack2<BF>(v[2 * q] * inv, v[2 * q + 1] * inv);
+              for (int q = 0; q < 8; ++q) y[q >> 2][q & 3] = pack2<BF>(v[2 * q] * inv, v[2 * q + 1] * inv);
 #pragma unroll
-              for (int d = 1; d < 4; d <<= 1) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                  if (q & d) continue;
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) {
-                    // lanes with bit d of the index set give piece q and take q | d, the others the reverse
-                    const bool hi = lane & d;
-                    const uint32_t get = __shfl_xor_sync(0xffffffffu, hi ? y[q][e] : y[q | d][e], d);
-                    if (hi) y[q][e] = get;
-                    else y[q | d][e] = get;
-                  }
-                }
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t get = __shfl_xor_sync(0xffffffffu, lane & 1 ? y[0][e] : y[1][e], 1);
+                if (lane & 1) y[0][e] = get;
+                else y[1][e] = get;
               }
 #pragma unroll
-              for (int q = 0; q < 4; ++q)  // y[q]: piece lane & 3 of the q-th of the four rows
+              for (int q = 0; q < 2; ++q)  // y[q]: piece lane & 1 of the q-th of the two rows
                 if (there[q])
-                  *reinterpret_cast<uint4*>(to[q] + c * 64) = make_uint4(y[q][0], y[q][1], y[q][2], y[q][3]);
+                  *reinterpret_cast<uint4*>(to[q] + c * 2) = make_uint4(y[q][0], y[q][1], y[q][2], y[q][3]);
             } else if (row_ok) {
-              float4* dst = reinterpret_cast<float4*>(P.ws_o + prow * D + (D / 2) * wg + 32 * c);
+              float4* dst = reinterpret_cast<float4*>(P.ws_o + prow * D + (D / 2) * wg + c);
 #pragma unroll
-              for (int q = 0; q < 8; ++q) dst[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+              for (int q = 0; q < 4; ++q) dst[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
             }
           }
           if (u.slot >= 0 && wg == 0 && row_ok) {
@@ -797,7 +793,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             P.ws_ml[2 * prow + 1] = l;
           }
         }
-        if (ok) {
+        if (held) {
           if (u.slot >= 0) {
             slots_used |= 1 << u.slot;
             if (tid == 0 && rank == 0)
@@ -809,7 +805,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         ++ui;
       }
-      if (!ok || !more) break;
+      if (!more) break;
       u = p;
       pending = true;
       const bool row_ok = tok < u.ntok;
@@ -826,17 +822,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int j0 = (u.t0 + t) * KT;
         const bool plain = j0 + KT <= u.vis0 && j0 + KT <= u.L;
         if (busy) {  // else spare rows: whatever P holds stays in them
-          const uint32_t ts = tmem + lane_base + F::COL_S + KT * sb;
+          const uint32_t ts = tmem + lane_base + F::COL_S + KT * sb + 64 * wg;  // this thread's 64 columns of S
           float x[64];
           tc_fence_after();
-          tmem_ld32_async(ts + 64 * wg, &x[0]);
-          tmem_ld32_async(ts + 64 * wg + 32, &x[32]);
+          tmem_ld32_async(ts, &x[0]);
+          tmem_ld32_async(ts + 32, &x[32]);
           tmem_ld_wait(x);
           if (!plain) {
-            const int c0 = vis - j0 - 64 * wg;  // columns of this half that the row sees
+            const int seen = vis - j0 - 64 * wg;  // columns that the row sees
 #pragma unroll
             for (int i = 0; i < 64; ++i)
-              if (i >= c0) x[i] = -INFINITY;
+              if (i >= seen) x[i] = -INFINITY;
           }
           float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -844,15 +840,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             mx[0] = fmaxf(fmaxf(mx[0], x[i]), x[i + 1]);
             mx[1] = fmaxf(fmaxf(mx[1], x[i + 2]), x[i + 3]);
           }
-          // x stays raw: P = 2^(x sc - m)
-          float tmax = fmaxf(mx[0], mx[1]) * sc;
+          float tmax = fmaxf(mx[0], mx[1]);
+          // S stays raw: P = 2^(S sc - m)
+          tmax *= sc;
           sm.xmax[par][wg][r] = tmax;
           if (lane == 0) sm.okx[par][wg][wq] = got;
-          // the barrier also orders this half's S reads before the other half's P
-          // stores (half 1 writes P over S columns that half 0 reads)
-          tc_fence_before();
           named_bar(pair_bar, 64);
-          tc_fence_after();
           tmax = fmaxf(tmax, sm.xmax[par][wg ^ 1][r]);
           ok = got && sm.okx[par][wg ^ 1][wq];
           if (!ok) break;
@@ -897,7 +890,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               sum2[i & 1] = add2(sum2[i & 1], pk2(p0, p1));
               pk[i] = pack2<BF>(p0, p1);
             }
-            tmem_st16_async(ts + 32 * wg + c / 2, pk);
+            tmem_st16_async(ts + c / 2, pk);  // over this thread's own columns, which are read
           }
           float s0, s1;
           upk2(add2(sum2[0], sum2[1]), s0, s1);
@@ -912,7 +905,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       g += T;
     }
-    ok = ok && p.b != -2;
+    ok = ok && held && p.b != -2;
     if (tid == 0 && rank == 0)
       for (int s = 0; s < 2; ++s)
         if (!(slots_used >> s & 1)) P.ws_meta[2 * worker + s] = make_int4(0, 0, 0, 0);

@@ -687,8 +687,8 @@ def chunk_attention(q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, sm_sc
     if dtype is None or not (q.dtype is k_cache.dtype is v_cache.dtype):
         raise L.DFTError("chunk_attention: q and the caches must be alike bfloat16 or float16")
     if o is None:
-        o = torch.empty(shape, dtype=q.dtype, device=q.device)
-        os = (Hq * D, D)
+        o = torch.empty_like(q)
+        os = o.stride()
     else:
         os = o.stride()
         if o.shape != shape or o.dtype is not q.dtype or os[2] != 1:
