@@ -117,7 +117,7 @@ struct Small {
   int okx[2][2][4];         // [tile parity][half][row warp] wait outcomes, shared by a row's two warps
   int okr[2][2][4];         // the same for the rescale's wait
   int okt[2][2][4];         // [unit parity][half][row warp] whether the warp goes on to the next unit
-  int64_t pre[kMaxB + 1];   // cost of the requests before b
+  uint32_t pre[kMaxB + 1];  // cost of the requests before b
   int qo[kMaxB + 1], kv[kMaxB + 1];
   Piece ring[kRing];           // the worker's pieces as they come, from the plan warp
   int4 slots[2][32];
@@ -127,6 +127,7 @@ struct Small {
 struct Params {
   dft_chunk_attn_args a;
   int G, TC, TQ;            // q-heads per kv-head, tokens of a query tile per CTA and in all
+  int shift;                // costs on the line are in 2^shift keys
   uint32_t inv_G;           // ceil(2^16 / G): row / G = row * inv_G >> 16 for rows below 128 and G up to 128
   float* ws_o;              // [2 workers][rows][D] partial O: slot 2c continues a unit, 2c + 1 begins one
   float* ws_ml;             // [2 workers][rows][2] partial (m, l)
@@ -181,7 +182,9 @@ __device__ __forceinline__ void warp_arrive(uint64_t& bar) {
 // Request b: n tokens in nt query tiles, L keys.  Tile i ends at token e =
 // min((i + 1) TQ, n) and reads the keys its last token sees, clamp(L - n + e,
 // 0, L); its cost is that + kUnitKeys, and the sum over the tiles before i is
-// an arithmetic series.
+// an arithmetic series.  Costs on the line are those sums over 2^shift, rounded
+// down (a tile's own is the difference of two), so that the line fits 32 bits:
+// with 64-bit divisions finding a first piece took 8000 cycles of fetching code.
 struct Req {
   int n, L, nt;
 };
@@ -189,57 +192,57 @@ __device__ __forceinline__ Req request(const Small& sm, int b, int TQ) {
   Req r;
   r.n = sm.qo[b + 1] - sm.qo[b];
   r.L = sm.kv[b + 1] - sm.kv[b];
-  r.nt = (r.n + TQ - 1) / TQ;
+  r.nt = (int)((uint32_t)(r.n + TQ - 1) / (uint32_t)TQ);
   return r;
 }
-__device__ __forceinline__ int tile_keys(const Req& r, int i, int TQ) {
-  const int64_t e = min((int64_t)(i + 1) * TQ, (int64_t)r.n);
-  return (int)max((int64_t)0, r.L - r.n + e);
-}
-__device__ __forceinline__ int64_t cost_before(const Req& r, int i, int TQ) {
-  int64_t last = 0;
+__device__ __forceinline__ uint32_t cost_before(const Req& r, int i, const Params& P) {
+  uint64_t last = 0;
   if (i == r.nt && i > 0) {  // the last tile is the one that may be short
-    last = r.L + kUnitKeys;
+    last = (uint32_t)r.L + kUnitKeys;
     --i;
   }
-  const int64_t a = r.L - (int64_t)r.n;
-  const int64_t z = a < 0 ? min((int64_t)i, -a / TQ) : 0;  // tiles that see no key
-  return last + (int64_t)i * kUnitKeys + (i - z) * a + TQ * (((int64_t)i * (i + 1) - z * (z + 1)) / 2);
+  const int a = r.L - r.n;
+  const uint32_t z = a < 0 ? min((uint32_t)i, (uint32_t)-a / (uint32_t)P.TQ) : 0u;  // tiles that see no key
+  const uint64_t pairs = (uint64_t)(uint32_t)i * (uint32_t)(i + 1) - (uint64_t)z * (z + 1);
+  const int64_t keys = (int64_t)(i - (int)z) * a + (int64_t)(pairs >> 1) * P.TQ;
+  return (uint32_t)((last + (uint64_t)(uint32_t)i * kUnitKeys + (uint64_t)keys) >> P.shift);
 }
 
 // The line: offsets to shared memory, and the cost of the requests before each
 // (by one warp; lane i sums a run of requests).  Returns the line's length.
-__device__ __forceinline__ int64_t plan_costs(Small& sm, const Params& P, int32_t* status) {
+__device__ __forceinline__ uint32_t plan_costs(Small& sm, const Params& P, int32_t* status) {
   const dft_chunk_attn_args& a = P.a;
-  const int lane = threadIdx.x & 31, per = (a.B + 31) / 32;
+  const int lane = threadIdx.x & 31, per = (a.B + 31) >> 5;
+#pragma unroll 1
   for (int i = lane; i <= a.B; i += 32) {
     sm.qo[i] = a.qo_indptr[i];
     sm.kv[i] = a.kv_indptr[i];
   }
   __syncwarp();
-  int64_t sum = 0;
+  const int b0 = lane * per, b1 = min(a.B, b0 + per);
+  uint32_t sum = 0;
   bool bad = false;
 #pragma unroll 1
-  for (int b = lane * per; b < min(a.B, (lane + 1) * per); ++b) {
+  for (int b = b0; b < b1; ++b) {
     const int q0 = sm.qo[b], q1 = sm.qo[b + 1], k0 = sm.kv[b], k1 = sm.kv[b + 1];
     const bool ok = q0 >= 0 && q0 <= q1 && q1 <= a.T && k0 >= 0 && k0 <= k1 && k1 <= a.n_kv && k1 - k0 <= 0x7FFFFF00;
     bad |= !ok;
     sm.pre[b] = sum;  // so far from the lane's first
     if (ok && q1 > q0) {
       const Req r = request(sm, b, P.TQ);
-      sum += a.Hkv * cost_before(r, r.nt, P.TQ);
+      sum += a.Hkv * cost_before(r, r.nt, P);
     }
   }
   if (bad && blockIdx.x == 0) raise_status(status, DFT_DEV_BAD_INDEX);
-  int64_t inc = sum;
+  uint32_t inc = sum;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int64_t o = __shfl_up_sync(0xffffffffu, inc, d);
+    const uint32_t o = __shfl_up_sync(0xffffffffu, inc, d);
     if (lane >= d) inc += o;
   }
 #pragma unroll 1
-  for (int b = lane * per; b < min(a.B, (lane + 1) * per); ++b) sm.pre[b] += inc - sum;
-  const int64_t total = __shfl_sync(0xffffffffu, inc, 31);
+  for (int b = b0; b < b1; ++b) sm.pre[b] += inc - sum;
+  const uint32_t total = __shfl_sync(0xffffffffu, inc, 31);
   if (lane == 0) sm.pre[a.B] = total;
   __syncwarp();
   return total;
@@ -247,35 +250,45 @@ __device__ __forceinline__ int64_t plan_costs(Small& sm, const Params& P, int32_
 
 // The next piece of the line from w, w < w1, that has something to do.
 template <int KT>
-__device__ __forceinline__ bool next_piece(const Small& sm, const Params& P, int64_t& w, int64_t w1, Piece& p) {
+__device__ __forceinline__ bool next_piece(const Small& sm, const Params& P, uint32_t& w, uint32_t w1, Piece& p) {
+#pragma unroll 1
   while (w < w1) {
     int lo = 0, hi = P.a.B;  // pre[lo] <= w < pre[hi]
+#pragma unroll 1
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (sm.pre[mid] <= w) lo = mid;
       else hi = mid;
     }
     const Req r = request(sm, lo, P.TQ);
-    const int64_t per_head = cost_before(r, r.nt, P.TQ);
-    int64_t rest = w - sm.pre[lo];
-    const int h = (int)(rest / per_head);
-    rest -= h * per_head;
+    const uint32_t at = w - sm.pre[lo], per_head = (sm.pre[lo + 1] - sm.pre[lo]) / (uint32_t)P.a.Hkv;
+    const uint32_t h = at / per_head, rest = at - h * per_head;
+    // the tile: cost_before(i) <= rest < cost_before(i + 1)
     int i = 0;
+    uint32_t c0 = 0, c1 = per_head;
+#pragma unroll 1
     for (int top = r.nt; top - i > 1;) {
       const int mid = (i + top) >> 1;
-      if (cost_before(r, mid, P.TQ) <= rest) i = mid;
-      else top = mid;
+      const uint32_t c = cost_before(r, mid, P);
+      if (c <= rest) {
+        i = mid;
+        c0 = c;
+      } else {
+        top = mid;
+        c1 = c;
+      }
     }
-    const int64_t x0 = rest - cost_before(r, i, P.TQ);
-    const int keys = tile_keys(r, i, P.TQ);
-    const int64_t cost = keys + kUnitKeys, x1 = min(cost, x0 + (w1 - w));
+    const uint32_t x0 = rest - c0, x1 = min(c1 - c0, x0 + (w1 - w));
+    const bool whole = x1 == c1 - c0;
     w += x1 - x0;
+    const int keys = max(0, r.L - r.n + (int)min((int64_t)(i + 1) * P.TQ, (int64_t)r.n));
     const int nt = (keys + KT - 1) / KT;
-    p.t0 = x0 == 0 ? 0 : (int)min((int64_t)nt, (x0 + KT / 2) / KT);
-    p.t1 = x1 == cost ? nt : (int)min((int64_t)nt, (x1 + KT / 2) / KT);
+    const auto tile = [&](uint32_t x) { return (int)min((uint64_t)nt, (((uint64_t)x << P.shift) + KT / 2) / KT); };
+    p.t0 = x0 == 0 ? 0 : tile(x0);
+    p.t1 = whole ? nt : tile(x1);
     if (p.t0 == p.t1 && !(nt == 0 && x0 == 0)) continue;
     p.b = lo;
-    p.h = h;
+    p.h = (int)h;
     p.tok0 = sm.qo[lo] + i * P.TQ;
     p.ntok = min(P.TQ, r.n - i * P.TQ);
     p.k0 = sm.kv[lo];
@@ -346,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   if (PAIR) cluster_arrive();  // this CTA's barriers are up
   asm volatile("griddepcontrol.wait;" ::: "memory");  // inputs and workspace are the launches before's until here
-  const int64_t total = warp == kPlanWarp ? plan_costs(sm, P, status) : 0;
+  const uint32_t total = warp == kPlanWarp ? plan_costs(sm, P, status) : 0u;
   if (PAIR) cluster_wait();    // the other CTA's are too, before anything arrives on them
   tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
@@ -470,8 +483,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp == kPlanWarp) {
     // ------------------------------------------ plan: the pieces, and their Q
-    const int64_t share = max((int64_t)kMinShare, (total + workers - 1) / workers), w1 = min(total, share * (worker + 1));
-    int64_t w = min(total, share * worker);
+    const uint32_t share = max((uint32_t)kMinShare >> P.shift, (total + workers - 1) / workers);
+    uint32_t w = (uint32_t)min((uint64_t)total, (uint64_t)share * worker);
+    const uint32_t w1 = (uint32_t)min((uint64_t)total, (uint64_t)w + share);
     const uint64_t pol = l2_evict_first();
     const uint32_t lead = elect_lane();
     bool ok = true;
@@ -1086,6 +1100,12 @@ extern "C" int dft_chunk_attn(const dft_chunk_attn_args* a, void* ws, int32_t* d
   memset(&P, 0, sizeof(P));
   P.a = *a;
   P.G = a->Hq / a->Hkv;
+  // The line's length is at most heads x (query tiles) x (keys + kUnitKeys), mostly
+  // far from it; 31 bits of it.  Up to 2^8 every tile keeps a cost of its own, and
+  // 2^40 keys' tiles are minutes of work.
+  const double line = (double)a->Hkv * ((double)a->T / (kRows / P.G) + a->B) * ((double)a->n_kv + kUnitKeys);
+  while (P.shift < 8 && line / (double)(1 << P.shift) >= 2147483647.0) ++P.shift;
+  static_assert(kUnitKeys >> 8 >= 2 && kMinShare >> 8 >= 1, "costs");
   P.inv_G = (65535u + P.G) / P.G;
   P.TC = kRows / P.G;
   P.TQ = P.TC * (a->D == 256 ? Cfg<256>::CG : 1);
