@@ -8,18 +8,17 @@
 // one tcgen05 MMA serves them all; a single token's G rows go through the same
 // tile, whose spare rows cost no memory traffic.  D <= 128: a CTA and 128 rows.
 // D = 256: two CTAs (cta_group::2) and 256 rows, each CTA holding half of every
-// K / V tile: 128 rows against 128 keys need O, two S and Q in 640 TMEM columns
-// of 512, and with 64 keys the S MMAs run at half rate (72 cycles for 128 x 64
-// x 16 from TMEM, bound by reading A); Q in shared memory leaves a CTA alone no
-// room for two 128 KB tiles.  Per tile of 128 keys, one pass with a running
-// maximum and sum:
+// K / V tile: a CTA alone has room for Q (64 KB) and one 128 KB tile of 128 keys
+// in its shared memory, not for the next one, and with 64 keys its S MMAs run at
+// half rate (72 cycles for 128 x 64 x 16, bound by reading A).  Per tile of 128
+// keys, one pass with a running maximum and sum:
 //   K, V  by slot, 16 keys at a time, into separate rings of stages by one
 //         producer warp each: where the 16 slots are consecutive (pages of 16 and
 //         more) one TMA box of 16 cache rows x 64 dims per copy, else 16-byte
 //         cp.async row by row (a gather of four rows per TMA copy took 39 ns a
 //         copy, 5 us per 64 KB)
-//   S     = Q K^T    kind::f16, fp32 in TMEM; Q from TMEM, or from shared memory
-//         for a pair
+//   S     = Q K^T    kind::f16, fp32 in TMEM; Q from shared memory, where one TMA
+//         box of tokens x G heads per 64 dims puts it while the unit before ends
 //   P     = 2^(S sm_scale log2e - m), two threads per row; the reference m moves
 //         (and O is rescaled in TMEM) only when the maximum grows by more than
 //         8, so P <= 2^8; rounded to the 16-bit type over its own S (the second
@@ -57,20 +56,23 @@ using namespace dft::tc;
 namespace {
 
 constexpr int kMaxB = 1024;
+constexpr int kMaxKeys = 1 << 25; // of a request: 2^18 tiles of up to 4000 cycles, half of what a wait is given
 constexpr int kRows = 128;        // query rows of a CTA
 constexpr int kSoftmax = 256;     // two threads per query row, in warps w and w + 4
 constexpr int kCtlWarp = 8, kProdWarp0 = 9, kPlanWarp = 11;  // a producer warp for K, one for V
-constexpr int kThreads = 384;     // twelve warps leave 168 registers a thread
+constexpr int kThreads = 384;     // twelve warps leave 168 registers a thread; a row of 64 scores takes most of them
 constexpr uint32_t kTmemCols = 512;
 constexpr int kMaxStages = 4, kRing = 4;
-// A unit's fixed cost in keys (query load, first tile's latency, output), and
-// the least share of a worker: under it a cut costs more than it spreads.
+// A unit's fixed cost in keys (query load, first tile's latency, output): with
+// 256 / 512 / 1024 a prompt of 8192 tokens at D = 128 took 456 / 416 / 430 us.
+// The least share of a worker, under which a cut costs more than it spreads:
+// with 256 / 384 / 512 a single token on 4096 keys took 20 / 20 / 20.5 us and on
+// 1000 keys 13.6 / 14.7 / 15.5.
 constexpr int kUnitKeys = 512;
 constexpr int kMinShare = 256;
 
-#ifndef DFT_KT
-#define DFT_KT(D) 128
-#endif
+constexpr int KT = 128;           // keys per tile
+constexpr int NB = 2;             // S / P buffers
 template <int N>
 using Int = std::integral_constant<int, N>;
 
@@ -78,8 +80,6 @@ template <int D>
 struct Cfg {
   static constexpr bool kPair = D == 256;
   static constexpr int CG = kPair ? 2 : 1;                    // CTAs of a worker
-  static constexpr int KT = DFT_KT(D);                        // keys per tile
-  static constexpr int NB = KT == 64 ? 4 : 2;                 // S / P buffers
   static constexpr int KS = kPair ? 2 : D == 128 ? 3 : 4, VS = D == 64 ? 4 : 2;  // stages of K and of V
   static constexpr int KR = KT / CG, KC = D / 64;             // K rows and 64-dim chunks in this CTA
   static constexpr int VC = D / 64 / CG;                      // V chunks in this CTA (all KT rows)
@@ -105,8 +105,8 @@ struct Small {
   uint64_t q_ready, q_empty;
   uint64_t k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages];
   uint64_t k_copied[kMaxStages], v_copied[kMaxStages];  // rank 1 of a pair: its cp.async rows of the stage
-  uint64_t s_full[4], p_full[4], pv_done[4];
-  uint64_t v_here[4];       // rank 1 of a pair: [S buffer] the tile's V is in (its boxes complete on rank 0)
+  uint64_t s_full[NB], p_full[NB], pv_done[NB];
+  uint64_t v_here[NB];      // rank 1 of a pair: [S buffer] the tile's V is in (its boxes complete on rank 0)
   uint64_t o_full, o_free, mma_done;
   uint64_t ring_full[kRing], ring_empty[kRing];
   uint32_t tmem_base;
@@ -118,6 +118,7 @@ struct Small {
   int okr[2][2][4];         // the same for the rescale's wait
   int okt[2][2][4];         // [unit parity][half][row warp] whether the warp goes on to the next unit
   uint32_t pre[kMaxB + 1];  // cost of the requests before b
+  int shift;                // costs on the line are in 2^shift keys
   int qo[kMaxB + 1], kv[kMaxB + 1];
   Piece ring[kRing];           // the worker's pieces as they come, from the plan warp
   int4 slots[2][32];
@@ -127,7 +128,6 @@ struct Small {
 struct Params {
   dft_chunk_attn_args a;
   int G, TC, TQ;            // q-heads per kv-head, tokens of a query tile per CTA and in all
-  int shift;                // costs on the line are in 2^shift keys
   uint32_t inv_G;           // ceil(2^16 / G): row / G = row * inv_G >> 16 for rows below 128 and G up to 128
   float* ws_o;              // [2 workers][rows][D] partial O: slot 2c continues a unit, 2c + 1 begins one
   float* ws_ml;             // [2 workers][rows][2] partial (m, l)
@@ -140,11 +140,6 @@ constexpr uint32_t smem_bytes() {
   return Cfg<D>::OFF_SMALL + (uint32_t)sizeof(Small) + 1024;  // + alignment slack
 }
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 template <bool BF>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   uint32_t r;
@@ -183,7 +178,7 @@ __device__ __forceinline__ void warp_arrive(uint64_t& bar) {
 // min((i + 1) TQ, n) and reads the keys its last token sees, clamp(L - n + e,
 // 0, L); its cost is that + kUnitKeys, and the sum over the tiles before i is
 // an arithmetic series.  Costs on the line are those sums over 2^shift, rounded
-// down (a tile's own is the difference of two), so that the line fits 32 bits:
+// down (a tile's own is the difference of two), so that the line fits 31 bits:
 // with 64-bit divisions finding a first piece took 8000 cycles of fetching code.
 struct Req {
   int n, L, nt;
@@ -195,21 +190,25 @@ __device__ __forceinline__ Req request(const Small& sm, int b, int TQ) {
   r.nt = (int)((uint32_t)(r.n + TQ - 1) / (uint32_t)TQ);
   return r;
 }
-__device__ __forceinline__ uint32_t cost_before(const Req& r, int i, const Params& P) {
+__device__ __forceinline__ uint64_t cost_before(const Req& r, int i, int TQ, int shift) {
   uint64_t last = 0;
   if (i == r.nt && i > 0) {  // the last tile is the one that may be short
     last = (uint32_t)r.L + kUnitKeys;
     --i;
   }
   const int a = r.L - r.n;
-  const uint32_t z = a < 0 ? min((uint32_t)i, (uint32_t)-a / (uint32_t)P.TQ) : 0u;  // tiles that see no key
+  const uint32_t z = a < 0 ? min((uint32_t)i, (uint32_t)-a / (uint32_t)TQ) : 0u;  // tiles that see no key
   const uint64_t pairs = (uint64_t)(uint32_t)i * (uint32_t)(i + 1) - (uint64_t)z * (z + 1);
-  const int64_t keys = (int64_t)(i - (int)z) * a + (int64_t)(pairs >> 1) * P.TQ;
-  return (uint32_t)((last + (uint64_t)(uint32_t)i * kUnitKeys + (uint64_t)keys) >> P.shift);
+  const int64_t keys = (int64_t)(i - (int)z) * a + (int64_t)(pairs >> 1) * TQ;
+  return (last + (uint64_t)(uint32_t)i * kUnitKeys + (uint64_t)keys) >> shift;
 }
 
 // The line: offsets to shared memory, and the cost of the requests before each
 // (by one warp; lane i sums a run of requests).  Returns the line's length.
+// Up to 2^8 every tile keeps a cost of its own; 2^39 keys are half a minute of
+// work, and a longer line is refused.
+constexpr int kMaxShift = 8;
+static_assert(kUnitKeys >> kMaxShift >= 2 && kMinShare >> kMaxShift >= 1, "costs");
 __device__ __forceinline__ uint32_t plan_costs(Small& sm, const Params& P, int32_t* status) {
   const dft_chunk_attn_args& a = P.a;
   const int lane = threadIdx.x & 31, per = (a.B + 31) >> 5;
@@ -220,36 +219,50 @@ __device__ __forceinline__ uint32_t plan_costs(Small& sm, const Params& P, int32
   }
   __syncwarp();
   const int b0 = lane * per, b1 = min(a.B, b0 + per);
-  uint32_t sum = 0;
   bool bad = false;
+  int shift = 0;
+  uint64_t inc, sum, total;
 #pragma unroll 1
-  for (int b = b0; b < b1; ++b) {
-    const int q0 = sm.qo[b], q1 = sm.qo[b + 1], k0 = sm.kv[b], k1 = sm.kv[b + 1];
-    const bool ok = q0 >= 0 && q0 <= q1 && q1 <= a.T && k0 >= 0 && k0 <= k1 && k1 <= a.n_kv && k1 - k0 <= 0x7FFFFF00;
-    bad |= !ok;
-    sm.pre[b] = sum;  // so far from the lane's first
-    if (ok && q1 > q0) {
-      const Req r = request(sm, b, P.TQ);
-      sum += a.Hkv * cost_before(r, r.nt, P);
+  while (true) {
+    sum = 0;
+#pragma unroll 1
+    for (int b = b0; b < b1; ++b) {
+      const int q0 = sm.qo[b], q1 = sm.qo[b + 1], k0 = sm.kv[b], k1 = sm.kv[b + 1];
+      const bool ok = q0 >= 0 && q0 <= q1 && q1 <= a.T && k0 >= 0 && k0 <= k1 && k1 <= a.n_kv && k1 - k0 <= kMaxKeys;
+      bad |= !ok;
+      sm.pre[b] = (uint32_t)sum;  // so far from the lane's first
+      if (ok && q1 > q0) {
+        const Req r = request(sm, b, P.TQ);
+        sum += a.Hkv * cost_before(r, r.nt, P.TQ, shift);
+      }
     }
+    inc = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint64_t o = __shfl_up_sync(0xffffffffu, inc, d);
+      if (lane >= d) inc += o;
+    }
+    total = __shfl_sync(0xffffffffu, inc, 31);
+    if (total >> 31 == 0) break;
+    if (shift == kMaxShift) {
+      bad = true;
+      total = 0;
+      break;
+    }
+    shift = min(kMaxShift, shift + 33 - __clzll((long long)total));
   }
   if (bad && blockIdx.x == 0) raise_status(status, DFT_DEV_BAD_INDEX);
-  uint32_t inc = sum;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const uint32_t o = __shfl_up_sync(0xffffffffu, inc, d);
-    if (lane >= d) inc += o;
-  }
 #pragma unroll 1
-  for (int b = b0; b < b1; ++b) sm.pre[b] += inc - sum;
-  const uint32_t total = __shfl_sync(0xffffffffu, inc, 31);
-  if (lane == 0) sm.pre[a.B] = total;
+  for (int b = b0; b < b1; ++b) sm.pre[b] += (uint32_t)(inc - sum);
+  if (lane == 0) {
+    sm.pre[a.B] = (uint32_t)total;
+    sm.shift = shift;
+  }
   __syncwarp();
-  return total;
+  return (uint32_t)total;
 }
 
 // The next piece of the line from w, w < w1, that has something to do.
-template <int KT>
 __device__ __forceinline__ bool next_piece(const Small& sm, const Params& P, uint32_t& w, uint32_t w1, Piece& p) {
 #pragma unroll 1
   while (w < w1) {
@@ -269,7 +282,7 @@ __device__ __forceinline__ bool next_piece(const Small& sm, const Params& P, uin
 #pragma unroll 1
     for (int top = r.nt; top - i > 1;) {
       const int mid = (i + top) >> 1;
-      const uint32_t c = cost_before(r, mid, P);
+      const uint32_t c = (uint32_t)cost_before(r, mid, P.TQ, sm.shift);
       if (c <= rest) {
         i = mid;
         c0 = c;
@@ -283,7 +296,7 @@ __device__ __forceinline__ bool next_piece(const Small& sm, const Params& P, uin
     w += x1 - x0;
     const int keys = max(0, r.L - r.n + (int)min((int64_t)(i + 1) * P.TQ, (int64_t)r.n));
     const int nt = (keys + KT - 1) / KT;
-    const auto tile = [&](uint32_t x) { return (int)min((uint64_t)nt, (((uint64_t)x << P.shift) + KT / 2) / KT); };
+    const auto tile = [&](uint32_t x) { return (int)min((uint64_t)nt, (((uint64_t)x << sm.shift) + KT / 2) / KT); };
     p.t0 = x0 == 0 ? 0 : tile(x0);
     p.t1 = whole ? nt : tile(x1);
     if (p.t0 == p.t1 && !(nt == 0 && x0 == 0)) continue;
@@ -308,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                       const __grid_constant__ CUtensorMap v_map, const __grid_constant__ Params P, int32_t* status) {
   using F = Cfg<D>;
   constexpr bool PAIR = F::kPair;
-  constexpr int KT = F::KT, NB = F::NB, kAhead = NB - 1, CG = F::CG;
+  constexpr int CG = F::CG;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   Small& sm = *reinterpret_cast<Small*>(smem + F::OFF_SMALL);
@@ -334,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(smem_u32(&sm.v_full[i]), 32 + 1 + 2 * (CG - 1));
         mbar_init(smem_u32(&sm.v_empty[i]), 1);
       }
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < NB; ++i) {
         mbar_init(smem_u32(&sm.s_full[i]), 1);
         mbar_init(smem_u32(&sm.p_full[i]), kSoftmax / 32 * CG);
         mbar_init(smem_u32(&sm.pv_done[i]), 1);
@@ -358,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   if (PAIR) cluster_arrive();  // this CTA's barriers are up
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // inputs and workspace are the launches before's until here
+  pdl_wait();  // inputs and workspace are the launches before's until here
   const uint32_t total = warp == kPlanWarp ? plan_costs(sm, P, status) : 0u;
   if (PAIR) cluster_wait();    // the other CTA's are too, before anything arrives on them
   tc_fence_after();
@@ -397,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int T = p.t1 - p.t0;
         if (T == 0) continue;
         ok = all(wait(sm.q_ready, ui & 1, abort_flag));
-        for (int t = 0; ok && t < T + kAhead; ++t) {
+        for (int t = 0; ok && t <= T; ++t) {
           if (t < T) {
             const int gt = g + t, st = gt % F::KS, sb = gt % NB;
             bool got = wait(sm.k_full[st], (gt / F::KS) & 1, abort_flag);
@@ -418,19 +431,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             commit(sm.s_full[sb]);
             if (t == T - 1) commit(sm.q_empty);
           }
-          if (t >= kAhead) {
-            const int gu = g + t - kAhead, st = gu % F::VS, pb = gu % NB;
+          if (t > 0) {
+            const int gu = g + t - 1, st = gu % F::VS, pb = gu % NB;
             bool got = wait(sm.v_full[st], (gu / F::VS) & 1, abort_flag);
             if (PAIR && got && lead) mbar_arrive_cluster(map_rank(smem_u32(&sm.v_here[pb]), 1));
             // the first P V of a unit overwrites O: the previous unit's epilogue has read it
-            if (got && t == kAhead && ui > 0) got = wait(sm.o_free, (ui - 1) & 1, abort_flag);
+            if (got && t == 1 && ui > 0) got = wait(sm.o_free, (ui - 1) & 1, abort_flag);
             ok = all(got && wait(sm.p_full[pb], (gu / NB) & 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
             if (sm.v_mixed[st]) fence_async_smem();
             const uint32_t vb = __shfl_sync(0xffffffffu, v_base + st * F::kVBytes, 0);
             const uint32_t ps = __shfl_sync(0xffffffffu, tmem + F::COL_S + KT * pb, 0);
-            const uint32_t keep = __shfl_sync(0xffffffffu, t > kAhead ? 1u : 0u, 0);
+            const uint32_t keep = __shfl_sync(0xffffffffu, t > 1 ? 1u : 0u, 0);
             // P: 64 keys in columns 0 to 31 of its buffer, 64 in 64 to 95.
             // V [keys x dims] is MN-major: of 16 keys, 64-dim chunks 2 KB apart, 8-key groups 1 KB apart
             const uint64_t bd = sw128_desc(vb, 2048, 1024);
@@ -439,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               mma_ts<CG>(lead, tmem + F::COL_O, ps + 8 * k + (k < 4 ? 0 : 32), bd + k * F::VC * 2048 / 16, id_o, k > 0 ? 1u : keep);
             commit(sm.v_empty[st]);
             commit(sm.pv_done[pb]);
-            if (t == T + kAhead - 1) commit(sm.o_full);
+            if (t == T) commit(sm.o_full);
           }
         }
         g += T;
@@ -483,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp == kPlanWarp) {
     // ------------------------------------------ plan: the pieces, and their Q
-    const uint32_t share = max((uint32_t)kMinShare >> P.shift, (total + workers - 1) / workers);
+    const uint32_t share = max((uint32_t)kMinShare >> sm.shift, (total + workers - 1) / workers);
     uint32_t w = (uint32_t)min((uint64_t)total, (uint64_t)share * worker);
     const uint32_t w1 = (uint32_t)min((uint64_t)total, (uint64_t)w + share);
     const uint64_t pol = l2_evict_first();
@@ -495,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int i = n % kRing;
       if (n >= kRing) ok = __all_sync(0xffffffffu, wait(sm.ring_empty[i], (n / kRing - 1) & 1, abort_flag));
       if (!ok) break;
-      const bool more = next_piece<KT>(sm, P, w, w1, p);
+      const bool more = next_piece(sm, P, w, w1, p);
       if (!more) p.b = -1;
       if (lane == 0) {
         sm.ring[i] = p;
@@ -876,7 +889,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               ok = done && sm.okr[par][wg ^ 1][wq];
               if (!ok) break;
               tc_fence_after();
-              const float alpha = grow ? ex2(m_used - m_new) : 1.f;
+              const float alpha = grow ? ex2_approx(m_used - m_new) : 1.f;
 #pragma unroll 1
               for (int c = 0; c < D / 2; c += 32) {
                 float v[32];
@@ -900,7 +913,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < 16; ++i) {
               float e0, e1;
               upk2(fma2(pk2(x[c + 2 * i], x[c + 2 * i + 1]), sc2, nm2), e0, e1);
-              const float p0 = ex2(e0), p1 = ex2(e1);
+              const float p0 = ex2_approx(e0), p1 = ex2_approx(e1);
               sum2[i & 1] = add2(sum2[i & 1], pk2(p0, p1));
               pk[i] = pack2<BF>(p0, p1);
             }
@@ -941,7 +954,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 constexpr int kMergeThreads = 256, kMergeY = 8;
 template <bool BF, int D>
 __global__ void __launch_bounds__(kMergeThreads) chunk_attn_merge(const __grid_constant__ Params P) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  pdl_wait();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   constexpr int kLanes = D / 4, kPass = kMergeThreads / kLanes, kSlotRows = kRows * Cfg<D>::CG;
   __shared__ int list[kMergeThreads + 1], flags[kMergeThreads], n_list;
@@ -977,7 +990,7 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_attn_merge(const __grid_c
       const float2 ml = reinterpret_cast<const float2*>(P.ws_ml)[prow];
       const float4 v = reinterpret_cast<const float4*>(P.ws_o + prow * D)[e];
       // a sum of 0: the row sees none of these keys (a NaN sum goes on)
-      const float wgt = ml.y == 0.f ? 0.f : ex2(ml.x - M);
+      const float wgt = ml.y == 0.f ? 0.f : ex2_approx(ml.x - M);
       acc.x += wgt * v.x;
       acc.y += wgt * v.y;
       acc.z += wgt * v.z;
@@ -1009,8 +1022,8 @@ int check_args(const dft_chunk_attn_args* a) {
   if (!al16(a->q) || !al16(a->o) || !al16(a->k_cache) || !al16(a->v_cache)) return DFT_ERR_UNSUPPORTED;
   if (a->q_st % 8 || a->q_sh % 8 || a->o_st % 8 || a->o_sh % 8 || a->kv_st % 8 || a->kv_sh % 8)
     return DFT_ERR_UNSUPPORTED;
-  if (a->q_st < 0 || a->q_sh < 0 || (a->T > 1 && a->o_st < a->D) || (a->Hq > 1 && a->o_sh < a->D) ||
-      a->kv_st < a->D || (a->Hkv > 1 && a->kv_sh < a->D))
+  if ((a->T > 1 && a->q_st <= 0) || (a->Hq > 1 && a->q_sh <= 0) || a->kv_st < a->D || (a->Hkv > 1 && a->kv_sh < a->D) ||
+      !rows_apart(a->D, {a->T, a->Hq}, {a->o_st, a->o_sh}))
     return DFT_ERR_INVALID;
   if (a->kv_st >= ((int64_t)1 << 31) || a->kv_sh >= ((int64_t)1 << 38) || a->q_st >= ((int64_t)1 << 38) ||
       a->q_sh >= ((int64_t)1 << 38) || a->n_slots > 0x7FFFFFFF)
@@ -1051,8 +1064,8 @@ bool encode(CUtensorMap* m, const dft_chunk_attn_args* a, const void* base, cons
 }
 
 template <bool BF, int D>
-int launch(const Params& P, int workers, const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map, int32_t* status,
-           cudaStream_t st) {
+int launch(const Params& P, int workers, const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map,
+           int32_t* status, cudaStream_t st) {
   DFT_CUDA_CHECK(cudaFuncSetAttribute(chunk_attn_kernel<BF, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)smem_bytes<D>()));
   cudaLaunchConfig_t cfg;
@@ -1063,7 +1076,7 @@ int launch(const Params& P, int workers, const CUtensorMap& q_map, const CUtenso
   cfg.dynamicSmemBytes = smem_bytes<D>();
   cfg.stream = st;
   cfg.attrs = attr;
-  // both kernels come up under the launch before them and wait for its end
+  // like the merge, it comes up under the launch before it and waits for its end
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
@@ -1071,14 +1084,7 @@ int launch(const Params& P, int workers, const CUtensorMap& q_map, const CUtenso
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.numAttrs = Cfg<D>::kPair ? 2 : 1;
   DFT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, chunk_attn_kernel<BF, D>, q_map, k_map, v_map, P, status));
-  memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3((unsigned)workers, kMergeY);
-  cfg.blockDim = dim3(kMergeThreads);
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  DFT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, chunk_attn_merge<BF, D>, P));
-  return DFT_OK;
+  return launch_pdl(chunk_attn_merge<BF, D>, dim3((unsigned)workers, kMergeY), dim3(kMergeThreads), 0, st, P);
 }
 
 }  // namespace
@@ -1100,30 +1106,27 @@ extern "C" int dft_chunk_attn(const dft_chunk_attn_args* a, void* ws, int32_t* d
   memset(&P, 0, sizeof(P));
   P.a = *a;
   P.G = a->Hq / a->Hkv;
-  // The line's length is at most heads x (query tiles) x (keys + kUnitKeys), mostly
-  // far from it; 31 bits of it.  Up to 2^8 every tile keeps a cost of its own, and
-  // 2^40 keys' tiles are minutes of work.
-  const double line = (double)a->Hkv * ((double)a->T / (kRows / P.G) + a->B) * ((double)a->n_kv + kUnitKeys);
-  while (P.shift < 8 && line / (double)(1 << P.shift) >= 2147483647.0) ++P.shift;
-  static_assert(kUnitKeys >> 8 >= 2 && kMinShare >> 8 >= 1, "costs");
   P.inv_G = (65535u + P.G) / P.G;
   P.TC = kRows / P.G;
   P.TQ = P.TC * (a->D == 256 ? Cfg<256>::CG : 1);
   P.ws_meta = reinterpret_cast<int4*>(static_cast<char*>(ws) + w.meta);
   P.ws_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + w.ml);
   P.ws_o = reinterpret_cast<float*>(static_cast<char*>(ws) + w.o);
-  // K, V: (slots, 64-dim chunks, heads); Q: (heads, tokens, chunks)
-  const int64_t chunks = a->D / 64;
+  // K, V: (slots, 64-dim chunks, heads); Q: (heads, tokens, chunks); the stride of a
+  // dimension of one may be anything and is not looked at
+  const int64_t chunks = a->D / 64, kv_sh = a->Hkv > 1 ? a->kv_sh : a->D;
+  const int64_t q_st = a->T > 1 ? a->q_st : a->D, q_sh = a->Hq > 1 ? a->q_sh : a->D;
   const int vc = a->D == 256 ? Cfg<256>::VC : (int)chunks;
   CUtensorMap q_map, k_map, v_map;
-  if (!encode(&q_map, a, a->q, {a->Hq, a->T, chunks}, {a->q_sh, a->q_st, 64}, {P.G, P.TC, 1}) ||
-      !encode(&k_map, a, a->k_cache, {a->n_slots, chunks, a->Hkv}, {a->kv_st, 64, a->kv_sh}, {8, (int)chunks, 1}) ||
-      !encode(&v_map, a, a->v_cache, {a->n_slots, chunks, a->Hkv}, {a->kv_st, 64, a->kv_sh}, {16, vc, 1}))
+  if (!encode(&q_map, a, a->q, {a->Hq, a->T, chunks}, {q_sh, q_st, 64}, {P.G, P.TC, 1}) ||
+      !encode(&k_map, a, a->k_cache, {a->n_slots, chunks, a->Hkv}, {a->kv_st, 64, kv_sh}, {8, (int)chunks, 1}) ||
+      !encode(&v_map, a, a->v_cache, {a->n_slots, chunks, a->Hkv}, {a->kv_st, 64, kv_sh}, {16, vc, 1}))
     return DFT_ERR_UNSUPPORTED;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool bf = a->dtype == DFT_BF16;
-#define DFT_GO(D_) \
-  return bf ? launch<true, D_>(P, workers, q_map, k_map, v_map, dev_status, st) : launch<false, D_>(P, workers, q_map, k_map, v_map, dev_status, st)
+#define DFT_GO(D_)                                                               \
+  return bf ? launch<true, D_>(P, workers, q_map, k_map, v_map, dev_status, st) \
+            : launch<false, D_>(P, workers, q_map, k_map, v_map, dev_status, st)
   if (a->D == 64) DFT_GO(64);
   if (a->D == 128) DFT_GO(128);
   DFT_GO(256);

@@ -46,6 +46,25 @@ __device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float v
   }
 }
 
+// whether rows of D elements at i * s[0] + j * s[1] + .. (i < n[0], j < n[1], ..) do
+// not overlap: by rising strides, each dimension steps over all that the ones
+// before it span (a dimension of one has no stride)
+template <int K>
+inline bool rows_apart(int64_t D, const int64_t (&n)[K], const int64_t (&s)[K]) {
+  bool used[K] = {};
+  double span = (double)D;
+  for (int k = 0; k < K; ++k) {
+    int at = -1;
+    for (int i = 0; i < K; ++i)
+      if (!used[i] && n[i] > 1 && (at < 0 || s[i] < s[at])) at = i;
+    if (at < 0) break;
+    if ((double)s[at] < span) return false;
+    span += (double)(n[at] - 1) * (double)s[at];
+    used[at] = true;
+  }
+  return true;
+}
+
 inline bool valid_dtype(int d) { return d == DFT_F32 || d == DFT_BF16 || d == DFT_F16; }
 
 // Score + build scratch layout (drafter lp / ids / rest rows, then the dense

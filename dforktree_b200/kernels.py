@@ -678,6 +678,8 @@ def chunk_attention(q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, sm_sc
     written (pass o to keep what they hold).  workspace: uint8, at least
     dft_chunk_attn_workspace_bytes, for this call alone; made here if None."""
     T, Hq, D = shape = q.shape
+    if 0 in q.stride()[:2] and q.numel():
+        q = q.contiguous()      # expanded over tokens or heads
     slots, Hkv, cd = rows = k_cache.shape
     qs, cs = q.stride(), k_cache.stride()
     if rows != v_cache.shape or cd != D or v_cache.stride() != cs or qs[2] != 1 or cs[2] != 1:

@@ -81,13 +81,15 @@ class PagedKV:
     def tree(self, anc, Hq, sm_scale=None):
         """The tree-masked verify over the planned keys, whose last N per
         request are the tree's nodes: a planned TreeAttentionWrapper that reads
-        the current maps and anc [B, N, N] at every run."""
+        anc [B, N, N] and the buffers of the last plan at every run (plan later
+        steps into them: out=maps)."""
         from .tree_attn import TreeAttentionWrapper
         m = self._planned()
         B, N = anc.shape[0], anc.shape[1]
         Hkv, D = self.k_cache.shape[2:]
+        longest = self.block_table.shape[1] * self.page_size
         t = TreeAttentionWrapper(self.device).plan(m["kv_indptr"], m["kv_indices"], Hq, Hkv, D, n=N, anc=anc,
-                                                   kv_lens_host=[max(self.max_len, N)] * B, sm_scale=sm_scale)
+                                                   kv_lens_host=[max(longest, N)] * B, sm_scale=sm_scale)
         t.status = self.status
         return t
 

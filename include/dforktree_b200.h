@@ -409,7 +409,8 @@ DFT_API int dft_page_plan(const dft_page_plan_args* a, int32_t* dev_status, void
  * at or above n_slots writes nothing and sets DFT_DEV_BAD_INDEX.  Slots are
  * distinct: of a slot named twice each piece takes one of the two rows.
  * 16-bit elements (bfloat16 or float16, k / v / caches alike); head dim
- * contiguous, any other strides. */
+ * contiguous, any other strides of k and v; the caches' rows do not overlap one
+ * another (DFT_ERR_INVALID), nor k and v. */
 typedef struct {
   int64_t T;
   int32_t Hkv, D, dtype;
@@ -451,10 +452,16 @@ DFT_API int dft_kv_commit(const dft_kv_commit_args* a, int32_t* dev_status, void
  * that a token does not see do not reach its row, whatever they are.
  * q, caches and o alike bfloat16 or float16; fp32 scores, softmax and sums,
  * P rounded to the type for the second product.  D in {64, 128, 256}; G <=
- * 128; rows and strides 16-byte aligned; B <= 1024; sm_scale > 0.
- * Offsets outside [0, T] / [0, n_kv] or descending leave the request's rows
- * unwritten and set DFT_DEV_BAD_INDEX; a slot outside [0, n_slots) sets it
- * too and leaves that request's result unspecified.  o overlaps no input.
+ * 128; rows and strides 16-byte aligned, kv_st < 2^31 elements and the others
+ * < 2^38; at least one slot; B <= 1024; sm_scale > 0.
+ * Offsets outside [0, T] / [0, n_kv] or descending, and more than 2^25 keys of a
+ * request, leave the request's rows unwritten and set DFT_DEV_BAD_INDEX; a slot
+ * outside [0, n_slots) sets it too and leaves that request's result
+ * unspecified.  A call whose keys, summed over all query tiles of 128 / G tokens
+ * (256 / G for D = 256) and kv-heads, reach 2^39 sets it and writes nothing.
+ * o's rows overlap neither one another nor an input.  The kernels are launched
+ * with programmatic stream serialisation: a kernel before them in the stream
+ * may trigger its dependents early, they wait for its end all the same.
  * workspace: dft_chunk_attn_workspace_bytes bytes, 16-byte aligned (0: none),
  * used by this call alone while it runs. */
 typedef struct {

@@ -667,3 +667,132 @@ def test_the_cycle_on_paged_caches():
             hist[b] = [np.concatenate([x, _np(y[0, b])[path[b][:alen[b]]]]) for x, y in zip(hist[b], (k, v))]
         assert cyc.kv_len.tolist() == [len(h[0]) for h in hist]
     assert int(cyc.status.item()) == 0
+
+
+# ----------------------------------------------------------------- edges --
+def test_more_work_than_31_bits_of_keys():
+    """One q-head group of 128 (a token a tile): the tiles' keys sum to 2.5e9,
+    past what the schedule counts one by one."""
+    n, L = 12289, 200003
+    g = torch.Generator(device=DEV).manual_seed(5)
+    q = torch.randn(n, 128, 64, device=DEV, generator=g).to(BF)
+    k, v = (torch.randn(L, 1, 64, device=DEV, generator=g).to(BF) for _ in range(2))
+    st = _status()
+    o = _K().chunk_attention(q, k, v, _i32([0, n]), _i32([0, L]), torch.arange(L, dtype=torch.int32, device=DEV),
+                             status=st)
+    assert st.item() == 0
+    for i in (0, 1, 4095, 6000, n - 2, n - 1):           # each as the last token of a request of its own
+        end = L - n + i + 1
+        c = dict(q=q[i:i + 1], k=k[:end], v=v[:end], qo=[0, 1], kv=[0, end], idx=np.arange(end), scale=0.125)
+        _held(c, o[i:i + 1])
+
+
+def test_a_request_of_too_many_keys_is_reported():
+    n = (1 << 25) + 1
+    idx = torch.zeros(n + 9, dtype=torch.int32, device=DEV)
+    q, k = torch.randn(3, 4, 64, device=DEV).to(BF), torch.randn(8, 2, 64, device=DEV).to(BF)
+    o, st = torch.full_like(q, 5.0), _status()
+    _K().chunk_attention(q, k, k, _i32([0, 1, 3]), _i32([0, n, n + 9]), idx, o=o, status=st)
+    assert st.item() == BAD_INDEX and (o[0] == 5.0).all()
+    assert torch.equal(o[1:], k[:1].repeat_interleave(2, 1).expand(2, 4, 64))    # nine times the same key
+
+
+@pytest.mark.parametrize("D,G", [(64, 5), (128, 7), (256, 3), (256, 5), (256, 64), (256, 100), (256, 128)])
+def test_head_groups_that_do_not_divide_a_tile(D, G):
+    c = _attn_case([90, 1, 33], [150, 600, 0], 2 * G, 2, D, BF, 16)
+    st = _status()
+    o = _attend(c, st)
+    assert st.item() == 0
+    _held(c, o)
+
+
+def test_expanded_queries_and_strided_outputs():
+    c = _attn_case([6, 2], [40, 200], 8, 4, 128, BF, 16)
+    one = torch.randn(1, 8, 128, device=DEV).to(BF)
+    for q in (one.expand(8, 8, 128), one[:, :1].expand(8, 8, 128), one[:, :1].expand(1, 8, 128).expand(8, 8, 128)):
+        d = dict(c, q=q)
+        wide = torch.full((8, 8, 256), 7.0, device=DEV, dtype=BF)
+        heads_first = torch.empty(8, 8, 128, device=DEV, dtype=BF).transpose(0, 1)
+        for o in (None, wide[..., 64:192], heads_first):
+            _held(d, _attend(d, o=o))
+        assert (wide[..., :64] == 7.0).all() and (wide[..., 192:] == 7.0).all()
+
+
+def test_two_calls_at_once_with_different_inputs():
+    """Alternating on two streams, each ordered within itself only."""
+    cs = [_attn_case([1] * 30, [900 + 7 * b for b in range(30)], 16, 4, 256, BF, 16),
+          _attn_case([300, 40], [200, 1000], 16, 8, 128, HF, 16)]
+    alone = [_attend(c) for c in cs]
+    args = [(c["q"], c["k"], c["v"], _i32(c["qo"]), _i32(c["kv"]), _i32(c["idx"])) for c in cs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in cs], [[], []]
+    for _ in range(6):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(_K().chunk_attention(*args[i], sm_scale=cs[i]["scale"]))
+    torch.cuda.synchronize()
+    for a, os in zip(alone, got):
+        assert all(torch.equal(a, o) for o in os)
+
+
+def test_a_padded_batch_leaves_what_lies_behind():
+    """Fixed buffers with room for more tokens than there are: the maps' spare
+    entries write no cache row, and o keeps its rows."""
+    from dforktree_b200.paged_kv import PagedKV
+    kv = PagedKV(3, 50, 1, 2, 64, page_size=8, device=DEV)
+    out = kv.outputs(3, 40)
+    kv.plan(_i64([0, 0, 0]), _i64([17, 0, 5]), out=out)
+    k, v = (torch.randn(40, 2, 64, device=DEV).to(BF) for _ in range(2))
+    kv.append(0, k, v)
+    q, o = torch.randn(40, 4, 64, device=DEV).to(BF), torch.full((40, 4, 64), 7.0, device=DEV, dtype=BF)
+    kv.attend(0, q, o=o)
+    assert kv.device_status() == 0 and (o[22:] == 7.0).all()
+    slots = out["slot_map"][:22]
+    assert torch.equal(kv.k_cache[0][slots], k[:22]) and torch.equal(kv.v_cache[0][slots], v[:22])
+    rest = torch.ones(kv.k_cache.shape[1], dtype=torch.bool, device=DEV)
+    rest[slots] = False
+    assert (kv.k_cache[0][rest] == 0).all() and (kv.v_cache[0][rest] == 0).all()
+    c = dict(q=q, k=k, v=v, qo=[0, 17, 17, 22], kv=[0, 17, 17, 22], idx=np.arange(22), scale=0.125)
+    _held(c, o)
+
+
+def test_a_pool_that_runs_out_and_recovers():
+    from dforktree_b200.paged_kv import PagedKV
+    kv = PagedKV(3, 64, 2, 2, 64, page_size=16, n_pages=5, device=DEV)
+    zero = _i64([0, 0, 0])
+    kv.plan(zero, _i64([33, 20, 0]), tokens=60)              # three pages and two
+    k, v, q = torch.randn(60, 2, 64, device=DEV).to(BF), torch.randn(60, 2, 64, device=DEV).to(BF), torch.randn(
+        60, 4, 64, device=DEV).to(BF)
+    kv.append(0, k, v)
+    before = kv.k_cache.clone(), kv.v_cache.clone(), kv.block_table.clone(), kv.held.clone(), kv.free_pages.clone()
+    m = kv.plan(_i64([33, 20, 0]), _i64([16, 0, 1]), tokens=60)   # two more: there are none
+    assert kv.device_status() == NO_PAGES and m["qo_indptr"].tolist() == [0] * 4 and (m["slot_map"] == -1).all()
+    o = torch.full_like(q, 7.0)
+    kv.append(0, v, k)
+    kv.attend(0, q, o=o)
+    kv.commit(_i64([[0, 1]] * 3), _i64([0, 0, 0]), 1)             # no request holds a tree: reported, nothing moves
+    assert (o == 7.0).all() and kv.device_status() == NO_PAGES | BAD_INDEX
+    for a, b in zip(before, (kv.k_cache, kv.v_cache, kv.block_table, kv.held, kv.free_pages)):
+        assert torch.equal(a, b)
+    kv.status.zero_()
+    kv.plan(_i64([0, 20, 0]), _i64([0, 12, 30]), tokens=60)       # the first request ends: three pages come back
+    assert kv.device_status() == 0 and kv.held.tolist() == [0, 2, 2] and kv.n_free.item() == 1
+
+
+def test_a_tree_over_a_request_that_fills_its_last_page():
+    """max_len 40 in pages of 16: the table holds 48, and a tree may use them."""
+    from dforktree_b200.paged_kv import PagedKV
+    kv = PagedKV(1, 40, 1, 2, 256, page_size=16, device=DEV)
+    kv.plan(_i64([0]), _i64([40]), tokens=40)
+    new = torch.randn(2, 48, 2, 256, device=DEV).to(BF)
+    kv.append(0, new[0][:40], new[1][:40])
+    kv.plan(_i64([40]), _i64([8]), tokens=8)
+    kv.append(0, new[0][40:], new[1][40:])
+    anc = torch.tril(torch.ones(8, 8, dtype=torch.bool, device=DEV))[None]
+    q = torch.randn(8, 4, 256, device=DEV).to(BF)
+    o = kv.tree(anc, 4).run(q, (kv.k_cache[0], kv.v_cache[0]))
+    a = kv.attend(0, q)                                           # a chain is causal
+    assert kv.device_status() == 0
+    c = dict(q=q, k=new[0], v=new[1], qo=[0, 8], kv=[0, 48], idx=np.arange(48), scale=1 / 16)
+    _held(c, a)
+    _held(c, o.view(8, 4, 256))

@@ -170,3 +170,34 @@ def test_oracle_plan_by_hand():
     assert stack == [0, 1] and table[0].tolist() == [2, 3, -1, -1] and held.tolist() == [2, 0, 1]
     assert got[3] == [10, 11, 12] and got[4] == [2, 3, 4]
     assert OP.page_plan([3, 5], [40, 0], [2, 0], table, held, stack, 4) is None
+
+
+# rows of 64 elements, two heads, ten slots
+OVERLAPS = [dict(kv_st=0), dict(kv_sh=0), dict(kv_st=64, kv_sh=64), dict(kv_st=120, kv_sh=64), dict(kv_sh=32),
+            dict(kv_st=-128), dict(kv_sh=-64), dict(kv_st=64, kv_sh=632)]
+
+
+@pytest.mark.parametrize("kw", OVERLAPS)
+def test_append_refuses_caches_whose_rows_overlap(lib, kw):
+    assert lib.dft_kv_append(ctypes.byref(_append(**kw)), None, None) == L.DFT_ERR_INVALID
+
+
+@pytest.mark.parametrize("kw", OVERLAPS + [dict(kv_sl=0), dict(kv_sl=64), dict(kv_sl=1272), dict(kv_sl=-1280)])
+def test_commit_refuses_caches_whose_rows_overlap(lib, kw):
+    assert lib.dft_kv_commit(ctypes.byref(_commit(L=3, **kw)), None, None) == L.DFT_ERR_INVALID
+
+
+@pytest.mark.parametrize("kw", [dict(o_st=0), dict(o_sh=0), dict(o_st=64), dict(o_st=504), dict(o_sh=56),
+                                dict(o_st=-512), dict(q_st=0), dict(q_sh=0), dict(q_st=-512), dict(n_slots=0),
+                                dict(kv_st=56), dict(kv_sh=56), dict(kv_sh=-64)])
+def test_attention_refuses_strides_that_name_no_rows(lib, kw):
+    a = _attn(**kw)
+    assert lib.dft_chunk_attn_workspace_bytes(ctypes.byref(a)) == -1
+    assert lib.dft_chunk_attn(ctypes.byref(a), FAKE, None, None) == L.DFT_ERR_INVALID
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(o_st=64, o_sh=256), dict(T=1, o_st=0, q_st=0), dict(kv_st=64, kv_sh=640),
+                                dict(kv_st=256), dict(n_slots=1, kv_st=64, kv_sh=64), dict(q_st=64, q_sh=64),
+                                dict(Hq=1, Hkv=1, q_sh=0, o_sh=0, kv_sh=0)])
+def test_attention_takes_these_layouts(lib, kw):
+    assert lib.dft_chunk_attn_workspace_bytes(ctypes.byref(_attn(**kw))) > 0
