@@ -85,6 +85,7 @@ struct Cfg {
   static constexpr int VC = D / 64 / CG;                      // V chunks in this CTA (all KT rows)
   static constexpr uint32_t kKBytes = KR * KC * 128, kVBytes = KT * VC * 128;
   static constexpr uint32_t kQBytes = kRows * D * 2;
+  static constexpr int kSlotRows = kRows * CG;                // of a partial
   static constexpr uint32_t OFF_V = KS * kKBytes, OFF_Q = OFF_V + VS * kVBytes;
   static constexpr uint32_t OFF_SMALL = OFF_Q + kQBytes;
   static constexpr uint32_t COL_O = 0, COL_S = D;  // S / P buffer b at COL_S + KT b
@@ -128,8 +129,11 @@ struct Small {
 struct Params {
   dft_chunk_attn_args a;
   int G, TC, TQ;            // q-heads per kv-head, tokens of a query tile per CTA and in all
-  uint32_t inv_G;           // ceil(2^16 / G): row / G = row * inv_G >> 16 for rows below 128 and G up to 128
-  float* ws_o;              // [2 workers][rows][D] partial O: slot 2c continues a unit, 2c + 1 begins one
+  uint32_t inv_G;           // ceil(2^16 / G): row / G = row * inv_G >> 16 for rows below 256 and G up to 128
+  // Partials: slot 2c continues a unit, 2c + 1 begins one.  O by 8 dims of all
+  // rows, so that a warp, a row to a lane, stores 1 KB in one piece (by rows its
+  // 32 pieces of 16 bytes took 16000 cycles for 128 rows of 256).
+  float* ws_o;              // [2 workers][D / 8][rows][8]
   float* ws_ml;             // [2 workers][rows][2] partial (m, l)
   int4* ws_meta;            // [2 workers] (flags, first token row, tokens, kv-head); flags 1: used, 2: the unit's last
 };
@@ -703,27 +707,30 @@ __global__ void __launch_bounds__(kThreads, 1)
                                         : wait(sm.v_full[st], (gt / F::VS) & 1, abort_flag)))
         return false;
       const int live = min(KT, u.L - j0);          // rows of real keys
-      const bool scan = u.vis0 < j0 + live;        // some token does not see them all
+      // rows from here on are not seen by every token (whole 16-byte turns of the block: 32 rows)
+      const int first = max(0, min(live, u.vis0 - j0)) >> 5;
       unsigned char* vb = smem + F::OFF_V + st * F::kVBytes;
       constexpr int kTurns = KT * 8 / kSoftmax;  // 16-byte pieces of a chunk for a thread
-      bool any = false;
+      bool any = false, wrote = false;
 #pragma unroll 1
       for (int c = 0; c < F::VC; ++c) {
-        uint4 x[kTurns];
         uint32_t hit = 0;
         const auto piece = [&](int i) {
           const int at = i * kSoftmax + tid;  // row at >> 3
           return reinterpret_cast<uint4*>(vb + (at >> 7) * (F::VC * 2048) + c * 2048) + (at & 127);
         };
-#pragma unroll
-        for (int i = 0; i < kTurns; ++i) {
-          if (i * kSoftmax + tid >= live * 8) *piece(i) = make_uint4(0u, 0u, 0u, 0u);
-          x[i] = scan ? *piece(i) : make_uint4(0u, 0u, 0u, 0u);
-        }
         // a half's exponent is all ones iff adding one to it carries out
 #pragma unroll
-        for (int i = 0; i < kTurns; ++i)
-          hit |= ((x[i].x & kExp) + kOne) | ((x[i].y & kExp) + kOne) | ((x[i].z & kExp) + kOne) | ((x[i].w & kExp) + kOne);
+        for (int i = 0; i < kTurns; ++i) {
+          if (i < first) continue;
+          if (i * kSoftmax + tid >= live * 8) {
+            *piece(i) = make_uint4(0u, 0u, 0u, 0u);
+            wrote = true;
+          } else {
+            const uint4 x = *piece(i);
+            hit |= ((x.x & kExp) + kOne) | ((x.y & kExp) + kOne) | ((x.z & kExp) + kOne) | ((x.w & kExp) + kOne);
+          }
+        }
         if (hit & 0x80008000u) {
           any = true;
           const auto clean = [&](uint32_t& y) { y &= ~(((((y & kExp) + kOne) & 0x80008000u) >> 15) * 0xFFFFu); };
@@ -742,7 +749,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         *reinterpret_cast<volatile int*>(&sm.odd[ui & 7]) = ui + 1;
         if (PAIR) st_cluster(map_rank(smem_u32(&sm.odd[ui & 7]), rank ^ 1), ui + 1);
       }
-      fence_async_smem();  // these writes before the tensor core's reads
+      if (any || wrote) fence_async_smem();  // these writes before the tensor core's reads
       return true;
     };
     // Unit after unit; the next one's Q, K and S come in while the last one's output goes out.
@@ -760,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         named_bar(pair_bar, 64);
         l = sm.lsum[0][r] + sm.lsum[1][r];
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        const int64_t prow = (int64_t)(2 * worker + max(u.slot, 0)) * (kRows * CG) + (row_ok ? tok * P.G + g_ : 0);
+        const int64_t prow = (int64_t)(2 * worker + max(u.slot, 0)) * F::kSlotRows;
         // the rows of this lane's two; its 16 bytes of each 32
         unsigned char* to[2];
         bool there[2];
@@ -810,14 +817,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (there[q])
                   *reinterpret_cast<uint4*>(to[q] + c * 2) = make_uint4(y[q][0], y[q][1], y[q][2], y[q][3]);
             } else if (row_ok) {
-              float4* dst = reinterpret_cast<float4*>(P.ws_o + prow * D + (D / 2) * wg + c);
+              float* dst = P.ws_o + prow * D + ((D / 16 * wg + (c >> 3)) * F::kSlotRows + rank * kRows + r) * 8;
 #pragma unroll
-              for (int q = 0; q < 4; ++q) dst[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+              for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<float4*>(dst + (q >> 1) * (F::kSlotRows * 8) + (q & 1) * 4) =
+                    make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
             }
           }
           if (u.slot >= 0 && wg == 0 && row_ok) {
-            P.ws_ml[2 * prow] = m_used;
-            P.ws_ml[2 * prow + 1] = l;
+            *reinterpret_cast<float2*>(P.ws_ml + 2 * (prow + rank * kRows + r)) = make_float2(m_used, l);
           }
         }
         if (held) {
@@ -951,58 +959,87 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Merge the partials of the unit that worker c begins and leaves unfinished: its
 // own, then the continuing slots of the workers after it up to the unit's last.
 //   o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s
-constexpr int kMergeThreads = 256, kMergeY = 8;
+constexpr int kMergeThreads = 256, kMergeY = 8, kMaxWorkers = 160;
 template <bool BF, int D>
 __global__ void __launch_bounds__(kMergeThreads) chunk_attn_merge(const __grid_constant__ Params P) {
   pdl_wait();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  constexpr int kLanes = D / 4, kPass = kMergeThreads / kLanes, kSlotRows = kRows * Cfg<D>::CG;
-  __shared__ int list[kMergeThreads + 1], flags[kMergeThreads], n_list;
+  // a warp: 8 rows, 32 dims; a pass of the block: kPass rows
+  constexpr int kWide = D / 32, kPass = kMergeThreads / 32 / kWide * 8, kSlotRows = Cfg<D>::kSlotRows;
+  __shared__ int list[kMaxWorkers + 1];
+  __shared__ uint32_t used[kMergeThreads / 32], ends[kMergeThreads / 32];
+  __shared__ float2 mls[kMaxWorkers * kPass];
+  static_assert(kMaxWorkers <= kMergeThreads, "a thread per worker");
   const int c = blockIdx.x, grid = gridDim.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int4 meta = P.ws_meta[2 * c + 1];
+  const int flags = (int)threadIdx.x > c && (int)threadIdx.x < grid ? P.ws_meta[2 * threadIdx.x].x : 0;
   if (!(meta.x & 1)) return;
   const dft_chunk_attn_args& a = P.a;
-  const int rows = meta.z * P.G, e = threadIdx.x % kLanes;
+  const int rows = meta.z * P.G, e = warp % kWide * 4 + (lane & 3);  // rows of the unit; this thread's 8 dims
   if (blockIdx.y * kPass >= rows) return;
   // the unit's partials: slot 2c + 1, then the used even slots after it to the unit's last
-  for (int k = threadIdx.x; k < grid; k += kMergeThreads) flags[k] = P.ws_meta[2 * k].x;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    int n = 0;
-    list[n++] = 2 * c + 1;
-    for (int k = c + 1; k < grid; ++k) {
-      if (flags[k] & 1) list[n++] = 2 * k;
-      if (flags[k] & 2) break;
-    }
-    n_list = n;
+  const uint32_t u = __ballot_sync(0xffffffffu, flags & 1), l = __ballot_sync(0xffffffffu, flags & 2);
+  if (lane == 0) {
+    used[warp] = u;
+    ends[warp] = l;
   }
   __syncthreads();
-  const int n = n_list;
-  for (int r = blockIdx.y * kPass + threadIdx.x / kLanes; r < rows; r += kMergeY * kPass) {
+  int n = 1;         // partials of the unit
+  bool open = true;  // no last one so far
+#pragma unroll
+  for (int w = 0; w < kMergeThreads / 32; ++w) {
+    const uint32_t to = ends[w] ? ends[w] ^ (ends[w] - 1) : 0xFFFFFFFFu;  // up to the first last one
+    const uint32_t mine = open ? used[w] & to : 0u;
+    if (w == warp) {
+      if (mine >> lane & 1) list[n + __popc(mine & ((1u << lane) - 1))] = 2 * threadIdx.x;
+    }
+    n += __popc(mine);
+    open = open && !ends[w];
+  }
+  if (threadIdx.x == 0) list[0] = 2 * c + 1;
+  const int low = P.TC * P.G;  // a unit's first rows are one CTA's, further ones the other's
+  for (int i0 = blockIdx.y * kPass; i0 < rows; i0 += kMergeY * kPass) {
+    // all partials' (m, l) of the pass's rows at once
+    __syncthreads();
+    for (int x = threadIdx.x; x < n * kPass; x += kMergeThreads) {
+      const int i = i0 + x % kPass;
+      if (i < rows)
+        mls[x] = *reinterpret_cast<const float2*>(P.ws_ml + 2 * (list[x / kPass] * kSlotRows + (i < low ? i : kRows + i - low)));
+    }
+    __syncthreads();
+    const int rr = warp / kWide * 8 + (lane >> 2), i = i0 + rr;
+    if (i >= rows) continue;
+    const int tok = (int)(i * P.inv_G >> 16), r = i < low ? i : kRows + i - low;  // its token, its row in a slot
     float M = -INFINITY;
-#pragma unroll 4
-    for (int k = 0; k < n; ++k) M = fmaxf(M, P.ws_ml[2 * ((int64_t)list[k] * kSlotRows + r)]);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int k = 0; k < n; ++k) M = fmaxf(M, mls[k * kPass + rr].x);
+    const float* part = P.ws_o + (e * kSlotRows + r) * 8;
+    float acc[8] = {};
     float L = 0.f;
 #pragma unroll 4
     for (int k = 0; k < n; ++k) {
-      const int64_t prow = (int64_t)list[k] * kSlotRows + r;
-      const float2 ml = reinterpret_cast<const float2*>(P.ws_ml)[prow];
-      const float4 v = reinterpret_cast<const float4*>(P.ws_o + prow * D)[e];
+      const float4* v = reinterpret_cast<const float4*>(part + (int64_t)list[k] * (kSlotRows * D));
+      const float4 v0 = v[0], v1 = v[1];
+      const float2 ml = mls[k * kPass + rr];
       // a sum of 0: the row sees none of these keys (a NaN sum goes on)
       const float wgt = ml.y == 0.f ? 0.f : ex2_approx(ml.x - M);
-      acc.x += wgt * v.x;
-      acc.y += wgt * v.y;
-      acc.z += wgt * v.z;
-      acc.w += wgt * v.w;
+      acc[0] += wgt * v0.x;
+      acc[1] += wgt * v0.y;
+      acc[2] += wgt * v0.z;
+      acc[3] += wgt * v0.w;
+      acc[4] += wgt * v1.x;
+      acc[5] += wgt * v1.y;
+      acc[6] += wgt * v1.z;
+      acc[7] += wgt * v1.w;
       L += wgt * ml.y;
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
-    const int tok = r / P.G;
     unsigned char* orow = static_cast<unsigned char*>(a.o) +
-                          ((int64_t)(meta.y + tok) * a.o_st + (int64_t)(meta.w * P.G + (r - tok * P.G)) * a.o_sh) * 2;
-    reinterpret_cast<uint2*>(orow)[e] =
-        make_uint2(pack2<BF>(acc.x * inv, acc.y * inv), pack2<BF>(acc.z * inv, acc.w * inv));
+                          ((int64_t)(meta.y + tok) * a.o_st + (int64_t)(meta.w * P.G + (i - tok * P.G)) * a.o_sh) * 2;
+    reinterpret_cast<uint4*>(orow)[e] =
+        make_uint4(pack2<BF>(acc[0] * inv, acc[1] * inv), pack2<BF>(acc[2] * inv, acc[3] * inv),
+                   pack2<BF>(acc[4] * inv, acc[5] * inv), pack2<BF>(acc[6] * inv, acc[7] * inv));
   }
 }
 
@@ -1031,10 +1068,10 @@ int check_args(const dft_chunk_attn_args* a) {
   return DFT_OK;
 }
 
-// one CTA per SM; the merge keeps a flag per worker
+// one CTA per SM; the merge has room for so many partials of a unit
 int worker_count(int D) {
   const int n = gtile::sm_count() / (D == 256 ? Cfg<256>::CG : 1);
-  return n < kMergeThreads ? n : kMergeThreads;
+  return n < kMaxWorkers ? n : kMaxWorkers;
 }
 
 struct Workspace {
