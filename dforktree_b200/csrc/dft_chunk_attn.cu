@@ -707,41 +707,36 @@ __global__ void __launch_bounds__(kThreads, 1)
                                         : wait(sm.v_full[st], (gt / F::VS) & 1, abort_flag)))
         return false;
       const int live = min(KT, u.L - j0);          // rows of real keys
-      // rows from here on are not seen by every token (whole 16-byte turns of the block: 32 rows)
+      // rows from 32 first on are not seen by every token
       const int first = max(0, min(live, u.vis0 - j0)) >> 5;
       unsigned char* vb = smem + F::OFF_V + st * F::kVBytes;
-      constexpr int kTurns = KT * 8 / kSoftmax;  // 16-byte pieces of a chunk for a thread
       bool any = false, wrote = false;
+      // A thread: 16 bytes of each chunk of rows (tid >> 3) + 32 i.  Kept short: this runs
+      // once a unit, and most of its 700 to 1000 cycles are fetching code (1250 unrolled).
 #pragma unroll 1
-      for (int c = 0; c < F::VC; ++c) {
-        uint32_t hit = 0;
-        const auto piece = [&](int i) {
-          const int at = i * kSoftmax + tid;  // row at >> 3
-          return reinterpret_cast<uint4*>(vb + (at >> 7) * (F::VC * 2048) + c * 2048) + (at & 127);
-        };
-        // a half's exponent is all ones iff adding one to it carries out
+      for (int i = first; i < KT / 32; ++i) {
+        uint4* at = reinterpret_cast<uint4*>(vb + (i * 2 + (tid >> 7)) * (F::VC * 2048)) + (tid & 127);
+        if (32 * i + (tid >> 3) >= live) {
 #pragma unroll
-        for (int i = 0; i < kTurns; ++i) {
-          if (i < first) continue;
-          if (i * kSoftmax + tid >= live * 8) {
-            *piece(i) = make_uint4(0u, 0u, 0u, 0u);
-            wrote = true;
-          } else {
-            const uint4 x = *piece(i);
-            hit |= ((x.x & kExp) + kOne) | ((x.y & kExp) + kOne) | ((x.z & kExp) + kOne) | ((x.w & kExp) + kOne);
-          }
+          for (int c = 0; c < F::VC; ++c) at[c * 128] = make_uint4(0u, 0u, 0u, 0u);
+          wrote = true;
+          continue;
         }
+        uint4 x[F::VC];
+#pragma unroll
+        for (int c = 0; c < F::VC; ++c) x[c] = at[c * 128];
+        // a half's exponent is all ones iff adding one to it carries out
+        uint32_t hit = 0;
+#pragma unroll
+        for (int c = 0; c < F::VC; ++c)
+          hit |= ((x[c].x & kExp) + kOne) | ((x[c].y & kExp) + kOne) | ((x[c].z & kExp) + kOne) | ((x[c].w & kExp) + kOne);
         if (hit & 0x80008000u) {
           any = true;
-          const auto clean = [&](uint32_t& y) { y &= ~(((((y & kExp) + kOne) & 0x80008000u) >> 15) * 0xFFFFu); };
+          uint32_t* y = reinterpret_cast<uint32_t*>(at);
 #pragma unroll 1
-          for (int i = 0; i < kTurns; ++i) {
-            uint4 y = *piece(i);
-            clean(y.x);
-            clean(y.y);
-            clean(y.z);
-            clean(y.w);
-            *piece(i) = y;
+          for (int j = 0; j < F::VC * 4; ++j) {
+            uint32_t& z = y[(j >> 2) * 512 + (j & 3)];
+            z &= ~(((((z & kExp) + kOne) & 0x80008000u) >> 15) * 0xFFFFu);
           }
         }
       }
