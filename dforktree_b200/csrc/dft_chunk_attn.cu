@@ -63,12 +63,15 @@ constexpr int kCtlWarp = 8, kProdWarp0 = 9, kPlanWarp = 11;  // a producer warp 
 constexpr int kThreads = 384;     // twelve warps leave 168 registers a thread; a row of 64 scores takes most of them
 constexpr uint32_t kTmemCols = 512;
 constexpr int kMaxStages = 4, kRing = 4;
-// A unit's fixed cost in keys (query load, first tile's latency, output): with
-// 256 / 512 / 1024 a prompt of 8192 tokens at D = 128 took 456 / 416 / 430 us.
+// A unit's fixed cost in keys (query load, first tile's latency, output).  D = 256:
+// with 256 / 384 / 512 / 768 a prompt of 8192 tokens took 429 / 414 / 415 / 422 us and
+// 8 ragged single tokens on 1000 keys 17.7 / 18.5 / 18.5 / 19.8; D <= 128, whose tiles
+// are as long and whose output is half: 12 ragged prompts of D = 128 61 / 65 / 65 / 69
+// us, 16 single tokens of D = 64 on 2000 keys 23.6 / 23.7 / 24.9 / 26.0.
+constexpr int unit_keys(int D) { return D == 256 ? 512 : 256; }
 // The least share of a worker, under which a cut costs more than it spreads:
-// with 256 / 384 / 512 a single token on 4096 keys took 20 / 20 / 20.5 us and on
-// 1000 keys 13.6 / 14.7 / 15.5.
-constexpr int kUnitKeys = 512;
+// with 128 / 256 / 384 / 512 a single token on 701 keys took 12.9 / 13.3 / 14.7 / 15.5
+// us and 64 tokens on 1000 keys, whose partials are 64 KB each, 32 with 128, 28 with 256.
 constexpr int kMinShare = 256;
 
 constexpr int KT = 128;           // keys per tile
@@ -128,6 +131,7 @@ struct Small {
 
 struct Params {
   dft_chunk_attn_args a;
+  int unit_keys;            // fixed cost of a unit
   int G, TC, TQ;            // q-heads per kv-head, tokens of a query tile per CTA and in all
   uint32_t inv_G;           // ceil(2^16 / G): row / G = row * inv_G >> 16 for rows below 256 and G up to 128
   // Partials: slot 2c continues a unit, 2c + 1 begins one.  O by 8 dims of all
@@ -180,7 +184,7 @@ __device__ __forceinline__ void warp_arrive(uint64_t& bar) {
 // -------------------------------------------------------------- schedule --
 // Request b: n tokens in nt query tiles, L keys.  Tile i ends at token e =
 // min((i + 1) TQ, n) and reads the keys its last token sees, clamp(L - n + e,
-// 0, L); its cost is that + kUnitKeys, and the sum over the tiles before i is
+// 0, L); its cost is that + unit_keys, and the sum over the tiles before i is
 // an arithmetic series.  Costs on the line are those sums over 2^shift, rounded
 // down (a tile's own is the difference of two), so that the line fits 31 bits:
 // with 64-bit divisions finding a first piece took 8000 cycles of fetching code.
@@ -194,17 +198,17 @@ __device__ __forceinline__ Req request(const Small& sm, int b, int TQ) {
   r.nt = (int)((uint32_t)(r.n + TQ - 1) / (uint32_t)TQ);
   return r;
 }
-__device__ __forceinline__ uint64_t cost_before(const Req& r, int i, int TQ, int shift) {
+__device__ __forceinline__ uint64_t cost_before(const Req& r, int i, const Params& P, int shift) {
   uint64_t last = 0;
   if (i == r.nt && i > 0) {  // the last tile is the one that may be short
-    last = (uint32_t)r.L + kUnitKeys;
+    last = (uint32_t)r.L + P.unit_keys;
     --i;
   }
   const int a = r.L - r.n;
-  const uint32_t z = a < 0 ? min((uint32_t)i, (uint32_t)-a / (uint32_t)TQ) : 0u;  // tiles that see no key
+  const uint32_t z = a < 0 ? min((uint32_t)i, (uint32_t)-a / (uint32_t)P.TQ) : 0u;  // tiles that see no key
   const uint64_t pairs = (uint64_t)(uint32_t)i * (uint32_t)(i + 1) - (uint64_t)z * (z + 1);
-  const int64_t keys = (int64_t)(i - (int)z) * a + (int64_t)(pairs >> 1) * TQ;
-  return (last + (uint64_t)(uint32_t)i * kUnitKeys + (uint64_t)keys) >> shift;
+  const int64_t keys = (int64_t)(i - (int)z) * a + (int64_t)(pairs >> 1) * P.TQ;
+  return (last + (uint64_t)(uint32_t)i * P.unit_keys + (uint64_t)keys) >> shift;
 }
 
 // The line: offsets to shared memory, and the cost of the requests before each
@@ -212,7 +216,7 @@ __device__ __forceinline__ uint64_t cost_before(const Req& r, int i, int TQ, int
 // Up to 2^8 every tile keeps a cost of its own; 2^39 keys are half a minute of
 // work, and a longer line is refused.
 constexpr int kMaxShift = 8;
-static_assert(kUnitKeys >> kMaxShift >= 2 && kMinShare >> kMaxShift >= 1, "costs");
+static_assert(unit_keys(64) >> kMaxShift >= 1 && unit_keys(256) >> kMaxShift >= 1 && kMinShare >> kMaxShift >= 1, "costs");
 __device__ __forceinline__ uint32_t plan_costs(Small& sm, const Params& P, int32_t* status) {
   const dft_chunk_attn_args& a = P.a;
   const int lane = threadIdx.x & 31, per = (a.B + 31) >> 5;
@@ -237,7 +241,7 @@ __device__ __forceinline__ uint32_t plan_costs(Small& sm, const Params& P, int32
       sm.pre[b] = (uint32_t)sum;  // so far from the lane's first
       if (ok && q1 > q0) {
         const Req r = request(sm, b, P.TQ);
-        sum += a.Hkv * cost_before(r, r.nt, P.TQ, shift);
+        sum += a.Hkv * cost_before(r, r.nt, P, shift);
       }
     }
     inc = sum;
@@ -286,7 +290,7 @@ __device__ __forceinline__ bool next_piece(const Small& sm, const Params& P, uin
 #pragma unroll 1
     for (int top = r.nt; top - i > 1;) {
       const int mid = (i + top) >> 1;
-      const uint32_t c = (uint32_t)cost_before(r, mid, P.TQ, sm.shift);
+      const uint32_t c = (uint32_t)cost_before(r, mid, P, sm.shift);
       if (c <= rest) {
         i = mid;
         c0 = c;
@@ -1137,6 +1141,7 @@ extern "C" int dft_chunk_attn(const dft_chunk_attn_args* a, void* ws, int32_t* d
   Params P;
   memset(&P, 0, sizeof(P));
   P.a = *a;
+  P.unit_keys = unit_keys(a->D);
   P.G = a->Hq / a->Hkv;
   P.inv_G = (65535u + P.G) / P.G;
   P.TC = kRows / P.G;
