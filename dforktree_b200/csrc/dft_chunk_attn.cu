@@ -863,10 +863,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld32_async(ts + 32, &x[32]);
           tmem_ld_wait(x);
           if (!plain) {
-            const int seen = vis - j0 - 64 * wg;  // columns that the row sees
+            const int seen = max(0, min(64, vis - j0 - 64 * wg));  // columns that the row sees
+            const uint32_t off[2] = {seen >= 32 ? 0u : 0xFFFFFFFFu << seen, seen >= 64 ? 0u : 0xFFFFFFFFu << max(0, seen - 32)};
 #pragma unroll
             for (int i = 0; i < 64; ++i)
-              if (i >= seen) x[i] = -INFINITY;
+              if (off[i >> 5] >> (i & 31) & 1) x[i] = -INFINITY;
           }
           float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
