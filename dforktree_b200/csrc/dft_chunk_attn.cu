@@ -325,8 +325,9 @@ __device__ __forceinline__ bool next_piece(const Small& sm, const Params& P, uin
 
 template <bool BF, int D>
 __global__ void __launch_bounds__(kThreads, 1)
-    chunk_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
-                      const __grid_constant__ CUtensorMap v_map, const __grid_constant__ Params P, int32_t* status) {
+    chunk_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap q1_map,
+                      const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                      const __grid_constant__ Params P, int32_t* status) {
   using F = Cfg<D>;
   constexpr bool PAIR = F::kPair;
   constexpr int CG = F::CG;
@@ -376,6 +377,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (PAIR) tmem_alloc_2(smem_u32(&sm.tmem_base), kTmemCols);
     else tmem_alloc(smem_u32(&sm.tmem_base), kTmemCols);
   }
+  for (uint32_t i = tid * 16; i < F::kQBytes; i += kThreads * 16)
+    *reinterpret_cast<uint4*>(smem + F::OFF_Q + i) = make_uint4(0u, 0u, 0u, 0u);
+  fence_async_smem();
   tc_fence_before();
   __syncthreads();
   if (PAIR) cluster_arrive();  // this CTA's barriers are up
@@ -524,17 +528,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!more) break;
       if (p.t1 == p.t0) continue;
-      // its Q, a box of tokens x G heads per 64 dims, once the piece before has no S
-      // MMA left; rows past the piece's tokens hold what follows and are nobody's
+      // Its Q, a box of tokens x G heads per 64 dims, once the piece before has no S
+      // MMA left; rows past the piece's tokens hold what follows and are nobody's.  A
+      // single token's box is its own: 64 KB of rows that are nobody's are not read,
+      // and zeros in them (from the start, while units are single tokens) leave the
+      // tensor core little to switch.
       if (ui > 0) ok = __all_sync(0xffffffffu, wait(sm.q_empty, (ui - 1) & 1, abort_flag));
       if (!ok) break;
       const uint32_t bar = PAIR ? map_rank(smem_u32(&sm.q_ready), 0) : smem_u32(&sm.q_ready);
-      if (lane == 0) mbar_expect_tx_cluster<PAIR>(bar, P.TC * P.G * D * 2);
+      const bool one = p.ntok == 1;
+      const int rows = one ? (rank ? 0 : P.G) : P.TC * P.G;
+      if (lane == 0) mbar_expect_tx_cluster<PAIR>(bar, rows * D * 2);
       __syncwarp();
+      if (rows > 0) {
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c)
-        tma_load_4d<CG>(lead, smem_u32(smem) + F::OFF_Q + c * (kRows * 128), &q_map, 0, p.h * P.G,
-                        p.tok0 + rank * P.TC, c, bar, pol);
+        for (int c = 0; c < D / 64; ++c)
+          tma_load_4d<CG>(lead, smem_u32(smem) + F::OFF_Q + c * (kRows * 128), one ? &q1_map : &q_map, 0, p.h * P.G,
+                          p.tok0 + rank * P.TC, c, bar, pol);
+      }
       ++ui;
     }
     if (!ok && lane == 0 && !*abort_flag) set_abort(sm, status);
@@ -1101,8 +1112,8 @@ bool encode(CUtensorMap* m, const dft_chunk_attn_args* a, const void* base, cons
 }
 
 template <bool BF, int D>
-int launch(const Params& P, int workers, const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map,
-           int32_t* status, cudaStream_t st) {
+int launch(const Params& P, int workers, const CUtensorMap& q_map, const CUtensorMap& q1_map, const CUtensorMap& k_map,
+           const CUtensorMap& v_map, int32_t* status, cudaStream_t st) {
   DFT_CUDA_CHECK(cudaFuncSetAttribute(chunk_attn_kernel<BF, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)smem_bytes<D>()));
   cudaLaunchConfig_t cfg;
@@ -1120,7 +1131,7 @@ int launch(const Params& P, int workers, const CUtensorMap& q_map, const CUtenso
   attr[1].val.clusterDim.x = 2;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.numAttrs = Cfg<D>::kPair ? 2 : 1;
-  DFT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, chunk_attn_kernel<BF, D>, q_map, k_map, v_map, P, status));
+  DFT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, chunk_attn_kernel<BF, D>, q_map, q1_map, k_map, v_map, P, status));
   return launch_pdl(chunk_attn_merge<BF, D>, dim3((unsigned)workers, kMergeY), dim3(kMergeThreads), 0, st, P);
 }
 
@@ -1155,16 +1166,17 @@ extern "C" int dft_chunk_attn(const dft_chunk_attn_args* a, void* ws, int32_t* d
   const int64_t chunks = a->D / 64, kv_sh = a->Hkv > 1 ? a->kv_sh : a->D;
   const int64_t q_st = a->T > 1 ? a->q_st : a->D, q_sh = a->Hq > 1 ? a->q_sh : a->D;
   const int vc = a->D == 256 ? Cfg<256>::VC : (int)chunks;
-  CUtensorMap q_map, k_map, v_map;
+  CUtensorMap q_map, q1_map, k_map, v_map;
   if (!encode(&q_map, a, a->q, {a->Hq, a->T, chunks}, {q_sh, q_st, 64}, {P.G, P.TC, 1}) ||
+      !encode(&q1_map, a, a->q, {a->Hq, a->T, chunks}, {q_sh, q_st, 64}, {P.G, 1, 1}) ||
       !encode(&k_map, a, a->k_cache, {a->n_slots, chunks, a->Hkv}, {a->kv_st, 64, kv_sh}, {8, (int)chunks, 1}) ||
       !encode(&v_map, a, a->v_cache, {a->n_slots, chunks, a->Hkv}, {a->kv_st, 64, kv_sh}, {16, vc, 1}))
     return DFT_ERR_UNSUPPORTED;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool bf = a->dtype == DFT_BF16;
-#define DFT_GO(D_)                                                               \
-  return bf ? launch<true, D_>(P, workers, q_map, k_map, v_map, dev_status, st) \
-            : launch<false, D_>(P, workers, q_map, k_map, v_map, dev_status, st)
+#define DFT_GO(D_)                                                                       \
+  return bf ? launch<true, D_>(P, workers, q_map, q1_map, k_map, v_map, dev_status, st) \
+            : launch<false, D_>(P, workers, q_map, q1_map, k_map, v_map, dev_status, st)
   if (a->D == 64) DFT_GO(64);
   if (a->D == 128) DFT_GO(128);
   DFT_GO(256);
