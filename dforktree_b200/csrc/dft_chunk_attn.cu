@@ -14,9 +14,9 @@
 // keys, one pass with a running maximum and sum:
 //   K, V  by slot, 16 keys at a time, into separate rings of stages by one
 //         producer warp each: where the 16 slots are consecutive (pages of 16 and
-//         more) one TMA box of 16 cache rows x 64 dims per copy, else 16-byte
-//         cp.async row by row (a gather of four rows per TMA copy took 39 ns a
-//         copy, 5 us per 64 KB)
+//         more) TMA boxes of 8 (K) or 16 (V) cache rows by 64-dim chunks, else
+//         16-byte cp.async row by row (a gather of four rows per TMA copy took
+//         39 ns a copy, 5 us per 64 KB)
 //   S     = Q K^T    kind::f16, fp32 in TMEM; Q from shared memory, where one TMA
 //         box of tokens x G heads per 64 dims puts it while the unit before ends
 //   P     = 2^(S sm_scale log2e - m), two threads per row; the reference m moves
@@ -40,6 +40,12 @@
 // V's rows past the request's end and its non-finite elements before the P V
 // product reads them; the epilogue adds such an element back to the rows that
 // do see its key.
+//
+// Measured (bf16, 16 q-heads, 4 kv-heads of 256): a prompt of 8192 tokens 402 to 450
+// us, 1.2 to 1.4 PFLOP/s, bound by the tensor cores under the power cap; 64 single
+// tokens on up to 4097 keys 125 us, 5.3 TB/s, bound by the stages' turnover (two of K
+// and two of V, held by MMAs of 256 rows); 512 tokens on 33280 keys in single-token
+// pages 265 us, 1.0 PFLOP/s, bound by the row copies; one token on 701 keys 13.4 us.
 //
 // Every wait is bounded (~1 s); on timeout the CTA raises DFT_DEV_TIMEOUT,
 // drains its copies and MMAs (bounded), frees TMEM and exits.
