@@ -486,11 +486,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       // once they are in.  K and V run apart, so it waits for neither alone; it
       // arrives for every tile, so a stage is not reused before and its parity
       // keeps its meaning.
+      // It takes a piece only when it owes no arrival: piece n + 1 comes once the S
+      // of piece n - 1 are done, and those need every K and V up to there.  What it
+      // owes for pieces up to n needs nothing of n + 1 (producers, Q and MMAs of a
+      // piece wait for earlier tiles alone), so the waits form no cycle; and no time
+      // goes, since the last V of n is read before the first K of n + 1.
       int end = 0, next[2] = {0, 0};  // tiles known of, and the next of K and of V
       bool ok = true, more = true;
       long long t0 = clock64();
       while (ok && (more || next[0] < end || next[1] < end)) {
-        if (more && max(next[0], next[1]) == end) {
+        if (more && next[0] == end && next[1] == end) {
           more = take(p);
           ok = p.b != -2;
           if (more) end += p.t1 - p.t0;

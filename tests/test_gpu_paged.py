@@ -796,3 +796,46 @@ def test_a_tree_over_a_request_that_fills_its_last_page():
     c = dict(q=q, k=new[0], v=new[1], qo=[0, 8], kv=[0, 48], idx=np.arange(48), scale=1 / 16)
     _held(c, a)
     _held(c, o.view(8, 4, 256))
+
+
+# ------------------------------------- short units beside long ones, row copies --
+def _in_runs(c, share, seed):
+    """c's key slots once more: of each request's blocks of 16 keys a share lies in
+    consecutive slots and the rest anywhere among that rest's slots."""
+    rng = np.random.default_rng(seed)
+    idx = np.arange(len(c["idx"]))
+    loose = [j for a, b in zip(c["kv"][:-1], c["kv"][1:]) for j0 in range(a, b, 16) if rng.random() >= share
+             for j in range(j0, min(j0 + 16, b))]
+    idx[loose] = rng.permutation(idx[loose])
+    return dict(c, idx=idx)
+
+
+@pytest.mark.parametrize("lens", [
+    [2000, 30], [2000, 30, 30], [30, 2000, 64, 1, 65], [1, 64, 65, 128, 129, 3000], [3000, 129, 128, 65, 64, 1],
+    [1500] + [40] * 20 + [1500] + [100] * 20, [64, 2500] * 12, [128, 1, 900] * 16, [200, 33] * 40, [700] * 40 + [5] * 90,
+    [4000] + [7] * 63,
+], ids=lambda x: f"{len(x)}-{x[0]}-{x[-1]}")
+@pytest.mark.parametrize("slots", ["page1", "page4", "page8", "page16", "runs"])
+def test_short_requests_beside_long_ones(lens, slots):
+    """Single tokens whose units are one tile or many, in every order of the two:
+    the pair form hands K and V of a tile over on their own times."""
+    page = int(slots[4:]) if slots != "runs" else 1
+    c = _attn_case([1] * len(lens), [n - 1 for n in lens], 16, 4, 256, BF, page, seed=len(slots))
+    for seed in range(1 if slots != "runs" else 3):
+        d = _in_runs(c, (0.2, 0.5, 0.8)[seed], seed) if slots == "runs" else c
+        st = _status()
+        o = _attend(d, st)
+        assert st.item() == 0
+        _held(d, o)
+
+
+@pytest.mark.parametrize("page", [1, 16])
+def test_many_one_tile_units_of_a_pair(page):
+    rng = np.random.default_rng(page)
+    for fresh, cached in (([1] * 300, rng.integers(0, 128, 300)), ([1] * 300, rng.integers(60, 256, 300)),
+                          (rng.integers(0, 6, 200), rng.integers(0, 200, 200))):
+        c = _attn_case([int(x) for x in fresh], [int(x) for x in cached], 8, 4, 256, HF, page)
+        st = _status()
+        o = _attend(c, st)
+        assert st.item() == 0
+        _held(c, o)
