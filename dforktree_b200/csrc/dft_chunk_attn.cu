@@ -933,7 +933,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             m_used = m_new;
           }
           // a row whose scores so far are all -inf has no reference yet: its P is 0
-          const float nm = (m_used == -INFINITY && !plain) ? 0.f : kBias - m_used;
+          const float nm = m_used == -INFINITY ? 0.f : kBias - m_used;
           const f32x2 sc2 = pk2(sc, sc), nm2 = pk2(nm, nm);
           f32x2 sum2[2] = {pk2(0.f, 0.f), pk2(0.f, 0.f)};
 #pragma unroll

@@ -446,8 +446,9 @@ DFT_API int dft_kv_commit(const dft_kv_commit_args* a, int32_t* dev_status, void
  * keys kv_indices[kv_indptr[b] .. kv_indptr[b+1]), L of them, the new tokens'
  * own last: for token i of the n and q-head hq
  *   o = softmax_j(q . k[j, hq/G] * sm_scale) . v[j, hq/G] over j <= L - n + i
- * with G = Hq / Hkv.  A token that sees no key (L < n) gets 0; rows of q
- * outside every request are left as they were in o.  Every length is read on
+ * with G = Hq / Hkv.  A token that sees no key (L < n), and a row whose every
+ * score is -infinity, get 0; rows of q outside every request are left as they
+ * were in o.  Every length is read on
  * the device, so a captured call follows its plan's buffers.  Values at keys
  * that a token does not see do not reach its row, whatever they are.
  * q, caches and o alike bfloat16 or float16; fp32 scores, softmax and sums,

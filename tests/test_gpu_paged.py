@@ -839,3 +839,34 @@ def test_many_one_tile_units_of_a_pair(page):
         o = _attend(c, st)
         assert st.item() == 0
         _held(c, o)
+
+
+# ------------------------------------------------------ scores of -infinity --
+@pytest.mark.parametrize("fresh,dead", [(1, (0, 128)), (1, (0, 500)), (1, (300, 600)), (40, (0, 256)), (40, (130, 520)),
+                                        (3, (5, 9))])
+@pytest.mark.parametrize("D,dtype", [(256, BF), (128, HF), (64, BF)])
+def test_keys_whose_scores_are_minus_infinity_weigh_nothing(D, dtype, fresh, dead):
+    """K of -infinity in a dim where q is positive, over whole tiles or parts of
+    them: the rows are those of the other keys."""
+    c = _attn_case([fresh, 2], [700, 90], 8, 2, D, dtype, 16, seed=9)
+    q, k = c["q"].clone(), c["k"].clone()
+    q[:, :, 0] = q[:, :, 0].abs() + 0.5
+    gone = c["idx"][dead[0]:dead[1]]
+    k[torch.from_numpy(gone).to(DEV), :, 0] = -float("inf")
+    st = _status()
+    o = _attend(dict(c, q=q, k=k), st)
+    assert st.item() == 0
+    n = dead[1] - dead[0]
+    _held(dict(c, q=q, idx=np.delete(c["idx"], slice(*dead)), kv=c["kv"] - n * (np.arange(3) > 0)), o)
+
+
+@pytest.mark.parametrize("D,dtype", [(256, BF), (128, HF), (64, BF)])
+def test_a_row_of_scores_of_minus_infinity_alone_is_zero(D, dtype):
+    for cached in (20, 127, 128, 900):
+        c = _attn_case([2, 1], [cached, 50], 8, 2, D, dtype, 16, seed=cached)
+        q, k = c["q"].clone(), c["k"].clone()
+        q[:, :, 0] = q[:, :, 0].abs() + 0.5
+        k[torch.from_numpy(c["idx"][:cached + 2]).to(DEV), :, 0] = -float("inf")
+        o = _attend(dict(c, q=q, k=k))
+        assert (o[:2] == 0).all()
+        _held(dict(c, q=q), o, rows=slice(2, 3))
