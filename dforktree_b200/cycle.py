@@ -208,8 +208,17 @@ class DraftTreeCycle:
                           aux_g=self.aux_g[l], aux_k_per_v=False, status=self.status)
 
     def accept(self, target):
+        """Greedy acceptance.  Where the step's page plan could not be made (paged
+        caches: a request past max_len, or no free pages) nothing is accepted:
+        accept_len 0, path, last and bonus -1, so that commit() leaves the
+        recurrent and conv states where the KV caches stay."""
         K.accept_greedy(self.tree["tokens"], self.tree["nxt"], self.tree["sib"], target, self.cfg.P,
                         status=self.status, out=(self.path, self.accept_len, self.last, self.bonus))
+        if self.cfg.attn_layers and self.cfg.page_size:
+            none = self._planned_tokens(self.tree_maps) == 0
+            self.accept_len.masked_fill_(none, 0)
+            for t in (self.path, self.last, self.bonus):
+                t.masked_fill_(none.view(-1, *[1] * (t.dim() - 1)), -1)
 
     def commit(self, x=None):
         """Closed-form state commit of every layer; with the cycle's pre-conv

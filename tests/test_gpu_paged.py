@@ -870,3 +870,52 @@ def test_a_row_of_scores_of_minus_infinity_alone_is_zero(D, dtype):
         o = _attend(dict(c, q=q, k=k))
         assert (o[:2] == 0).all()
         _held(dict(c, q=q), o, rows=slice(2, 3))
+
+
+# ------------------------------------------------------------- paged cycle --
+def _small_cycle(**kw):
+    from dforktree_b200 import synth
+    from dforktree_b200.cycle import CycleConfig, DraftTreeCycle
+    from dforktree_b200.ngram_gpu import load_npz_arrays
+    V = 2048
+    cfg = CycleConfig(**{**dict(B=3, V=V, N=16, layers=3, Hk=2, Hv=4, attn_layers=1, Hq=8, Hkv=2, Da=256, prefix=64,
+                                P=8, page_size=16, max_len=64), **kw})
+    table = _K().Table(load_npz_arrays(synth.make_ngram_table(V, 20000, 60000, seed=1)), beta3=60.0)
+    return DraftTreeCycle(cfg, table, DEV)
+
+
+def test_a_step_whose_plan_cannot_be_made_moves_no_state():
+    """One request's tree does not fit max_len: recurrent, conv and KV state of
+    every request stay, nothing counts as accepted, and the step after it is
+    that of a cycle which never met it."""
+    from dforktree_b200.workload import cycle_inputs, path_target
+    g = torch.Generator(device=DEV).manual_seed(6)
+    q, k, v = (torch.randn(1, 90, h, 256, device=DEV, generator=g).to(BF) for h in (8, 2, 2))
+    kt, vt = (torch.randn(1, 3, 16, 2, 256, device=DEV, generator=g).to(BF) for _ in range(2))
+    got = []
+    for early in (True, False):
+        cyc = _small_cycle()
+        cyc.extend(_i64([50, 10, 30]), q, k, v)
+        inp = cycle_inputs(cyc.cfg, DEV, seed=70)
+
+        def step():
+            cyc.step(inp["logits"], inp["root"], inp["pre1"], inp["x"], inp["a"], inp["b"],
+                     lambda tree: path_target(tree, inp["acc_len"]), inp["q"], kt, vt)
+
+        if early:
+            names = ("pool", "conv_state", "kv_len")
+            before = [getattr(cyc, n).clone() for n in names] + [cyc.kv.k_cache.clone(), cyc.kv.v_cache.clone()]
+            step()                                   # 50 + 16 tokens: past max_len
+            assert int(cyc.status.item()) == BAD_INDEX
+            for a, b in zip(before, [getattr(cyc, n) for n in names] + [cyc.kv.k_cache, cyc.kv.v_cache]):
+                assert torch.equal(a, b)
+            assert cyc.accept_len.tolist() == [0, 0, 0] and (cyc.path == -1).all()
+            assert (cyc.last == -1).all() and (cyc.bonus == -1).all()
+            cyc.status.zero_()
+        cyc.kv_len[0] = 20                           # the long request is cut back
+        step()
+        assert int(cyc.status.item()) == 0 and (cyc.accept_len > 0).all()
+        assert cyc.kv_len.tolist() == [n + a for n, a in zip((20, 10, 30), cyc.accept_len.clamp(max=8).tolist())]
+        got.append([x.clone() for x in (cyc.pool, cyc.conv_state, cyc.kv.k_cache, cyc.kv.v_cache, cyc.o_attn, cyc.path,
+                                        cyc.last, cyc.bonus)])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
