@@ -211,11 +211,16 @@ class DraftTreeCycle:
         """Greedy acceptance.  Where the step's page plan could not be made (paged
         caches: a request past max_len, or no free pages) nothing is accepted:
         accept_len 0, path, last and bonus -1, so that commit() leaves the
-        recurrent and conv states where the KV caches stay."""
+        recurrent and conv states where the KV caches stay.  With paged caches an
+        accepted path also ends at its P-th node, the last that commit() can move:
+        accept_len, last and bonus follow (the nodes cut off are drafted again)."""
         K.accept_greedy(self.tree["tokens"], self.tree["nxt"], self.tree["sib"], target, self.cfg.P,
                         status=self.status, out=(self.path, self.accept_len, self.last, self.bonus))
         if self.cfg.attn_layers and self.cfg.page_size:
-            none = self._planned_tokens(self.tree_maps) == 0
+            none, over = self._planned_tokens(self.tree_maps) == 0, self.accept_len > self.cfg.P
+            self.last.copy_(torch.where(over, self.path[:, -1], self.last))
+            self.bonus.copy_(target.reshape(self.tree["tokens"].shape).gather(1, self.last.view(-1, 1)).view(-1))
+            self.accept_len.clamp_(max=self.cfg.P)
             self.accept_len.masked_fill_(none, 0)
             for t in (self.path, self.last, self.bonus):
                 t.masked_fill_(none.view(-1, *[1] * (t.dim() - 1)), -1)

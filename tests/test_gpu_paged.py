@@ -919,3 +919,34 @@ def test_a_step_whose_plan_cannot_be_made_moves_no_state():
         got.append([x.clone() for x in (cyc.pool, cyc.conv_state, cyc.kv.k_cache, cyc.kv.v_cache, cyc.o_attn, cyc.path,
                                         cyc.last, cyc.bonus)])
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_an_accepted_path_longer_than_the_rows_kept_ends_there():
+    """P below the tree's depth: what counts as accepted is what every state holds,
+    as in a cycle with room whose target agrees with the first P nodes only."""
+    from dforktree_b200.workload import cycle_inputs
+    g = torch.Generator(device=DEV).manual_seed(7)
+    q, k, v = (torch.randn(1, 90, h, 256, device=DEV, generator=g).to(BF) for h in (8, 2, 2))
+    kt, vt = (torch.randn(1, 3, 16, 2, 256, device=DEV, generator=g).to(BF) for _ in range(2))
+    got, deepest = [], []
+    for P in (3, 16):
+        cyc = _small_cycle(P=P, max_len=128, chain_first=True)
+        cyc.extend(_i64([50, 10, 30]), q, k, v)
+        inp = cycle_inputs(cyc.cfg, DEV, seed=70)
+
+        def target(tree):
+            # every node agrees with its first child; past the third node of a path only where P has room
+            nxt = tree["nxt"].view(3, 16)
+            t = torch.where(nxt >= 0, tree["tokens"].view(3, 16).gather(1, nxt.clamp(min=0)), -7)
+            depth = tree["anc"].view(3, 16, 16).sum(-1)
+            deepest.append(depth.max().item())
+            return t if P == 3 else torch.where(depth >= 3, t + 10 ** 6, t)
+
+        cyc.step(inp["logits"], inp["root"], inp["pre1"], inp["x"], inp["a"], inp["b"], target, inp["q"], kt, vt)
+        assert int(cyc.status.item()) == 0 and cyc.accept_len.tolist() == [3, 3, 3]
+        assert cyc.kv_len.tolist() == [53, 13, 33] and (cyc.path[:, :3] >= 0).all()
+        got.append([x.clone() for x in (cyc.pool, cyc.conv_state, cyc.path[:, :3], cyc.last,
+                                        cyc.bonus + (10 ** 6 if P == 3 else 0))])
+        got[-1] += [cyc.kv.k_cache[0][cyc.tree_maps["slot_map"].view(3, 16)[:, :3]],
+                    cyc.kv.v_cache[0][cyc.tree_maps["slot_map"].view(3, 16)[:, :3]]]
+    assert min(deepest) > 4 and all(torch.equal(a, b) for a, b in zip(*got))
