@@ -81,15 +81,21 @@ class PagedKV:
     def tree(self, anc, Hq, sm_scale=None):
         """The tree-masked verify over the planned keys, whose last N per
         request are the tree's nodes: a planned TreeAttentionWrapper that reads
-        anc [B, N, N] and the buffers of the last plan at every run (plan later
-        steps into them: out=maps)."""
+        anc [B, N, N] (float32, or converted at every run) and the buffers of the
+        last plan at every run (plan later steps into them: out=maps)."""
         from .tree_attn import TreeAttentionWrapper
         m = self._planned()
-        B, N = anc.shape[0], anc.shape[1]
+        B = m["qo_indptr"].numel() - 1
+        if anc.dim() != 3 or anc.shape[0] != B or anc.shape[1] != anc.shape[2]:
+            raise L.DFTError("PagedKV.tree: anc is [B, N, N] for the planned B requests")
+        if anc.device != m["qo_indptr"].device:
+            raise L.DFTError(f"PagedKV.tree: anc is read at every run and must be on {m['qo_indptr'].device}")
+        N = anc.shape[1]
         Hkv, D = self.k_cache.shape[2:]
         longest = self.block_table.shape[1] * self.page_size
         t = TreeAttentionWrapper(self.device).plan(m["kv_indptr"], m["kv_indices"], Hq, Hkv, D, n=N, anc=anc,
-                                                   kv_lens_host=[max(longest, N)] * B, sm_scale=sm_scale)
+                                                   kv_lens_host=[max(longest, N)] * B, sm_scale=sm_scale,
+                                                   live_anc=True)
         t.status = self.status
         return t
 

@@ -32,11 +32,13 @@ class TreeAttentionWrapper:
         self._plan = None
 
     def plan(self, kv_indptr, kv_indices, num_qo_heads, num_kv_heads, head_dim, n, anc=None, custom_mask=None,
-             kv_lens_host=None, page_size=1, sm_scale=None):
+             kv_lens_host=None, page_size=1, sm_scale=None, live_anc=False):
         """kv_indptr [B + 1] / kv_indices: each request's key slots (prefix
         first, then its n tree tokens in node order).  kv_lens_host: host list
         of per-request key counts (the plan's HOST_KV_LEN); read from
-        kv_indptr, with a sync, when omitted."""
+        kv_indptr, with a sync, when omitted.  An anc that is not contiguous
+        float32 is converted here; with live_anc at every run, which then reads
+        what it holds by that time."""
         if page_size != 1:
             raise L.DFTError("tree attention plans page size 1 (fc1_plan.py:23)")
         B = kv_indptr.numel() - 1
@@ -57,7 +59,8 @@ class TreeAttentionWrapper:
         self._plan = dict(B=B, n=n, Hq=num_qo_heads, Hkv=num_kv_heads, D=head_dim,
                           kv_indptr=kv_indptr.to(device=self.device, dtype=torch.int32).contiguous(),
                           kv_indices=kv_indices.to(device=self.device, dtype=torch.int32).contiguous(),
-                          anc=anc.reshape(B, n, n).to(device=self.device, dtype=torch.float32).contiguous(),
+                          anc=anc if live_anc else
+                          anc.reshape(B, n, n).to(device=self.device, dtype=torch.float32).contiguous(),
                           max_kv_len=max(kv_lens_host), sm_scale=sm_scale)
         return self
 

@@ -950,3 +950,67 @@ def test_an_accepted_path_longer_than_the_rows_kept_ends_there():
         got[-1] += [cyc.kv.k_cache[0][cyc.tree_maps["slot_map"].view(3, 16)[:, :3]],
                     cyc.kv.v_cache[0][cyc.tree_maps["slot_map"].view(3, 16)[:, :3]]]
     assert min(deepest) > 4 and all(torch.equal(a, b) for a, b in zip(*got))
+
+
+# ------------------------------------------------- one tree wrapper, many steps --
+@pytest.mark.parametrize("kind", ["float32", "bool", "half", "strided"])
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_tree_wrapper_follows_its_ancestor_matrix(kind, captured):
+    """One tree() for several steps: the matrix and the maps change in place."""
+    from dforktree_b200 import synth
+    from dforktree_b200.paged_kv import PagedKV
+    Hq, Hkv, D, N = 8, 2, 256, 16
+    rng, g = np.random.default_rng(3), torch.Generator(device=DEV).manual_seed(3)
+    kv = PagedKV(2, 200, 1, Hkv, D, page_size=16, device=DEV)
+    maps, cached, fresh = kv.outputs(2, 2 * N), _i64([0, 0]), _i64([N, N])
+    anc = {"float32": lambda: torch.zeros(2, N, N, device=DEV), "half": lambda: torch.zeros(2, N, N, device=DEV, dtype=HF),
+           "bool": lambda: torch.zeros(2, N, N, device=DEV, dtype=torch.bool),
+           "strided": lambda: torch.zeros(N, N, 2, device=DEV).permute(2, 0, 1)}[kind]()
+    q, o = torch.zeros(2, N, Hq, D, device=DEV, dtype=BF), torch.zeros(2, N, Hq, D, device=DEV, dtype=BF)
+    k, v = (torch.zeros(2 * N, Hkv, D, device=DEV, dtype=BF) for _ in range(2))
+    kv.plan(cached, fresh, out=maps)
+    tree = kv.tree(anc, Hq)
+
+    def body():
+        kv.plan(cached, fresh, out=maps)
+        kv.append(0, k, v)
+        tree.run(q, (kv.k_cache[0], kv.v_cache[0]), out=o)
+
+    if captured:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            body()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            body()
+    hist = [[np.zeros((0, Hkv, D))] * 2 for _ in range(2)]
+    for step in range(3):
+        want = np.stack([OB.tree_struct(synth.random_tree_parents(N, rng), 4)[0] for _ in range(2)])
+        anc.copy_(torch.from_numpy(want).to(DEV))
+        for t in (q, k, v):
+            t.copy_(torch.randn(t.shape, device=DEV, generator=g))
+        graph.replay() if captured else body()
+        for b in range(2):
+            rows = [_np(x[b * N:(b + 1) * N]) for x in (k, v)]
+            kk, vv = (np.concatenate([x, y]) for x, y in zip(hist[b], rows))
+            n0 = len(hist[b][0])
+            for n in range(N):
+                see = np.concatenate([np.arange(n0), n0 + np.nonzero(want[b][n] > 0.5)[0]])
+                r, bound = OP.chunk_attention(_np(q[b, n:n + 1]), kk, vv, [0, 1], [0, len(see)], see, D ** -0.5, 2.0 ** -8)
+                assert (np.abs(_np(o[b, n]) - r[0]) <= bound[0]).all(), (step, b, n)
+            hist[b] = [x[:n0 + 5] for x in (kk, vv)]      # the first five nodes stay
+        cached += 5
+    assert kv.device_status() == 0
+
+
+def test_a_tree_refuses_matrices_that_it_cannot_read_at_every_run():
+    from dforktree_b200 import _lib as L
+    from dforktree_b200.paged_kv import PagedKV
+    kv = PagedKV(2, 64, 1, 2, 256, page_size=16, device=DEV)
+    kv.plan(_i64([0, 0]), _i64([8, 8]), tokens=16)
+    for anc in (torch.zeros(2, 8, 8), torch.zeros(1, 8, 8, device=DEV), torch.zeros(2, 8, 9, device=DEV),
+                torch.zeros(2, 64, device=DEV)):
+        with pytest.raises(L.DFTError):
+            kv.tree(anc, 8)
