@@ -160,6 +160,9 @@ class DraftTreeCycle:
         c = self.cfg
         if not c.page_size or not c.attn_layers:
             raise K.L.DFTError("extend needs attention layers and page_size > 0")
+        T, La = q.shape[1] if q.dim() == 4 else -1, c.attn_layers
+        if q.shape != (La, T, c.Hq, c.Da) or not k.shape == v.shape == (La, T, c.Hkv, c.Da) or fresh.numel() != c.B:
+            raise K.L.DFTError("extend: fresh [B], q [La, T, Hq, Da], k and v [La, T, Hkv, Da]")
         o = torch.zeros_like(q, memory_format=torch.contiguous_format)
         self.kv.plan(self.kv_len, fresh, tokens=q.shape[1])
         for j in range(c.attn_layers):
@@ -183,6 +186,8 @@ class DraftTreeCycle:
         fc1_branch64.py:39); output in self.o_attn.  Paged caches take the
         tree's k, v [B, N, Hkv, Da] first."""
         if self.cfg.page_size:
+            if k is None or v is None:
+                raise K.L.DFTError("attend_layer: paged caches take the tree's k and v [B, N, Hkv, Da]")
             self.kv.append(j, k.flatten(0, 1), v.flatten(0, 1))
             return self.attn.run(q, (self.kv.k_cache[j], self.kv.v_cache[j]), out=self.o_attn)
         return self.attn.run(q, (self.k_cache[j], self.v_cache[j]), out=self.o_attn)
@@ -239,12 +244,24 @@ class DraftTreeCycle:
             self.kv.commit(self.path, self.accept_len, c.N)
             self.kv_len += torch.minimum(self.accept_len.clamp(max=c.P), self._planned_tokens(self.tree_maps))
 
+    def _check_attention(self, q, k, v):
+        """A paged step's q, k and v, before anything is built or planned."""
+        c = self.cfg
+        if not (c.attn_layers and c.page_size):
+            return
+        if q is None or k is None or v is None:
+            raise K.L.DFTError("a step over paged caches takes q, and the tree's k and v")
+        q_shape, kv_shape = (c.attn_layers, c.B, c.N, c.Hq, c.Da), (c.attn_layers, c.B, c.N, c.Hkv, c.Da)
+        if q.shape not in (q_shape, (c.attn_layers, c.B * c.N, c.Hq, c.Da)) or not k.shape == v.shape == kv_shape:
+            raise K.L.DFTError("a step over paged caches takes q [La, B, N, Hq, Da], k and v [La, B, N, Hkv, Da]")
+
     def verify(self, x, a, b, q=None, k=None, v=None):
         """Every layer in model order: tree conv + GDN verify per GDN layer
         (each launch overlapping the previous layer's tail), tree attention
         per attention layer (q [La, B, N, Hq, Da]; with paged caches also the
         tree tokens' k, v [La, B, N, Hkv, Da])."""
         l = j = 0
+        self._check_attention(q, k, v)
         if self.cfg.attn_layers and self.cfg.page_size:
             self.plan_tree()
         for kind in self.cfg.layer_kinds:
@@ -260,6 +277,7 @@ class DraftTreeCycle:
         when the cycle has attention layers, and k, v [La, B, N, Hkv, Da] when
         their caches are paged; target_fn(tree) -> the target model's token
         per node [B, N] (int64)."""
+        self._check_attention(q, k, v)
         self.build(logits, root, pre1)
         self.verify(x, a, b, q, k, v)
         self.accept(target_fn(self.tree))

@@ -1014,3 +1014,30 @@ def test_a_tree_refuses_matrices_that_it_cannot_read_at_every_run():
                 torch.zeros(2, 64, device=DEV)):
         with pytest.raises(L.DFTError):
             kv.tree(anc, 8)
+
+
+def test_a_paged_step_checks_its_tensors_before_it_plans():
+    from dforktree_b200 import _lib as L
+    from dforktree_b200.workload import cycle_inputs, path_target
+    g = torch.Generator(device=DEV).manual_seed(6)
+    q, k, v = (torch.randn(1, 60, h, 256, device=DEV, generator=g).to(BF) for h in (8, 2, 2))
+    kt, vt = (torch.randn(1, 3, 16, 2, 256, device=DEV, generator=g).to(BF) for _ in range(2))
+    cyc = _small_cycle(max_len=128)
+    cyc.extend(_i64([20, 10, 30]), q, k, v)
+    inp = cycle_inputs(cyc.cfg, DEV, seed=70)
+    held, tokens = cyc.kv.held.clone(), cyc.tree["tokens"].clone()
+    for bad in (dict(k=None), dict(v=None), dict(k=None, v=None), dict(q=None), dict(k=kt[:, :2]), dict(v=vt[:0]),
+                dict(q=inp["q"][:, :, :8]), dict(k=kt[..., :128], v=vt[..., :128])):
+        a = {**dict(q=inp["q"], k=kt, v=vt), **bad}
+        with pytest.raises(L.DFTError):
+            cyc.step(inp["logits"], inp["root"], inp["pre1"], inp["x"], inp["a"], inp["b"],
+                     lambda tree: path_target(tree, inp["acc_len"]), **a)
+        with pytest.raises(L.DFTError):
+            cyc.verify(inp["x"], inp["a"], inp["b"], **a)
+    with pytest.raises(L.DFTError):
+        cyc.attend_layer(0, inp["q"][0])
+    for bad in (dict(k=k[:, :59]), dict(v=v[:, :, :1]), dict(q=q[0]), dict(q=q[:, :, :4]), dict(fresh=_i64([1, 2]))):
+        with pytest.raises(L.DFTError):
+            cyc.extend(**{**dict(fresh=_i64([1, 1, 1]), q=q, k=k, v=v), **bad})
+    assert torch.equal(held, cyc.kv.held) and torch.equal(tokens, cyc.tree["tokens"])
+    assert cyc.kv_len.tolist() == [20, 10, 30] and int(cyc.status.item()) == 0
