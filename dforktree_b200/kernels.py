@@ -548,6 +548,19 @@ def _ids(t, dtype):
     return t if t.dtype is dtype and t.is_contiguous() else t.to(dtype).contiguous()
 
 
+def _offsets(t):
+    """int32 offsets; what 32 bits do not hold becomes -1, which every kernel reports."""
+    if t.dtype is not torch.int32:
+        t = t.to(torch.int64)
+        t = torch.where((t >= 0) & (t < 2 ** 31), t, -1)
+    return _ids(t, torch.int32)
+
+
+def _slots(t):
+    """int32 cache slots; what 32 bits do not hold stays outside any cache."""
+    return _ids(t if t.dtype is torch.int32 else t.to(torch.int64).clamp(-1, 2 ** 31 - 1), torch.int32)
+
+
 _HALF = {torch.bfloat16: L.DFT_BF16, torch.float16: L.DFT_F16}
 
 
@@ -650,7 +663,7 @@ def kv_commit(k_cache, v_cache, kv_indptr, kv_indices, path, accept_len, N, stat
     if dtype is None or v_cache.dtype is not k_cache.dtype or (D > 1 and cs[3] != 1):
         raise L.DFTError("kv_commit: the caches must be alike bfloat16 or float16, their head dim contiguous")
     cur = _on_current_device("kv_commit", k_cache, v_cache, kv_indptr, kv_indices, path, accept_len, status)
-    kv_indptr, kv_indices = _ids(kv_indptr, torch.int32), _ids(kv_indices, torch.int32)
+    kv_indptr, kv_indices = _offsets(kv_indptr), _slots(kv_indices)
     path, accept_len = _ids(path, torch.int64), _ids(accept_len, torch.int64)
     _KV_COMMIT((Ln, B, int(N), P, Hkv, D, dtype, k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2], slots,
                 kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(), path.data_ptr(),
@@ -700,8 +713,7 @@ def chunk_attention(q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, sm_sc
         raise L.DFTError("chunk_attention: qo_indptr and kv_indptr hold B + 1 offsets each")
     cur = _on_current_device("chunk_attention", q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, o, workspace,
                              status)
-    qo_indptr, kv_indptr = _ids(qo_indptr, torch.int32), _ids(kv_indptr, torch.int32)
-    kv_indices = _ids(kv_indices, torch.int32)
+    qo_indptr, kv_indptr, kv_indices = _offsets(qo_indptr), _offsets(kv_indptr), _slots(kv_indices)
     need = _CHUNK_ATTN_BYTES.get((cur, D)) or _chunk_attn_bytes(cur, D)
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)

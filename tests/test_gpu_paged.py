@@ -1041,3 +1041,34 @@ def test_a_paged_step_checks_its_tensors_before_it_plans():
             cyc.extend(**{**dict(fresh=_i64([1, 1, 1]), q=q, k=k, v=v), **bad})
     assert torch.equal(held, cyc.kv.held) and torch.equal(tokens, cyc.tree["tokens"])
     assert cyc.kv_len.tolist() == [20, 10, 30] and int(cyc.status.item()) == 0
+
+
+# ------------------------------------------------ int64 offsets and slots --
+def test_int64_offsets_and_slots():
+    """Taken as they are; values past 32 bits are reported, not wrapped."""
+    c = _attn_case([4, 5], [30, 20], 8, 2, 128, BF, 1)
+    call = lambda qo, kv, idx, o, st: _K().chunk_attention(c["q"], c["k"], c["v"], _i64(qo), _i64(kv), _i64(idx),
+                                                           sm_scale=c["scale"], o=o, status=st)
+    qo, kv, idx = (x.tolist() for x in (c["qo"], c["kv"], c["idx"]))
+    st, clean = _status(), torch.empty_like(c["q"])
+    call(qo, kv, idx, clean, st)
+    assert st.item() == 0
+    _held(c, clean)
+    big = 2 ** 32
+    for bad in (dict(qo=[0, 4, 9 + big]), dict(kv=[0, 34, 59 + big]), dict(idx=idx[:40] + [idx[40] + big] + idx[41:]),
+                dict(idx=idx[:40] + [idx[40] - big] + idx[41:])):
+        a = {**dict(qo=qo, kv=kv, idx=idx), **bad}
+        st, o = _status(), torch.full_like(clean, 5.0)
+        call(a["qo"], a["kv"], a["idx"], o, st)
+        assert st.item() == BAD_INDEX and torch.equal(o[:4], clean[:4])
+        assert "idx" in bad or (o[4:] == 5.0).all()
+    kc, vc = (torch.randn(20, 2, 64, device=DEV).to(BF) for _ in range(2))
+    k0, v0 = kc.clone(), vc.clone()
+    tree = [3, 1, 4, 2]
+    for kv, idx in (([0, 4 + big], tree), ([0, 4], [3, 1 + big, 4, 2]), ([0, 4], [3, 1, 4, 2 - big])):
+        st = _status()
+        _K().kv_commit(kc, vc, _i64(kv), _i64(idx), _i64([[0, 2, 3]]), _i64([3]), 4, status=st)
+        assert st.item() == BAD_INDEX and torch.equal(kc, k0) and torch.equal(vc, v0)
+    st = _status()
+    _K().kv_commit(kc, vc, _i64([0, 4]), _i64(tree), _i64([[0, 2, 3]]), _i64([3]), 4, status=st)
+    assert st.item() == 0 and torch.equal(kc[tree[:3]], k0[[3, 4, 2]]) and torch.equal(vc[tree[:3]], v0[[3, 4, 2]])

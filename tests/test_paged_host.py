@@ -201,3 +201,13 @@ def test_attention_refuses_strides_that_name_no_rows(lib, kw):
                                 dict(Hq=1, Hkv=1, q_sh=0, o_sh=0, kv_sh=0)])
 def test_attention_takes_these_layouts(lib, kw):
     assert lib.dft_chunk_attn_workspace_bytes(ctypes.byref(_attn(**kw))) > 0
+
+
+def test_wide_offsets_and_slots_do_not_wrap():
+    wide = torch.tensor([0, 7, 2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 7, 2 ** 62, -1, -2 ** 32, -2 ** 40 + 3])
+    assert K._offsets(wide).tolist() == [0, 7, 2 ** 31 - 1] + [-1] * 7
+    assert K._slots(wide).tolist() == [0, 7] + [2 ** 31 - 1] * 5 + [-1] * 3
+    for f in (K._offsets, K._slots):
+        same = torch.tensor([3, -5], dtype=torch.int32)
+        assert f(same) is same and f(wide).dtype is f(wide[::2]).dtype is torch.int32
+        assert f(torch.tensor([3, 4], dtype=torch.int16)).tolist() == [3, 4]
