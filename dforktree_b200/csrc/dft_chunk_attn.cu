@@ -82,6 +82,7 @@ constexpr int kMinShare = 256;
 
 constexpr int KT = 128;           // keys per tile
 constexpr int NB = 2;             // S / P buffers
+constexpr float kLog2e = 1.4426950408889634f;
 template <int N>
 using Int = std::integral_constant<int, N>;
 
@@ -699,7 +700,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int rt = (int)(r * P.inv_G >> 16), g_ = r - rt * P.G;  // the row's token in the CTA, and its head
     const int tok = rt < P.TC ? rank * P.TC + rt : 1 << 20;      // in the piece; rows past the last token are spare
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const float sc = a.sm_scale * 1.4426950408889634f;
+    const float sc = a.sm_scale * kLog2e;
     // a partial slot that no piece of this CTA fills is marked so
     int slots_used = 0;
     // A row's two warps meet at the same named barriers in the same order; every
@@ -1072,7 +1073,7 @@ int check_args(const dft_chunk_attn_args* a) {
   if (!a || a->B < 0 || a->T < 0 || a->Hq <= 0 || a->Hkv <= 0 || a->Hq % a->Hkv || a->n_slots < 0 || a->n_kv < 0)
     return DFT_ERR_INVALID;
   if (a->dtype != DFT_BF16 && a->dtype != DFT_F16) return DFT_ERR_INVALID;
-  if (!(a->sm_scale > 0.f) || a->sm_scale > 3e38f) return DFT_ERR_INVALID;
+  if (!(a->sm_scale > 0.f) || !(a->sm_scale * kLog2e < INFINITY)) return DFT_ERR_INVALID;  // the kernel scales by both
   if ((a->D != 64 && a->D != 128 && a->D != 256) || a->Hq / a->Hkv > 128 || a->B > kMaxB) return DFT_ERR_UNSUPPORTED;
   if (a->B == 0 || a->T == 0) return DFT_OK;
   if (!a->q || !a->o || !a->qo_indptr || !a->kv_indptr || !a->k_cache || !a->v_cache || a->n_slots < 1 ||

@@ -454,7 +454,8 @@ DFT_API int dft_kv_commit(const dft_kv_commit_args* a, int32_t* dev_status, void
  * q, caches and o alike bfloat16 or float16; fp32 scores, softmax and sums,
  * P rounded to the type for the second product.  D in {64, 128, 256}; G <=
  * 128; rows and strides 16-byte aligned, kv_st < 2^31 elements and the others
- * < 2^38; at least one slot; B <= 1024; sm_scale > 0.
+ * < 2^38; at least one slot; B <= 1024; sm_scale > 0 and sm_scale * log2(e)
+ * finite.
  * Offsets outside [0, T] / [0, n_kv] or descending, and more than 2^25 keys of a
  * request, leave the request's rows unwritten and set DFT_DEV_BAD_INDEX; a slot
  * outside [0, n_slots) sets it too and leaves that request's result

@@ -211,3 +211,9 @@ def test_wide_offsets_and_slots_do_not_wrap():
         same = torch.tensor([3, -5], dtype=torch.int32)
         assert f(same) is same and f(wide).dtype is f(wide[::2]).dtype is torch.int32
         assert f(torch.tensor([3, 4], dtype=torch.int16)).tolist() == [3, 4]
+
+
+def test_attention_refuses_scales_that_overflow_with_log2_e(lib):
+    for scale, rc in ((2.36e38, 1), (2.9e38, 1), (3.4e38, 1), (2.35e38, 0), (1e-38, 0)):
+        a = _attn(sm_scale=scale)
+        assert (lib.dft_chunk_attn_workspace_bytes(ctypes.byref(a)) == -1) == (rc == 1), scale
