@@ -202,7 +202,7 @@ __device__ __forceinline__ Req request(const Small& sm, int b, int TQ) {
   Req r;
   r.n = sm.qo[b + 1] - sm.qo[b];
   r.L = sm.kv[b + 1] - sm.kv[b];
-  r.nt = (int)((uint32_t)(r.n + TQ - 1) / (uint32_t)TQ);
+  r.nt = (int)(((uint32_t)r.n + (uint32_t)TQ - 1) / (uint32_t)TQ);  // n + TQ may pass 2^31
   return r;
 }
 __device__ __forceinline__ uint64_t cost_before(const Req& r, int i, const Params& P, int shift) {
