@@ -47,8 +47,9 @@
 // and two of V, held by MMAs of 256 rows); 512 tokens on 33280 keys in single-token
 // pages 265 us, 1.0 PFLOP/s, bound by the row copies; one token on 701 keys 13.4 us.
 //
-// Every wait is bounded (~1 s); on timeout the CTA raises DFT_DEV_TIMEOUT,
-// drains its copies and MMAs (bounded), frees TMEM and exits.
+// Every wait is bounded (~1 s); on timeout the CTA raises DFT_DEV_TIMEOUT (its
+// pair gives up with it), waits (bounded) for its MMAs and for every copy that was
+// issued, frees TMEM and exits.
 #include "dft_common.cuh"
 #include "dft_gdn_tile.cuh"
 #include "dft_tc.cuh"
@@ -121,7 +122,8 @@ struct Small {
   uint64_t o_full, o_free, mma_done;
   uint64_t ring_full[kRing], ring_empty[kRing];
   uint32_t tmem_base;
-  int abort;
+  int abort;                // of both CTAs of a pair
+  int sent[3], relayed[2];  // after the roles' end: tiles of K, of V and pieces' Q issued; tiles of K, V relayed
   int odd[8];               // [piece & 7] = piece + 1 when one of its masked tiles held a non-finite value
   float xmax[2][2][kRows];  // [tile parity][half][row] tile max exchange between a row's two threads
   float lsum[2][kRows];     // [half][row] final row sums
@@ -167,8 +169,10 @@ __device__ __forceinline__ float unpack(uint16_t v) {
   return BF ? __uint_as_float((uint32_t)v << 16) : __half2float(__ushort_as_half(v));
 }
 
-__device__ __forceinline__ void set_abort(Small& sm, int32_t* status) {
+template <bool PAIR>
+__device__ __forceinline__ void set_abort(Small& sm, int rank, int32_t* status) {
   *reinterpret_cast<volatile int*>(&sm.abort) = 1;
+  if (PAIR) st_cluster(map_rank(smem_u32(&sm.abort), rank ^ 1), 1);
   raise_status(status, DFT_DEV_TIMEOUT);
 }
 
@@ -478,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++ui;
       }
       ok = ok && p.b != -2;
-      if (!ok && lane == 0 && !*abort_flag) set_abort(sm, status);
+      if (!ok && lane == 0 && !*abort_flag) set_abort<PAIR>(sm, rank, status);
       // every MMA issued above has retired before TMEM is freed
       commit(sm.mma_done);
     } else {
@@ -514,7 +518,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         ok = ok && __all_sync(0xffffffffu, !*abort_flag && clock64() - t0 < 2000000000ll);
       }
-      if (!ok && lane == 0 && !*abort_flag) set_abort(sm, status);
+      if (lane == 0) {
+        sm.relayed[0] = next[0];
+        sm.relayed[1] = next[1];
+      }
+      if (!ok && lane == 0 && !*abort_flag) set_abort<PAIR>(sm, rank, status);
     }
     if (lane == 0 && !mbar_wait(smem_u32(&sm.mma_done), 0)) raise_status(status, DFT_DEV_TIMEOUT);
     __syncwarp();
@@ -560,7 +568,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       ++ui;
     }
-    if (!ok && lane == 0 && !*abort_flag) set_abort(sm, status);
+    if (lane == 0) sm.sent[2] = ui;
+    if (!ok && lane == 0 && !*abort_flag) set_abort<PAIR>(sm, rank, status);
   } else if (warp >= kProdWarp0) {
     // ------------------------------------------- producers: paged K/V tiles
     // A dependent instruction costs a lone warp 4 to 6 cycles, so what a tile
@@ -681,12 +690,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok) g += T;
       }
       ok = ok && p.b != -2;
-      if (!ok && lane == 0 && !*abort_flag) set_abort(sm, status);
-      // The last copies land before the block's shared memory goes, whatever
-      // became of their readers (rank 0's barriers take rank 1's boxes too).
+      if (!ok && lane == 0 && !*abort_flag) set_abort<PAIR>(sm, rank, status);
+      if (lane == 0) sm.sent[V] = g;
       cp_async_wait_all();
-      if (rank == 0)
-        for (int gt = max(0, g - kStages); gt < g; ++gt) mbar_wait(smem_u32(&full[gt % kStages]), (gt / kStages) & 1);
     };
     if (warp == kProdWarp0) produce(Int<0>());
     else produce(Int<1>());
@@ -967,11 +973,38 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid == 0 && rank == 0)
       for (int s = 0; s < 2; ++s)
         if (!(slots_used >> s & 1)) P.ws_meta[2 * worker + s] = make_int4(0, 0, 0, 0);
-    if (!ok && !*abort_flag) set_abort(sm, status);
+    if (!ok && !*abort_flag) set_abort<PAIR>(sm, rank, status);
   }
   tc_fence_before();
   __syncthreads();
   if (PAIR) cluster_sync();  // nothing of the other CTA's arrives here any more
+  if (*abort_flag) {
+    // A wait gave up (in both CTAs of a pair, or neither): MMAs may not have taken
+    // all copies, and those must land before their shared memory goes.  No role runs
+    // any more, so a phase that lacks arrivals gets them here and is waited for; its
+    // transactions, rank 1's among them, are all on rank 0's barriers.  Every phase
+    // before the ones below is complete: their stages were handed out again.
+    if (rank == 0 && tid == 0) {
+      const auto other = [&](int& x) { return PAIR ? (int)ld_cluster(map_rank(smem_u32(&x), 1)) : x; };
+      const auto settle = [&](uint64_t& bar, int missing, int phase) {
+        for (int i = 0; i < missing; ++i) mbar_arrive(smem_u32(&bar));
+        mbar_wait(smem_u32(&bar), phase & 1);
+      };
+      const int q0 = sm.sent[2], q1 = other(sm.sent[2]), nq = max(q0, q1);
+      if (nq > 0) settle(sm.q_ready, (q0 < nq) + (q1 < nq), nq - 1);
+#pragma unroll 1
+      for (int v = 0; v < 2; ++v) {
+        const int n = v ? F::VS : F::KS, g0 = sm.sent[v], g1 = other(sm.sent[v]);
+        const int relayed = PAIR ? other(sm.relayed[v]) : 0, g = max(g0, g1);
+#pragma unroll 1
+        for (int gt = max(0, g - n); gt < g; ++gt)
+          settle((v ? sm.v_full : sm.k_full)[gt % n], (gt < g0 ? 0 : 32 + 1) + (PAIR ? (gt >= g1) + (gt >= relayed) : 0),
+                 gt / n);
+      }
+    }
+    __syncwarp();
+    if (PAIR) cluster_sync();  // rank 1's shared memory stays until then
+  }
   if (warp == kCtlWarp) {
     tc_fence_after();
     if (PAIR) tmem_dealloc_2(tmem, kTmemCols);

@@ -348,6 +348,11 @@ __device__ __forceinline__ void mbar_expect_tx_cluster(uint32_t bar, uint32_t by
 __device__ __forceinline__ void st_cluster(uint32_t cluster_addr, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;\n\tfence.acq_rel.cluster;" ::"r"(cluster_addr), "r"(v) : "memory");
 }
+__device__ __forceinline__ uint32_t ld_cluster(uint32_t cluster_addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
 // Issued by the lane with `lead` set (elect_lane), in code that the whole warp
 // runs: descriptors then stay in uniform registers.  Under a branch of one lane
 // they went through vector registers, 72 to 150 cycles an MMA.
