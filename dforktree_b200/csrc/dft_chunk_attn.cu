@@ -41,11 +41,14 @@
 // product reads them; the epilogue adds such an element back to the rows that
 // do see its key.
 //
-// Measured (bf16, 16 q-heads, 4 kv-heads of 256): a prompt of 8192 tokens 402 to 450
-// us, 1.2 to 1.4 PFLOP/s, bound by the tensor cores under the power cap; 64 single
-// tokens on up to 4097 keys 125 us, 5.3 TB/s, bound by the stages' turnover (two of K
-// and two of V, held by MMAs of 256 rows); 512 tokens on 33280 keys in single-token
-// pages 265 us, 1.0 PFLOP/s, bound by the row copies; one token on 701 keys 13.4 us.
+// Measured (bf16, 16 q-heads, 4 kv-heads of 256), in captured graphs of a few ms and,
+// in brackets, call by call on changing inputs: a prompt of 8192 tokens 398 to 450 us,
+// 1.2 to 1.4 PFLOP/s (468 us, 1.2), bound by the tensor cores under the power cap; 64
+// single tokens on up to 4097 keys 122 us, 5.4 TB/s (145 us, 4.6), bound by the stages'
+// turnover (two of K and two of V, held by MMAs of 256 rows); 512 tokens on 33280 keys in
+// single-token pages 260 us, 1.1 PFLOP/s (307 us, 0.90), bound by the row copies' issue
+// and latency (L2 18 % busy; in pages of 16 a shorter such chunk takes 0.8 of the time);
+// one token on 701 keys 13.5 us (15.1).
 //
 // Every wait is bounded (~1 s); on timeout the CTA raises DFT_DEV_TIMEOUT (its
 // pair gives up with it), waits (bounded) for its MMAs and for every copy that was

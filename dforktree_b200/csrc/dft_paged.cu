@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 // One CTA per (request, layer).  A thread owns columns of the row; it reads
 // the path's rows eight at a time before it writes them: path ascends, so
 // path[i] >= i and a later read never meets an earlier write.  Bound by the
-// chain offsets -> path -> slots -> rows, about 4 us; 64 requests of 16 layers
+// chain offsets -> path -> slots -> rows, about 4 us; 64 requests of 8 layers
 // (50 MB) 9.5 us.
 constexpr int kCommitThreads = 256;
 constexpr int kBatch = 8;

@@ -82,7 +82,9 @@ class PagedKV:
         """The tree-masked verify over the planned keys, whose last N per
         request are the tree's nodes: a planned TreeAttentionWrapper that reads
         anc [B, N, N] (float32, or converted at every run) and the buffers of the
-        last plan at every run (plan later steps into them: out=maps)."""
+        last plan at every run (plan later steps into them: out=maps).  How a
+        request's keys are split follows the table's width, max_len, since the
+        host knows no lengths."""
         from .tree_attn import TreeAttentionWrapper
         m = self._planned()
         B = m["qo_indptr"].numel() - 1
